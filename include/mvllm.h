@@ -947,6 +947,59 @@ int mv_layernorm_residual(const float* y1, int64_t ld1, const float* r1, const f
 int mv_layernorm_gather(const float* x, int64_t ldx, const int32_t* idx, const float* w, float eps, void* out,
                         int64_t ldo, int rows, int n, int f32, mv_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * A step that verifies drafted tokens over the paged cache (csrc/tree_ops.hip, tree_attn.hip).  No counterpart in the
+ * reference, whose decode step is one token a row.
+ *
+ * Row b (a sequence) has ctx_lens[b] cached tokens and brings nodes row_start[b] .. row_start[b + 1] - 1 of the step's
+ * tokens (at most max_nodes; the rest is left alone).  Node i continues the earlier node parents[.] of its row (anything
+ * else: none; parents == NULL: the node in front of it).  It lies in the cache at index ctx_lens[b] + i of the sequence, at position
+ * ctx_lens[b] + its depth.  A mask has `words` 64-bit words per token: bit i % 64 of word i / 64 is node i of the row.  Trees and
+ * masks go up to 256 nodes a row.  No two rows may share a page that nodes lie in.
+ * ------------------------------------------------------------------------------------------------ */
+
+/* Pages, slots, positions, rows and ancestor masks of a step.  block_table [rows, bt_cols] (row stride bt_stride) in place: the columns
+ * that the nodes open behind those of the cached tokens get free_pages [n_free] in row order.  taken [rows] = pages a row took; -1: the
+ * free ones did not last up to this row, or it has no columns for them - it takes none and its slots are -1.  slots [tokens] = page *
+ * page size + place (-1 also where the page is not in [0, num_pages)), positions, row_of [tokens]; mask [tokens, words] (NULL:
+ * none) = the node and its ancestors.  Without parents and mask rows may be of any length.  page * num_pages < 2^31. */
+int mv_tree_plan(const int32_t* ctx_lens, const int32_t* row_start, const int32_t* parents, int32_t* block_table, int64_t bt_stride,
+                 int bt_cols, const int32_t* free_pages, int n_free, int rows, int tokens, int max_nodes, int page, int num_pages,
+                 int32_t* slots, int32_t* positions, int32_t* row_of, uint64_t* mask, int words, int32_t* taken, mv_stream_t stream);
+
+/* qkv [tokens, ld] = q [heads * d] | k [kv_heads * d] | v [kv_heads * d], bf16 or (src_f32) fp32.  Every head of q and of k: RMS norm over
+ * itself (q_norm / k_norm fp32 [d]; NULL: none), then the rotation of its first `rot` dimensions by positions[t] * inv_freq[i] (fp64
+ * [rot / 2]; adjacent pairs, or i with i + rot / 2); q to q_out [tokens, ldq], k and v to the caches' slot slots[t] (outside
+ * [0, cache_slots): not stored), bf16 or (dst_f32, from fp32 rows only) fp32.  fp32 throughout, rounded once.  q_out may be
+ * q's part of qkv where the types agree. */
+int mv_qkv_norm_rotary_slots(const void* qkv, int64_t ld, const float* q_norm, const float* k_norm, float eps, const double* inv_freq,
+                             int rot, int adjacent, const int32_t* positions, const int32_t* slots, void* q_out, int64_t ldq,
+                             void* k_cache, void* v_cache, int64_t cache_slots, int tokens, int heads, int kv_heads, int d, int src_f32,
+                             int dst_f32, mv_stream_t stream);
+
+/* out[t, h] = sum_j softmax_j(q[t, h] . k_j * scale) v_j over the row's cached tokens and the nodes of mask[t] (NULL: the nodes up to t),
+ * whose keys and values are in the cache [num_pages, page, hkv, d].  q [tokens, ldq], out [tokens, ldo], caches bf16 or (f32) fp32, all 16-byte
+ * aligned; d 64 or 128, hq / hkv <= 8, page a power of two >= 16.  A node that sees nothing: zeros.  Places whose page is not in
+ * [0, num_pages) and keys behind column bt_cols do not count.  scale > 0.  num_splits (1 .. 64) pieces of the keys side by side;
+ * workspace: of mv_tree_attn_workspace_bytes, 16-byte aligned, needs no clearing, of one running call at a time. */
+size_t mv_tree_attn_workspace_bytes(int tokens, int hq, int d, int num_splits);
+/* How many pieces a step should be given (max_keys: the longest row there may be). */
+int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, int max_keys);
+int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_cache, const int32_t* ctx_lens, const int32_t* row_start,
+                 const int32_t* block_table, int64_t bt_stride, int bt_cols, const uint64_t* mask, int words, void* out, int64_t ldo,
+                 void* workspace, size_t workspace_bytes, int rows, int tokens, int max_nodes, int hq, int hkv, int d, int page,
+                 int num_pages, float scale, int num_splits, int f32, mv_stream_t stream);
+
+/* The walk from node 0 to the lowest later node whose parent is the current one and whose token is picks[current], and so on, up to max_path
+ * nodes: path [rows, max_path] (-1 behind its end), ids [rows, max_path] = the picks along it (-1), counts [rows], lens [rows] = ctx_lens +
+ * counts (NULL: not wanted; not ctx_lens itself).  layers > 0: then keys and values (row_bytes a token, a multiple of 16, in each of the
+ * layers' caches; the addresses are host arrays) at index ctx_lens + path[j] of the sequence go to index ctx_lens + j; places without a page:
+ * not.  One launch per 64 layers. */
+int mv_tree_accept(const int64_t* tokens, const int64_t* picks, const int32_t* parents, const int32_t* row_start, const int32_t* ctx_lens,
+                   const int32_t* block_table, int64_t bt_stride, int bt_cols, void* const* k_caches, void* const* v_caches, int layers,
+                   int64_t row_bytes, int page, int num_pages, int rows, int n_tokens, int max_nodes, int max_path, int32_t* path,
+                   int64_t* ids, int32_t* counts, int32_t* lens, mv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

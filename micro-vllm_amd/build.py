@@ -35,6 +35,8 @@ SOURCES = [
     "diff_attn.hip",
     "delta.hip",
     "gla.hip",
+    "tree_ops.hip",
+    "tree_attn.hip",
 ]
 
 # Libraries that hold a part of the sources, `lib/libmvllm_<name>.so`: what one model family needs, for a

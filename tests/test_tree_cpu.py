@@ -1,0 +1,138 @@
+"""Host side of the ops of a step that verifies drafted tokens: what the C entry points and their Python shims refuse before anything is
+launched, and the oracle of their GPU tests against other statements of the same things."""
+import pytest
+import torch
+
+from oracle import ref_tree as ref
+from tree_util import AttnCase
+
+NULL, P = None, 1 << 20      # an address that is 16-byte aligned; nothing may follow it
+
+
+@pytest.fixture(scope="module")
+def nv():
+    import micro_vllm_amd  # noqa: F401
+    from micro_vllm_amd import _native
+    return _native
+
+
+def plan(nv, ctx=P, starts=P, parents=P, bt=P, stride=8, cols=8, free=P, n_free=4, rows=2, tokens=10, nodes=8, page=16, pages=10, slots=P, pos=P,
+         row=P, mask=P, words=1, taken=P):
+    return nv.lib().mv_tree_plan(ctx, starts, parents, bt, stride, cols, free, n_free, rows, tokens, nodes, page, pages, slots, pos, row, mask,
+                                 words, taken, NULL)
+
+
+def test_plan_refuses(nv):
+    bad = [dict(ctx=NULL), dict(starts=NULL), dict(bt=NULL), dict(free=NULL), dict(slots=NULL), dict(pos=NULL), dict(row=NULL), dict(taken=NULL),
+           dict(rows=-1), dict(tokens=-1), dict(nodes=-1), dict(page=0), dict(pages=0), dict(cols=-1), dict(stride=7), dict(n_free=-1),
+           dict(words=0), dict(words=5), dict(nodes=65, words=1)]
+    for b in bad:
+        assert plan(nv, **b) == nv.MV_ERR_INVALID_ARG, b
+    assert plan(nv, nodes=257, words=4) == nv.MV_ERR_UNSUPPORTED
+    assert plan(nv, nodes=257, mask=NULL) == nv.MV_ERR_UNSUPPORTED           # parents alone
+    assert plan(nv, page=1 << 16, pages=1 << 16) == nv.MV_ERR_UNSUPPORTED     # slots past 32 bits
+    assert plan(nv, rows=0, ctx=NULL, bt=NULL) == nv.MV_OK
+
+
+def store(nv, qkv=P, ld=1024, qn=P, kn=P, freq=P, rot=64, pos=P, slots=P, out=P, ldq=512, k=P, v=P, n=100, tokens=3, hq=8, hkv=4, d=64, src=0, dst=0):
+    return nv.lib().mv_qkv_norm_rotary_slots(qkv, ld, qn, kn, 1e-6, freq, rot, 0, pos, slots, out, ldq, k, v, n, tokens, hq, hkv, d, src, dst, NULL)
+
+
+def test_store_refuses(nv):
+    bad = [dict(qkv=NULL), dict(pos=NULL), dict(slots=NULL), dict(out=NULL), dict(k=NULL), dict(v=NULL), dict(freq=NULL), dict(ld=1023), dict(ldq=511),
+           dict(tokens=-1), dict(hq=0), dict(hkv=0), dict(d=0), dict(rot=-2), dict(rot=63), dict(rot=66), dict(n=0)]
+    for b in bad:
+        assert store(nv, **b) == nv.MV_ERR_INVALID_ARG, b
+    assert store(nv, dst=1) == nv.MV_ERR_UNSUPPORTED
+    assert store(nv, tokens=0, qkv=NULL) == nv.MV_OK
+
+
+def attn(nv, q=P, ldq=512, k=P, v=P, ctx=P, starts=P, bt=P, stride=8, cols=8, mask=P, words=1, out=P, ldo=512, ws=NULL, ws_bytes=0, rows=2, tokens=9,
+         nodes=8, hq=8, hkv=4, d=64, page=16, pages=20, scale=0.1, splits=1, f32=0):
+    return nv.lib().mv_tree_attn(q, ldq, k, v, ctx, starts, bt, stride, cols, mask, words, out, ldo, ws, ws_bytes, rows, tokens, nodes, hq, hkv, d,
+                                 page, pages, scale, splits, f32, NULL)
+
+
+def test_attention_refuses(nv):
+    bad = [dict(q=NULL), dict(k=NULL), dict(v=NULL), dict(ctx=NULL), dict(starts=NULL), dict(bt=NULL), dict(out=NULL), dict(q=P + 8), dict(k=P + 2),
+           dict(out=P + 4), dict(ldq=508), dict(ldq=516), dict(ldo=500), dict(ldo=515), dict(rows=-1), dict(tokens=-1), dict(nodes=-1), dict(hq=6),
+           dict(hkv=0), dict(cols=0), dict(stride=7), dict(page=0), dict(pages=0), dict(splits=0), dict(scale=0.0), dict(scale=-1.0),
+           dict(scale=float("nan")), dict(scale=float("inf")), dict(words=0), dict(words=5), dict(nodes=65)]
+    for b in bad:
+        assert attn(nv, **b) == nv.MV_ERR_INVALID_ARG, b
+    for b in (dict(d=96, hq=4, ldq=384, ldo=384), dict(hq=36, ldq=4096, ldo=4096), dict(page=48), dict(page=8), dict(nodes=257, words=4), dict(splits=65)):
+        assert attn(nv, **b) == nv.MV_ERR_UNSUPPORTED, b
+    assert attn(nv, splits=2) == nv.MV_ERR_WORKSPACE
+    need = nv.lib().mv_tree_attn_workspace_bytes(9, 8, 64, 2)
+    assert need >= 2 * 9 * 8 * 66 * 4
+    assert attn(nv, splits=2, ws=P, ws_bytes=need - 1) == nv.MV_ERR_WORKSPACE
+    assert attn(nv, splits=2, ws=P + 4, ws_bytes=need) == nv.MV_ERR_WORKSPACE
+    for b in (dict(rows=0), dict(tokens=0), dict(nodes=0)):
+        assert attn(nv, q=NULL, **b) == nv.MV_OK
+
+
+def accept(nv, tokens=P, picks=P, parents=P, starts=P, ctx=P, bt=P, stride=8, cols=8, k=(P,), v=(P,), layers=1, row_bytes=256, page=16, pages=20, rows=2,
+           n=9, nodes=8, max_path=8, path=P, ids=P, counts=P, lens=P):
+    import ctypes
+    arr = lambda t: None if t is None else (ctypes.c_void_p * len(t))(*t)      # noqa: E731
+    return nv.lib().mv_tree_accept(tokens, picks, parents, starts, ctx, bt, stride, cols, arr(k), arr(v), layers, row_bytes, page, pages, rows, n,
+                                   nodes, max_path, path, ids, counts, lens, NULL)
+
+
+def test_accept_refuses(nv):
+    bad = [dict(tokens=NULL), dict(picks=NULL), dict(starts=NULL), dict(ctx=NULL), dict(path=NULL), dict(ids=NULL), dict(counts=NULL), dict(bt=NULL),
+           dict(k=None), dict(v=None), dict(k=(NULL,)), dict(v=(P + 8,)), dict(rows=-1), dict(n=-1), dict(nodes=-1), dict(max_path=0), dict(layers=-1),
+           dict(page=0), dict(pages=0), dict(row_bytes=0), dict(stride=7)]
+    for b in bad:
+        assert accept(nv, **b) == nv.MV_ERR_INVALID_ARG, b
+    for b in (dict(nodes=257), dict(max_path=257), dict(row_bytes=24)):
+        assert accept(nv, **b) == nv.MV_ERR_UNSUPPORTED, b
+    assert accept(nv, rows=0, tokens=NULL) == nv.MV_OK
+
+
+def test_shims_refuse_tensors_off_the_device(nv):
+    from micro_vllm_amd.core import tree_decode as ops
+    z = torch.zeros(4, dtype=torch.int32)
+    case = AttnCase([5], [3], 4, 2, 64, 16, torch.bfloat16)
+    with pytest.raises(AssertionError):
+        ops.tree_plan(z, z, torch.zeros(4, 4, dtype=torch.int32), z, 4, 16, 10, tokens=4)
+    with pytest.raises(AssertionError):
+        ops.tree_attn(case.q, case.k, case.v, z, z, torch.zeros(4, 4, dtype=torch.int32), None, 4)
+    with pytest.raises(AssertionError):
+        ops.qkv_norm_rotary_slots(torch.zeros(4, 8 * 64), z, z, case.k, case.v, 4)
+    with pytest.raises(AssertionError):
+        ops.TreeCaches([case.k], [case.v])
+    with pytest.raises(AssertionError):
+        ops.tree_accept(z.long(), z.long(), z, z, 4)
+
+
+def test_pick_of_splits_stays_in_its_range(nv):
+    L = nv.lib()
+    for rows in (1, 3, 64, 5000):
+        for nodes in (1, 16, 256):
+            for keys in (1, 64, 5000, 1 << 20):
+                assert 1 <= L.mv_tree_attn_pick_splits(rows, nodes, 8, 2, 64, keys) <= 64
+
+
+def test_oracle_attention_is_a_dense_softmax():
+    """A row's oracle output against scaled_dot_product_attention with the same mask laid out densely."""
+    case = AttnCase([21], [13], 4, 2, 64, 16, torch.float32, seed=1)
+    o, mag, _, count = case.reference()
+    keys = [(case.table[0][j // 16], j % 16) for j in range(34)]
+    k = torch.stack([case.k[p, s] for p, s in keys]).double().permute(1, 0, 2)
+    v = torch.stack([case.v[p, s] for p, s in keys]).double().permute(1, 0, 2)
+    see = torch.zeros(13, 34, dtype=torch.bool)
+    see[:, :21] = True
+    for i in range(13):
+        for j in case.seen[i]:
+            see[i, 21 + j] = True
+    want = torch.nn.functional.scaled_dot_product_attention(case.q[:13].double().permute(1, 0, 2), k.repeat_interleave(2, 0), v.repeat_interleave(2, 0),
+                                                            attn_mask=see[None])
+    assert torch.allclose(o, want.permute(1, 0, 2), atol=1e-12) and count.tolist() == see.sum(1).tolist() and (mag >= o.abs() - 1e-12).all()
+
+
+def test_oracle_plan_by_hand():
+    parents = torch.tensor([-1, 0, 0, 1, -1, 4, 0])
+    slots, pos, rows, seen, taken, table = ref.plan([5, 3], [0, 4, 7], [[2, -1], [7, -1]], [9, 4], 4, 20, parents)
+    assert taken == [-1, 1] and slots[:4] == [-1] * 4 and slots[4:] == [7 * 4 + 3, 9 * 4, 9 * 4 + 1] and table == [[2, -1], [7, 9]]
+    assert pos[:4] == [5, 6, 6, 7] and seen[3] == {0, 1, 3} and rows == [0] * 4 + [1] * 3
