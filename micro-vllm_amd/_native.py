@@ -193,7 +193,7 @@ PROTOTYPES = {
     "mv_tree_plan": (_I, [_P, _P, _P, _P, _L, _I, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P]),
     "mv_qkv_norm_rotary_slots": (_I, [_P, _L, _P, _P, _F, _P, _I, _I, _P, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _I, _I, _P]),
     "mv_tree_attn_workspace_bytes": (_Z, [_I, _I, _I, _I]),
-    "mv_tree_attn_pick_splits": (_I, [_I, _I, _I, _I, _I, _I]),
+    "mv_tree_attn_pick_splits": (_I, [_I, _I, _I, _I, _I, _I, _I]),
     "mv_tree_attn": (_I, [_P, _L, _P, _P, _P, _P, _P, _L, _I, _P, _I, _P, _L, _P, _Z, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P]),
     "mv_tree_accept": (_I, [_P, _P, _P, _P, _P, _P, _L, _I, _P, _P, _I, _L, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P]),
     "mv_graph_begin_capture": (_I, [_P]),

@@ -168,7 +168,7 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx
     _same_device(q, k_cache, v_cache, ctx_lens, row_start, block_table, mask, out, workspace)
     L = nv.lib()
     if num_splits <= 0:
-        num_splits = L.mv_tree_attn_pick_splits(rows, int(max_nodes), heads, kv_heads, d, cols * page)
+        num_splits = L.mv_tree_attn_pick_splits(rows, int(max_nodes), heads, kv_heads, d, cols * page, int(q.dtype == torch.float32))
     need = L.mv_tree_attn_workspace_bytes(tokens, heads, d, num_splits)
     if need and workspace is None:
         workspace = torch.empty(need // 4, dtype=torch.float32, device=q.device)
@@ -181,10 +181,11 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx
     return out
 
 
-def tree_attn_workspace(tokens: int, rows: int, max_nodes: int, heads: int, kv_heads: int, d: int, max_keys: int, num_splits: int = 0) -> int:
+def tree_attn_workspace(tokens: int, rows: int, max_nodes: int, heads: int, kv_heads: int, d: int, max_keys: int, num_splits: int = 0,
+                        dtype: torch.dtype = torch.bfloat16) -> int:
     """Bytes of workspace of a tree_attn call (max_keys: its block table's columns times the page size); 0: none."""
     L = nv.lib()
-    splits = num_splits if num_splits > 0 else L.mv_tree_attn_pick_splits(rows, max_nodes, heads, kv_heads, d, max_keys)
+    splits = num_splits if num_splits > 0 else L.mv_tree_attn_pick_splits(rows, max_nodes, heads, kv_heads, d, max_keys, int(dtype == torch.float32))
     return L.mv_tree_attn_workspace_bytes(tokens, heads, d, splits)
 
 

@@ -11,7 +11,8 @@ namespace mv {
 constexpr float kTreeNegBig = -1.0e30f;        // a running maximum before any visible key
 constexpr int kTreeMaxNodes = 256;
 constexpr int kTreeMaxWords = kTreeMaxNodes / 64;
-constexpr int kTreeBlock = 16;                 // keys of a block: pages hold whole blocks
+constexpr int kTreeBlock = 16;                 // pages hold whole runs of this many keys
+constexpr int kTreeMaxSplits = 64;
 
 struct TreeArgs {
     const void *q, *k_cache, *v_cache;
@@ -24,6 +25,7 @@ struct TreeArgs {
     int64_t ldo;
     float *part, *state;         // splits: sums [split][token][head][d], (maximum, denominator) [split][token][head]
     int bt_cols, rows, tokens, max_nodes, hq, hkv, g, page, page_shift, num_pages, nsplit, row_blocks;
+    int round_keys;              // keys that a split's workgroup takes in one round
     float scale_log2;
 };
 
@@ -31,21 +33,17 @@ struct TreeSpan {
     int start, n, ctx, total;    // first token, nodes, cached tokens, keys that have a place in the table
 };
 __device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int b) {
-    TreeSpan s;
-    s.start = min(max(a.row_start[b], 0), a.tokens);
-    s.n = min(min(max(a.row_start[b + 1], s.start), a.tokens) - s.start, a.max_nodes);
-    s.ctx = max(a.ctx[b], 0);
+    TreeSpan s;      // (b is the same for a wave: scalar registers, whatever instruction loads them)
+    s.start = min(max(__builtin_amdgcn_readfirstlane(a.row_start[b]), 0), a.tokens);
+    s.n = min(min(max(__builtin_amdgcn_readfirstlane(a.row_start[b + 1]), s.start), a.tokens) - s.start, a.max_nodes);
+    s.ctx = max(__builtin_amdgcn_readfirstlane(a.ctx[b]), 0);
     s.total = (int)min((int64_t)s.ctx + s.n, (int64_t)a.bt_cols << a.page_shift);
     return s;
 }
-// Blocks of a split: all splits of a row but the last take as many, and none fewer than a block a wave
-__device__ __forceinline__ int split_blocks(const TreeArgs& a, int total) {
-    const int blocks = (total + kTreeBlock - 1) / kTreeBlock;
-    return max((blocks + a.nsplit - 1) / a.nsplit, 4);
-}
+// Blocks are dealt to the splits in rounds of one for every wave of a workgroup, so which keys a wave asks for first does not depend on
+// a row's length.  Splits of a row that have any:
 __device__ __forceinline__ int filled_splits_tree(const TreeArgs& a, int total) {
-    const int per = split_blocks(a, total), blocks = (total + kTreeBlock - 1) / kTreeBlock;
-    return (blocks + per - 1) / per;
+    return max(1, min(a.nsplit, (total + a.round_keys - 1) / a.round_keys));
 }
 // 64 bits of a node's mask from bit `first` (negative: cached tokens in front of the nodes, visible) on
 __device__ __forceinline__ uint64_t mask_from(const uint64_t (&w)[kTreeMaxWords], int first) {
@@ -59,6 +57,24 @@ __device__ __forceinline__ uint64_t mask_from(const uint64_t (&w)[kTreeMaxWords]
         if (i == at + 1) hi = w[i];
     }
     return sh ? (lo >> sh) | (hi << (64 - sh)) : lo;
+}
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+
+__device__ __forceinline__ float max_of_quarters(float v) {      // over lanes l, l ^ 16, l ^ 32, l ^ 48, in the vector unit
+    const unsigned u = __float_as_uint(v);
+    const auto x = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const float m = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+    const unsigned w = __float_as_uint(m);
+    const auto y = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+// infinities and NaN of two packed bf16 become zero; whether there were any
+__device__ __forceinline__ bool drop_odd(uint32_t& w) {
+    const bool lo = (w & 0x7f80u) == 0x7f80u, hi = (w & 0x7f800000u) == 0x7f800000u;
+    w &= (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
+    return lo || hi;
 }
 
 template <bool F32> struct TreeT;
@@ -78,12 +94,65 @@ template <> struct TreeT<false> {
     }
 };
 
+// dimensions c .. c + 3 of a stacked row: the output, or a split's sums
+template <bool F32, int D>
+__device__ __forceinline__ void leave_rows(const TreeArgs& a, const TreeSpan& s, bool whole, int split, int kvh, int sr, int c, float top,
+                                           float den, f32x4_t o) {
+    typedef TreeT<F32> X;
+    const int64_t t = s.start + sr / a.g;
+    const int head = kvh * a.g + sr % a.g;
+    if (whole) {
+        const float inv = den != 0.f ? 1.0f / den : 0.f;      // nothing visible: zeros
+        X::st4((typename X::T*)a.out + t * a.ldo + (int64_t)head * D + c, o * inv);
+    } else {
+        const int64_t at = ((int64_t)split * a.tokens + t) * a.hq + head;
+        *reinterpret_cast<f32x4_t*>(a.part + at * D + c) = o;
+        if (c == 0) {
+            a.state[2 * at] = top;
+            a.state[2 * at + 1] = den;
+        }
+    }
+}
+
+// Values that are not finite, of keys that some row may not see, were left out of a split's products; here they are added to the sums of a
+// row that sees them: whatever its weight, the result is that infinity or NaN.  `block`: keys that the kernel takes together.  Rare, and
+// slow: a loop over the split's keys.
+template <bool F32, int D>
+__device__ __forceinline__ void add_odd(const TreeArgs& a, const TreeSpan& s, int b, int kvh, int split, int block, int sr, int c, f32x4_t& o) {
+    typedef TreeT<F32> X;
+    const int node = sr / a.g, waves = a.round_keys / block;
+    for (int first = split * a.round_keys; first < s.total; first += a.nsplit * a.round_keys)
+        for (int key = first; key < min(first + waves * block, s.total); ++key) {
+            const int pg = a.block_table[(int64_t)b * a.bt_stride + (key >> a.page_shift)];
+            if (pg < 0 || pg >= a.num_pages) continue;
+            const int kb = key / block * block;
+            if (kb + block <= s.ctx) {       // such a block was left out of the products' care only if one of its pages is missing
+                bool there = true;
+                for (int k = kb; k < kb + block; k += kTreeBlock) {
+                    const int p = a.block_table[(int64_t)b * a.bt_stride + min(k >> a.page_shift, a.bt_cols - 1)];
+                    there &= p >= 0 && p < a.num_pages;
+                }
+                if (there && kb + block <= s.total) continue;
+            } else if (key >= s.ctx) {
+                const int j = key - s.ctx;
+                if (a.mask ? !(a.mask[(int64_t)(s.start + node) * a.words + (j >> 6)] >> (j & 63) & 1) : j > node) continue;
+            }
+            const f32x4_t x = X::ld4((const typename X::T*)a.v_cache +
+                                     ((((int64_t)pg << a.page_shift) + (key & (a.page - 1))) * a.hkv + kvh) * D + c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (!(fabsf(x[j]) <= 3.4028235e38f)) o[j] += x[j];
+        }
+}
+
+// ------------------------------------------------------------------ fp32
 // Both products on v_mfma_f32_16x16x4_f32 (operand A lane (r, q) = A[r][slot q], B likewise, result lane (r, q) = C[4 q + j][r]); the
 // contraction's slots are labels.  S^T = K . Q^T: slot q of step j of a group of 16 dimensions is dimension 4 q + j, so a key's and a
 // query's values are read 16 (8) bytes a lane.  O^T = V^T . P^T: slot q of step j is key 4 q + j, which is where S^T left its score;
 // row r of output block c is dimension 64 h + 4 r + c, so a value row too is read as it lies.  Nothing goes through LDS until the end.
-template <bool F32, int D>
+template <int D>
 __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
+    constexpr bool F32 = true;
     typedef TreeT<F32> X;
     typedef typename X::T T;
     constexpr int RT = 2, W = 4, KG = D / 16, H = D / 64;
@@ -94,9 +163,8 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
     const int rb = rest % a.row_blocks, bh = rest / a.row_blocks, kvh = bh % a.hkv, b = bh / a.hkv;
     const TreeSpan s = tree_span(a, b);
     const int stacked = s.n * a.g, row0 = rb * RT * 16;
-    const int per = split_blocks(a, s.total), blocks = (s.total + kTreeBlock - 1) / kTreeBlock;
-    const int blk0 = split * per, blk1 = min(blk0 + per, blocks);
-    if (row0 >= stacked || (blk0 >= blk1 && split > 0)) return;
+    const int blocks = (s.total + kTreeBlock - 1) / kTreeBlock;
+    if (row0 >= stacked || split >= filled_splits_tree(a, s.total)) return;
 
     f32x4_t qf[RT][KG];
     uint64_t words[RT][kTreeMaxWords];
@@ -128,7 +196,8 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
             for (int c = 0; c < 4; ++c) acc[i][h][c] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
     const int64_t stride = (int64_t)a.hkv * D;
-    for (int blk = blk0 + wid; blk < blk1; blk += W) {
+    bool odd = false;
+    for (int blk = split * W + wid; blk < blocks; blk += a.nsplit * W) {
         const int kb = blk * kTreeBlock, pg = a.block_table[(int64_t)b * a.bt_stride + (kb >> a.page_shift)];
         if (pg < 0 || pg >= a.num_pages) continue;      // a place without a page: its keys do not count
         const int64_t row = ((int64_t)pg << a.page_shift) + (kb & (a.page - 1));
@@ -143,8 +212,7 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
             for (int h = 0; h < H; ++h) vf[j][h] = X::ld4(vp + j * stride + 64 * h);
         const bool open = kb + kTreeBlock <= s.ctx;      // every key visible to every row (uniform)
         // Where a row may not see a key, its weight is zero and the product would still hand on a value that is not finite: such
-        // values are left out of the product and added by hand to the rows that do see them; behind the last key everything is.
-        bool odd = false;
+        // values are left out here and added at the end (add_odd); behind the last key everything is left out.
         if (!open) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -158,7 +226,6 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
                             odd = true;
                         }
                     }
-            odd = __builtin_amdgcn_ballot_w64(odd) != 0;
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -194,27 +261,6 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[i][h][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[j][h][c], p[j], acc[i][h][c], 0, 0, 0);
                 }
-            if (odd) {
-                for (int key = 0; key < 16 && kb + key < s.total; ++key) {
-                    float pk = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float v = __shfl(p[j], (key >> 2) * 16 + r, 64);
-                        if ((key & 3) == j) pk = v;
-                    }
-                    if (!(seen >> key & 1)) continue;
-                    const T* v = (const T*)a.v_cache + (row + key) * stride + (int64_t)kvh * D;
-#pragma unroll
-                    for (int h = 0; h < H; ++h)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const f32x4_t x = X::ld4(v + 64 * h + 16 * q + 4 * e);
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                if (!(fabsf(x[c]) <= 3.4028235e38f)) acc[i][h][c][e] += pk * x[c];
-                        }
-                }
-            }
         }
     }
 #pragma unroll
@@ -233,8 +279,9 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
                 *reinterpret_cast<f32x4_t*>(&oL[wid][i * 16 + r][64 * h + 16 * q + 4 * e]) =
                     (f32x4_t){acc[i][h][0][e], acc[i][h][1][e], acc[i][h][2][e], acc[i][h][3][e]};
     }
-    __syncthreads();
+    const bool any_odd = __syncthreads_or(odd);
     const bool whole = filled_splits_tree(a, s.total) <= 1;
+#pragma unroll 1
     for (int it = threadIdx.x; it < RT * 16 * (D / 4); it += 256) {
         const int rr = it / (D / 4), c = it % (D / 4) * 4, sr = row0 + rr;
         if (sr >= stacked) break;
@@ -249,19 +296,221 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
             den = fmaf(lL[w][rr], f, den);
             o += *reinterpret_cast<const f32x4_t*>(&oL[w][rr][c]) * f;
         }
-        const int64_t t = s.start + sr / a.g;
-        const int head = kvh * a.g + sr % a.g;
-        if (whole) {
-            const float inv = den != 0.f ? 1.0f / den : 0.f;      // nothing visible: zeros
-            X::st4((T*)a.out + t * a.ldo + (int64_t)head * D + c, o * inv);
-        } else {
-            const int64_t at = ((int64_t)split * a.tokens + t) * a.hq + head;
-            *reinterpret_cast<f32x4_t*>(a.part + at * D + c) = o;
-            if (c == 0) {
-                a.state[2 * at] = top;
-                a.state[2 * at + 1] = den;
+        if (any_odd) add_odd<F32, D>(a, s, b, kvh, split, 16, sr, c, o);
+        leave_rows<F32, D>(a, s, whole, split, kvh, sr, c, top, den, o);
+    }
+}
+
+// ------------------------------------------------------------------ bf16, up to 64 stacked rows a workgroup
+// Every wave has keys of its own (32 at a time) and all the rows: nothing is shared until the end, no barrier in the loop.
+//   S^T = K . Q^T   v_mfma_f32_16x16x32_bf16, operand A = key rows as they lie in memory (lane (r, q): row r, dimensions 32 k + 8 q ..);
+//   O^T = V^T . P^T operand B = P as S^T left it, rounded to bf16 (keys 4 q + j and 16 + 4 q + j), operand A through the wave's own piece of
+//                   LDS with the transposing read, which delivers those keys.
+// The normaliser sums the unrounded weights; rounding a weight to bf16 (2^-8 of it) is what the matrix instruction asks for, and half of what
+// the rounding of the output costs anyway.  The next block's keys and values are requested into the registers that this one leaves.
+// RG groups of four waves take 16 RT stacked rows each and the same keys: more rows in one wave are more than 256 registers (heads of 128), and what
+// the groups ask for twice comes out of the L1 cache.
+template <int D, int RT, int RG>
+constexpr size_t kNarrowLds = [] {
+    constexpr size_t stage = RG * 4 * 32 * (D * 2 + 32), merge = RG * 4 * RT * 16 * (D + 4) * sizeof(float);
+    return stage > merge ? stage : merge;
+}();
+
+template <int D, int RT, int RG>
+__global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs a) {
+    constexpr int W = 4, KS = D / 32, DT = D / 16, VROW = D * 2 + 32, VPR = D / 8, NV = 32 * VPR / 64, OROW = D + 4, ROWS = RG * RT * 16;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kNarrowLds<D, RT, RG>];
+    __shared__ float mL[W][ROWS], lL[W][ROWS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+    const int wid = wave & 3, rg = wave >> 2;
+    const int split = blockIdx.x % a.nsplit, rest = blockIdx.x / a.nsplit;
+    const int rb = rest % a.row_blocks, bh = rest / a.row_blocks, kvh = bh % a.hkv, b = bh / a.hkv;
+    typedef const int32_t __attribute__((address_space(4))) Entry;      // (nothing here writes the table: scalar loads)
+    Entry* bt = (Entry*)(uintptr_t)(a.block_table + (int64_t)b * a.bt_stride);
+    auto pages_of = [&](int blk, int (&pg)[2]) {
+        pg[0] = bt[min((blk * 32) >> a.page_shift, a.bt_cols - 1)];
+        pg[1] = bt[min((blk * 32 + 16) >> a.page_shift, a.bt_cols - 1)];
+    };
+    int blk = split * W + wid, pg[2];
+    bool odd = false;
+    pages_of(blk, pg);
+    const TreeSpan s = tree_span(a, b);
+    const int stacked = s.n * a.g, row0 = rb * ROWS, blocks = (s.total + 31) / 32;
+    if (row0 >= stacked || split >= filled_splits_tree(a, s.total)) return;
+
+    // (a request = a base that is the same for the wave, in scalar registers, and a lane's offset of 32 bits that never changes)
+    const unsigned row_bytes = (unsigned)a.hkv * D * 2, k_at = r * row_bytes + 16 * q, v_from = (lane / VPR) * row_bytes + (lane % VPR) * 16;
+    uint4 kR[2][KS], vR[NV];
+    auto base_of = [&](const void* cache, int at, int half, int page) {
+        const int64_t row = ((int64_t)(page >= 0 && page < a.num_pages ? page : 0) << a.page_shift) + ((at * 32 + 16 * half) & (a.page - 1));
+        return (const unsigned char*)cache + row * row_bytes + kvh * D * 2;
+    };
+    auto load_k = [&](int at, const int (&page)[2]) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const unsigned char* p = base_of(a.k_cache, at, x, page[x]);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) kR[x][k] = ld16(p + 64 * k + k_at);
+        }
+    };
+    auto load_v = [&](int at, const int (&page)[2]) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const unsigned char* p = base_of(a.v_cache, at, x, page[x]);
+#pragma unroll
+            for (int i = 0; i < NV / 2; ++i) vR[x * (NV / 2) + i] = ld16(p + i * (64 / VPR) * row_bytes + v_from);
+        }
+    };
+    load_k(blk, pg);
+    load_v(blk, pg);
+
+    bf16x8_t qf[RT][KS];
+    int node[RT];
+    uint64_t word0[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int sr = min(row0 + rg * RT * 16 + i * 16 + r, stacked - 1);
+        node[i] = sr / a.g;
+        const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.start + node[i]) * a.ldq + (int64_t)(kvh * a.g + sr % a.g) * D + 8 * q;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) qf[i][k] = __builtin_bit_cast(bf16x8_t, ld16(qp + 32 * k));
+        word0[i] = a.mask ? a.mask[(int64_t)(s.start + node[i]) * a.words] : 0;
+    }
+    // what row i sees of the 32 keys from kb on
+    auto visible = [&](int i, int kb) -> uint32_t {
+        const int first = kb - s.ctx;
+        if (!a.mask) {
+            const int up = node[i] + 1 - first;
+            return up >= 32 ? ~0u : up > 0 ? (1u << up) - 1 : 0;
+        }
+        if (first < 0) return first <= -32 ? ~0u : (uint32_t)(word0[i] << -first) | ((1u << -first) - 1);
+        const int at = first >> 6, sh = first & 63;
+        const uint64_t* w = a.mask + (int64_t)(s.start + node[i]) * a.words;
+        uint64_t v = (at == 0 ? word0[i] : at < a.words ? w[at] : 0) >> sh;
+        if (sh > 32 && at + 1 < a.words) v |= w[at + 1] << (64 - sh);
+        return (uint32_t)v;
+    };
+
+    f32x4_t acc[RT][DT];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        m[i] = kTreeNegBig;
+        l[i] = 0.f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) acc[i][t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    }
+    unsigned char* vst = lds + wave * (32 * VROW);
+    const int v_at = (lane / VPR) * VROW + (lane % VPR) * 16, tr_at = (4 * q + (r >> 2)) * VROW + (r & 3) * 8;
+
+    while (blk < blocks) {
+        const int kb = blk * 32, next = blk + a.nsplit * W;
+        uint32_t valid = (pg[0] >= 0 && pg[0] < a.num_pages ? 0xffffu : 0) | (pg[1] >= 0 && pg[1] < a.num_pages ? 0xffff0000u : 0);
+        if (s.total - kb < 32) valid &= (1u << (s.total - kb)) - 1;
+        const bool open = valid == ~0u && kb + 32 <= s.ctx;       // every key there and visible to every row (uniform)
+        if (!open) {     // values of keys that do not count are zero, what is not finite is added at the end (add_odd)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const bool there = valid >> (i * (64 / VPR) + lane / VPR) & 1;
+                if (!there) vR[i] = make_uint4(0, 0, 0, 0);
+                const bool o0 = drop_odd(vR[i].x), o1 = drop_odd(vR[i].y), o2 = drop_odd(vR[i].z), o3 = drop_odd(vR[i].w);
+                odd |= o0 | o1 | o2 | o3;
             }
         }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) *reinterpret_cast<uint4*>(vst + v_at + i * (64 / VPR) * VROW) = vR[i];
+        int pn[2] = {-1, -1};
+        if (next < blocks) pages_of(next, pn);
+        f32x4_t sc[RT][2];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                sc[i][x] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+                    sc[i][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kR[x][k]), qf[i][k], sc[i][x], 0, 0, 0);
+            }
+        __builtin_amdgcn_sched_barrier(0);      // (the requests go into the registers that the products have read: not before them)
+        if (next < blocks) {
+            load_k(next, pn);
+            load_v(next, pn);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        pg[0] = pn[0];
+        pg[1] = pn[1];
+        bf16x8_t pf[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            if (!open) {
+                const uint32_t seen = visible(i, kb) & valid;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (!(seen >> (16 * x + 4 * q + j) & 1)) sc[i][x][j] = -__builtin_inff();
+            }
+            float top = fmaxf(fmaxf(fmaxf(sc[i][0][0], sc[i][0][1]), fmaxf(sc[i][0][2], sc[i][0][3])),
+                              fmaxf(fmaxf(sc[i][1][0], sc[i][1][1]), fmaxf(sc[i][1][2], sc[i][1][3]))) * a.scale_log2;
+            top = max_of_quarters(top);
+            if (__builtin_amdgcn_ballot_w64(top > m[i]) != 0) {      // (else a factor of one for every row)
+                const float mn = fmaxf(m[i], top), alpha = __builtin_amdgcn_exp2f(m[i] - mn);
+                m[i] = mn;
+                l[i] *= alpha;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) acc[i][t] *= alpha;
+            }
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[i][e >> 2][e & 3], a.scale_log2, -m[i]));
+            l[i] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            pf[i] = __builtin_bit_cast(bf16x8_t, make_uint4(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]),
+                                                            pack_bf16x2(p[6], p[7])));
+        }
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            const unsigned char* vb = vst + tr_at + 32 * t;
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(vb));
+            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(vb + 16 * VROW));
+            const s16x8_t both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+                acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, both), pf[i], acc[i][t], 0, 0, 0);
+        }
+        blk = next;
+    }
+    __syncthreads();       // (the states lie where values were staged)
+    float* oL = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        l[i] += __shfl_xor(l[i], 16, 64);
+        l[i] += __shfl_xor(l[i], 32, 64);
+        if (q == 0) {
+            mL[wid][(rg * RT + i) * 16 + r] = m[i];
+            lL[wid][(rg * RT + i) * 16 + r] = l[i];
+        }
+#pragma unroll
+        for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4_t*>(oL + (wid * ROWS + (rg * RT + i) * 16 + r) * OROW + 16 * t + 4 * q) = acc[i][t];
+    }
+    const bool any_odd = __syncthreads_or(odd);
+    const bool whole = filled_splits_tree(a, s.total) <= 1;
+#pragma unroll 1
+    for (int it = threadIdx.x; it < ROWS * (D / 4); it += RG * 256) {
+        const int rr = it / (D / 4), c = it % (D / 4) * 4, sr = row0 + rr;
+        if (sr >= stacked) break;
+        float top = mL[0][rr];
+#pragma unroll
+        for (int w = 1; w < W; ++w) top = fmaxf(top, mL[w][rr]);
+        float den = 0.f;
+        f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float f = __builtin_amdgcn_exp2f(mL[w][rr] - top);
+            den = fmaf(lL[w][rr], f, den);
+            o += *reinterpret_cast<const f32x4_t*>(oL + (w * ROWS + rr) * OROW + c) * f;
+        }
+        if (any_odd) add_odd<false, D>(a, s, b, kvh, split, 32, sr, c, o);
+        leave_rows<false, D>(a, s, whole, split, kvh, sr, c, top, den, o);
     }
 }
 
@@ -290,6 +539,19 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
     X::st4((typename X::T*)a.out + t * a.ldo + (int64_t)head * D + c, o * inv);
 }
 
+// Rows, workgroups and keys of a launch
+struct TreeForm {
+    int row_tiles, row_blocks, round_keys;
+};
+static TreeForm tree_form(int max_nodes, int g, int d, int f32) {
+    const int64_t stacked = (int64_t)max_nodes * g;
+    TreeForm f;
+    f.row_tiles = f32 ? 2 : stacked <= 16 ? 1 : stacked <= 32 ? 2 : 4;
+    f.row_blocks = (int)((stacked + 16 * f.row_tiles - 1) / (16 * f.row_tiles));
+    f.round_keys = f32 ? 64 : 128;
+    return f;
+}
+
 }  // namespace mv
 
 extern "C" {
@@ -299,13 +561,15 @@ size_t mv_tree_attn_workspace_bytes(int tokens, int hq, int d, int num_splits) {
     return (size_t)num_splits * tokens * hq * (d + 2) * sizeof(float);
 }
 
-int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, int max_keys) {
-    if (rows <= 0 || max_nodes <= 0 || hq <= 0 || hkv <= 0 || max_keys <= 0) return 1;
-    const int64_t row_blocks = ((int64_t)max_nodes * (hq / hkv) + 31) / 32, units = rows * (int64_t)hkv * row_blocks;
-    int64_t splits = (2 * mv::num_cus() + units - 1) / units;
-    const int64_t most = ((int64_t)max_keys + 63) / 64;
+int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, int max_keys, int f32) {
+    using namespace mv;
+    if (rows <= 0 || max_nodes <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || max_keys <= 0) return 1;
+    const TreeForm f = tree_form(max_nodes, hq / hkv, d, f32);
+    const int64_t units = (int64_t)rows * hkv * f.row_blocks;
+    int64_t splits = (num_cus() + units - 1) / units;
+    const int64_t most = ((int64_t)max_keys + f.round_keys - 1) / f.round_keys;
     if (splits > most) splits = most;
-    return (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+    return (int)(splits < 1 ? 1 : splits > kTreeMaxSplits ? kTreeMaxSplits : splits);
 }
 
 int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_cache, const int32_t* ctx_lens, const int32_t* row_start,
@@ -316,7 +580,7 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     if (rows < 0 || tokens < 0 || max_nodes < 0 || hq <= 0 || hkv <= 0 || hq % hkv || page <= 0 || num_pages <= 0 || bt_cols <= 0 ||
         bt_stride < bt_cols || num_splits < 1 || !(scale > 0.f) || scale > 3.0e38f)
         return MV_ERR_INVALID_ARG;
-    if ((d != 64 && d != 128) || hq / hkv > 8 || (page & (page - 1)) || page < kTreeBlock || max_nodes > kTreeMaxNodes || num_splits > 64)
+    if ((d != 64 && d != 128) || hq / hkv > 8 || (page & (page - 1)) || page < kTreeBlock || max_nodes > kTreeMaxNodes || num_splits > kTreeMaxSplits)
         return MV_ERR_UNSUPPORTED;
     if (rows == 0 || tokens == 0 || max_nodes == 0) return MV_OK;
     if (!q || !k_cache || !v_cache || !ctx_lens || !row_start || !block_table || !out) return MV_ERR_INVALID_ARG;
@@ -353,24 +617,31 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     a.page_shift = __builtin_ctz((unsigned)page);
     a.num_pages = num_pages;
     a.nsplit = num_splits;
-    a.row_blocks = (max_nodes * a.g + 31) / 32;
+    const TreeForm f = tree_form(max_nodes, a.g, d, f32);
+    a.row_blocks = f.row_blocks;
+    a.round_keys = f.round_keys;
     a.scale_log2 = scale * 1.4426950408889634f;
     const int64_t grid = (int64_t)rows * hkv * a.row_blocks * num_splits;
     if (grid > 0x7fffffff || rows > 65535) return MV_ERR_UNSUPPORTED;
     hipStream_t s = (hipStream_t)stream;
     const dim3 g1((unsigned)grid);
-#define MV_TREE(F32_, D_)                                                                                                     \
-    do {                                                                                                                      \
-        hipLaunchKernelGGL((tree_attn_f32_kernel<F32_, D_>), g1, dim3(256), 0, s, a);                                           \
-        if (num_splits > 1)                                                                                                   \
-            hipLaunchKernelGGL((tree_attn_merge_kernel<F32_, D_>), dim3((unsigned)((max_nodes * hq + 1024 / D_ - 1) / (1024 / D_)), (unsigned)rows), \
-                               dim3(256), 0, s, a);                                                                             \
-    } while (0)
-    if (f32 && d == 64) MV_TREE(true, 64);
-    else if (f32) MV_TREE(true, 128);
-    else if (d == 64) MV_TREE(false, 64);
-    else MV_TREE(false, 128);
+#define MV_TREE(K_, T_) hipLaunchKernelGGL((K_), g1, dim3(T_), 0, s, a)
+    if (f32 && d == 64) MV_TREE((tree_attn_f32_kernel<64>), 256);
+    else if (f32) MV_TREE((tree_attn_f32_kernel<128>), 256);
+    else if (d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<64, 1, 1>), 256);
+    else if (d == 64 && f.row_tiles == 2) MV_TREE((tree_attn_narrow_kernel<64, 2, 1>), 256);
+    else if (d == 64) MV_TREE((tree_attn_narrow_kernel<64, 4, 1>), 256);
+    else if (f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<128, 1, 1>), 256);
+    else if (f.row_tiles == 2) MV_TREE((tree_attn_narrow_kernel<128, 2, 1>), 256);
+    else MV_TREE((tree_attn_narrow_kernel<128, 2, 2>), 512);
 #undef MV_TREE
+    if (num_splits > 1) {
+        const dim3 g2((unsigned)(((int64_t)max_nodes * hq + 1024 / d - 1) / (1024 / d)), (unsigned)rows);
+        if (f32 && d == 64) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 64>), g2, dim3(256), 0, s, a);
+        else if (f32) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 128>), g2, dim3(256), 0, s, a);
+        else if (d == 64) hipLaunchKernelGGL((tree_attn_merge_kernel<false, 64>), g2, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((tree_attn_merge_kernel<false, 128>), g2, dim3(256), 0, s, a);
+    }
     return check_launch();
 }
 

@@ -111,7 +111,7 @@ def test_pick_of_splits_stays_in_its_range(nv):
     for rows in (1, 3, 64, 5000):
         for nodes in (1, 16, 256):
             for keys in (1, 64, 5000, 1 << 20):
-                assert 1 <= L.mv_tree_attn_pick_splits(rows, nodes, 8, 2, 64, keys) <= 64
+                assert all(1 <= L.mv_tree_attn_pick_splits(rows, nodes, 8, 2, 64, keys, f32) <= 64 for f32 in (0, 1))
 
 
 def test_oracle_attention_is_a_dense_softmax():
