@@ -12,7 +12,7 @@ on one device, which has to be the current one; every call goes to the current s
 `workspace`), and can be captured.  Rows must not share the pages that a step's nodes lie in.
 """
 import ctypes
-from typing import NamedTuple, Optional
+from typing import Optional
 
 import torch
 
@@ -21,40 +21,66 @@ from .. import _native as nv
 MAX_NODES = 256      # nodes of a row with a tree or a mask
 
 
-def _i32(t: torch.Tensor, n: Optional[int] = None) -> int:
-    assert t.is_cuda and t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous(), "contiguous int32 device vector expected"
-    assert n is None or t.shape[0] == n, f"{t.shape[0]} values where {n} are expected"
+_I32, _I64, _F32, _BF16 = torch.int32, torch.int64, torch.float32, torch.bfloat16
+
+
+def _vec(t: torch.Tensor, n: int, dev: int, dtype=_I32) -> int:
+    """Address of a contiguous vector of n values on device `dev` (one call a tensor of a step's many: what it asks is what there is to ask)."""
+    assert t.shape == (n,) and t.dtype is dtype and t.get_device() == dev and t.is_contiguous(), \
+        f"contiguous {dtype} vector of {n} on cuda:{dev} expected, got {t.dtype} {tuple(t.shape)} on {t.device}"
     return t.data_ptr()
 
 
-def _table(t: torch.Tensor, rows: int):
-    assert t.is_cuda and t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == rows and (t.stride(1) == 1 or t.shape[1] == 1), \
-        "int32 block table [rows, columns] expected"
-    return t.data_ptr(), t.stride(0) if rows > 1 else t.shape[1], t.shape[1]
+def _table(t: torch.Tensor, rows: int, dev: int):
+    shape = t.shape
+    assert len(shape) == 2 and shape[0] == rows and t.dtype is _I32 and t.get_device() == dev, "int32 block table [rows, columns] expected"
+    stride, one = t.stride()
+    assert one == 1 or shape[1] == 1, "block table rows must be contiguous"
+    return t.data_ptr(), stride if rows > 1 else shape[1], shape[1]
 
 
-def _same_device(first: torch.Tensor, *others):
-    idx = first.get_device()
-    assert idx == torch.cuda.current_device(), "the tensors' device has to be the current one"
-    for t in others:
-        assert t is None or t.get_device() == idx, "tensors on different devices"
+def _current(t: torch.Tensor) -> int:
+    """Device of a call: that of its first tensor, which has to be the current one."""
+    dev = t.get_device()
+    assert dev >= 0, "device tensors expected"
+    assert dev == torch._C._cuda_getDevice(), "the tensors' device has to be the current one"
+    return dev
 
 
-class TreePlan(NamedTuple):
+def _mask(m: torch.Tensor, tokens: int, max_nodes: int, dev: int):
+    shape = m.shape
+    assert m.dtype is _I64 and len(shape) == 2 and shape[0] == tokens and m.is_contiguous() and m.get_device() == dev, \
+        "int64 mask [tokens, words] expected"
+    assert shape[1] * 64 >= max_nodes, f"{shape[1]} mask words for {max_nodes} nodes"
+    return m.data_ptr(), shape[1]
+
+
+class TreePlan:
     """What tree_plan leaves.  Per token: slots (page * page size + place in it, -1: none), positions, rows, mask [tokens, words] int64
     (bit i of word i // 64: node i of the row is the token itself or an ancestor; None where no mask was asked for); per row: taken, the
-    pages taken off the free list, -1 for a row that did not get its pages."""
-    slots: torch.Tensor
-    positions: torch.Tensor
-    rows: torch.Tensor
-    mask: Optional[torch.Tensor]
-    taken: torch.Tensor
+    pages taken off the free list, -1 for a row that did not get its pages.  The buffers are checked once, here."""
+    __slots__ = ("_t", "_p", "tokens", "n_rows", "words", "device")
+
+    def __init__(self, slots: torch.Tensor, positions: torch.Tensor, rows: torch.Tensor, mask: Optional[torch.Tensor], taken: torch.Tensor):
+        self.tokens, self.n_rows, self.device = slots.shape[0], taken.shape[0], slots.get_device()
+        assert self.device >= 0, "device tensors expected"
+        self._t = (slots, positions, rows, mask, taken)
+        m, self.words = (None, 0) if mask is None else _mask(mask, self.tokens, 1, self.device)
+        self._p = (*[_vec(t, self.tokens, self.device) for t in (slots, positions, rows)], m, _vec(taken, self.n_rows, self.device))
+
+    slots = property(lambda self: self._t[0])
+    positions = property(lambda self: self._t[1])
+    rows = property(lambda self: self._t[2])
+    mask = property(lambda self: self._t[3])
+    taken = property(lambda self: self._t[4])
+
+    def __iter__(self):
+        return iter(self._t)
 
     @classmethod
     def empty(cls, rows: int, tokens: int, max_nodes: int, device, mask: bool = True) -> "TreePlan":
-        i32 = [torch.empty(n, dtype=torch.int32, device=device) for n in (tokens, tokens, tokens, rows)]
-        words = max(1, (max_nodes + 63) // 64)
-        m = torch.empty(tokens, words, dtype=torch.int64, device=device) if mask else None
+        i32 = [torch.empty(n, dtype=_I32, device=device) for n in (tokens, tokens, tokens, rows)]
+        m = torch.empty(tokens, max(1, (max_nodes + 63) // 64), dtype=_I64, device=device) if mask else None
         return cls(i32[0], i32[1], i32[2], m, i32[3])
 
 
@@ -69,41 +95,42 @@ def tree_plan(ctx_lens: torch.Tensor, row_start: torch.Tensor, block_table: torc
     pages are not there any more, and every row behind it that needs some, or one that has no columns for them, gets none (taken -1, slots
     -1, its columns untouched).  parents int32 [tokens], None: a chain.  `tokens` (default: those of parents or out) is the number of
     tokens that the outputs hold; `mask` (default: with parents or out, what they have) says whether a mask is wanted."""
-    rows = ctx_lens.shape[0]
-    if tokens is None:
-        assert out is not None or parents is not None, "how many tokens the step has is given by parents, out or tokens"
-        tokens = (out.slots if out is not None else parents).shape[0]
+    rows, dev = ctx_lens.shape[0], _current(ctx_lens)
     if out is None:
+        if tokens is None:
+            assert parents is not None, "how many tokens the step has is given by parents, out or tokens"
+            tokens = parents.shape[0]
         out = TreePlan.empty(rows, tokens, max_nodes, ctx_lens.device, mask=parents is not None if mask is None else mask)
     else:
+        assert (tokens is None or tokens == out.tokens) and out.n_rows == rows and out.device == dev, "out is of another step's sizes"
         assert mask is None or mask == (out.mask is not None)
-    m, words = out.mask, 0
-    if m is not None:
-        assert m.is_cuda and m.dtype == torch.int64 and m.dim() == 2 and m.shape[0] == tokens and m.is_contiguous()
-        words = m.shape[1]
-        assert words * 64 >= max_nodes, f"{words} mask words for {max_nodes} nodes"
-    assert (m is None and parents is None) or max_nodes <= MAX_NODES, f"trees and masks go up to {MAX_NODES} nodes a row"
-    bt, bt_stride, cols = _table(block_table, rows)
-    _same_device(ctx_lens, row_start, block_table, free_pages, parents, *out)
+        tokens = out.tokens
+    slots, positions, row_of, m, taken = out._p
+    assert m is None or out.words * 64 >= max_nodes, f"{out.words} mask words for {max_nodes} nodes"
+    assert max_nodes <= MAX_NODES or (m is None and parents is None), f"trees and masks go up to {MAX_NODES} nodes a row"
+    bt, bt_stride, cols = _table(block_table, rows, dev)
+    free = free_pages.shape[0]
     nv.check("mv_tree_plan", nv.lib().mv_tree_plan(
-        _i32(ctx_lens), _i32(row_start, rows + 1), None if parents is None else _i32(parents, tokens), bt, bt_stride, cols,
-        _i32(free_pages), free_pages.shape[0], rows, tokens, int(max_nodes), int(page), int(num_pages), _i32(out.slots, tokens),
-        _i32(out.positions, tokens), _i32(out.rows, tokens), None if m is None else m.data_ptr(), words, _i32(out.taken, rows),
+        _vec(ctx_lens, rows, dev), _vec(row_start, rows + 1, dev), None if parents is None else _vec(parents, tokens, dev), bt, bt_stride,
+        cols, _vec(free_pages, free, dev), free, rows, tokens, max_nodes, page, num_pages, slots, positions, row_of, m, out.words, taken,
         nv.stream_ptr()))
     return out
 
 
-def _norm(w: Optional[torch.Tensor], d: int):
-    if w is None:
-        return None
-    assert w.is_cuda and w.dtype == torch.float32 and w.numel() == d and w.is_contiguous(), "norm weight: float32 [head size]"
-    return w.data_ptr()
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: int):
+    shape, dtype = k_cache.shape, k_cache.dtype
+    assert len(shape) == 4 and v_cache.shape == shape and v_cache.dtype is dtype, "caches [pages, page, kv heads, d] of one type expected"
+    assert dtype is _BF16 or dtype is _F32, f"bf16 or float32 caches, not {dtype}"
+    assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.get_device() == dev and v_cache.get_device() == dev
+    return shape
 
 
-def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor):
-    assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype, "caches [pages, page, kv heads, d]"
-    assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.dtype in (torch.bfloat16, torch.float32)
-    return k_cache.shape
+def _heads(t: torch.Tensor, shape, dtype, dev: int, what: str) -> int:
+    """Row stride of [tokens, heads, d] whose heads lie side by side."""
+    assert t.shape == shape and t.dtype is dtype and t.get_device() == dev, f"{what}: {dtype} {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}"
+    row, head, one = t.stride()
+    assert one == 1 and (head == shape[2] or shape[1] == 1), f"{what}: heads must lie side by side"
+    return row if shape[0] > 1 else shape[1] * shape[2]
 
 
 def qkv_norm_rotary_slots(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -116,26 +143,21 @@ def qkv_norm_rotary_slots(qkv: torch.Tensor, positions: torch.Tensor, slots: tor
     with i + half), all of it in fp32 and rounded once.  q goes to out [tokens, heads, d], k and v to k_cache / v_cache
     [pages, page, kv_heads, d] at slots[t] (negative or past the last page: not stored; no two tokens may name one slot).  qkv bf16 with bf16
     caches, float32 with either; out has the caches' type and may be q's own part of qkv where the types agree."""
-    pages, page, kv_heads, d = _cache(k_cache, v_cache)
-    assert qkv.is_cuda and qkv.dim() == 2 and qkv.dtype in (torch.bfloat16, torch.float32) and (qkv.stride(1) == 1 or qkv.shape[1] == 1)
-    tokens = qkv.shape[0]
-    assert qkv.shape[1] == (heads + 2 * kv_heads) * d, f"rows of {qkv.shape[1]} values are not {heads} + 2 x {kv_heads} heads of {d}"
-    src_f32, dst_f32 = qkv.dtype == torch.float32, k_cache.dtype == torch.float32
-    assert src_f32 or not dst_f32, "float32 caches take float32 rows"
+    dev = _current(qkv)
+    pages, page, kv_heads, d = _cache(k_cache, v_cache, dev)
+    (tokens, width), src, dst = qkv.shape, qkv.dtype, k_cache.dtype
+    assert width == (heads + 2 * kv_heads) * d, f"rows of {width} values are not {heads} + 2 x {kv_heads} heads of {d}"
+    assert (src is _BF16 and dst is _BF16) or src is _F32, "bf16 rows with bf16 caches, or float32 rows"
+    ld, one = qkv.stride()
+    assert one == 1 or width == 1
     if out is None:
-        out = torch.empty(tokens, heads, d, dtype=k_cache.dtype, device=qkv.device)
-    assert out.shape == (tokens, heads, d) and out.dtype == k_cache.dtype and out.stride(2) == 1 and (heads == 1 or out.stride(1) == d)
-    rot = 0
-    if inv_freq is not None:
-        rot = 2 * inv_freq.numel()
-        assert inv_freq.is_cuda and inv_freq.dtype == torch.float64 and inv_freq.is_contiguous() and rot <= d
-    _same_device(qkv, positions, slots, k_cache, v_cache, q_norm, k_norm, inv_freq, out)
-    ld = qkv.stride(0) if tokens > 1 else qkv.shape[1]
-    ldq = out.stride(0) if tokens > 1 else heads * d
+        out = torch.empty(tokens, heads, d, dtype=dst, device=qkv.device)
+    rot = 0 if inv_freq is None else 2 * inv_freq.shape[0]
     nv.check("mv_qkv_norm_rotary_slots", nv.lib().mv_qkv_norm_rotary_slots(
-        qkv.data_ptr(), ld, _norm(q_norm, d), _norm(k_norm, d), float(eps), nv.ptr(inv_freq), rot, int(adjacent), _i32(positions, tokens),
-        _i32(slots, tokens), out.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(), pages * page, tokens, int(heads), kv_heads, d,
-        int(src_f32), int(dst_f32), nv.stream_ptr()))
+        qkv.data_ptr(), ld if tokens > 1 else width, None if q_norm is None else _vec(q_norm, d, dev, _F32),
+        None if k_norm is None else _vec(k_norm, d, dev, _F32), eps, None if rot == 0 else _vec(inv_freq, rot // 2, dev, torch.float64), rot,
+        adjacent, _vec(positions, tokens, dev), _vec(slots, tokens, dev), out.data_ptr(), _heads(out, (tokens, heads, d), dst, dev, "out"),
+        k_cache.data_ptr(), v_cache.data_ptr(), pages * page, tokens, heads, kv_heads, d, src is _F32, dst is _F32, nv.stream_ptr()))
     return out
 
 
@@ -149,35 +171,34 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx
     column do not count; tokens behind the last row, and nodes past max_nodes, keep what `out` held.  Scores and softmax in fp32; bf16:
     weights rounded to bf16 in front of the product with the values.  num_splits 0: picked; `workspace`: float32, at least
     tree_attn_workspace(...) bytes, of this call alone while it runs (default: allocated)."""
-    pages, page, kv_heads, d = _cache(k_cache, v_cache)
-    assert q.is_cuda and q.dim() == 3 and q.dtype == k_cache.dtype and q.shape[2] == d, "q [tokens, heads, head size] of the caches' type"
-    tokens, heads, _ = q.shape
-    assert q.stride(2) == 1 and (heads == 1 or q.stride(1) == d), "q heads must be contiguous"
+    dev = _current(q)
+    pages, page, kv_heads, d = _cache(k_cache, v_cache, dev)
+    shape, dtype = q.shape, q.dtype
+    assert len(shape) == 3 and shape[2] == d and dtype is k_cache.dtype, "q [tokens, heads, head size] of the caches' type"
+    tokens, heads, _ = shape
     assert heads % kv_heads == 0, f"{heads} heads on {kv_heads}"
     rows = ctx_lens.shape[0]
-    words = 0
-    if mask is not None:
-        assert mask.is_cuda and mask.dtype == torch.int64 and mask.dim() == 2 and mask.shape[0] == tokens and mask.is_contiguous()
-        words = mask.shape[1]
-        assert words * 64 >= max_nodes, f"{words} mask words for {max_nodes} nodes"
+    m, words = (None, 0) if mask is None else _mask(mask, tokens, max_nodes, dev)
     if out is None:
-        out = torch.zeros(tokens, heads, d, dtype=q.dtype, device=q.device)
-    assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1 and (heads == 1 or out.stride(1) == d)
-    assert out.data_ptr() != q.data_ptr() or q.numel() == 0, "out may not be q"
-    bt, bt_stride, cols = _table(block_table, rows)
-    _same_device(q, k_cache, v_cache, ctx_lens, row_start, block_table, mask, out, workspace)
-    L = nv.lib()
+        out = torch.zeros(shape, dtype=dtype, device=q.device)
+    q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+    assert out_ptr != q_ptr or tokens == 0, "out may not be q"
+    bt, bt_stride, cols = _table(block_table, rows, dev)
+    L, f32 = nv.lib(), dtype is _F32
     if num_splits <= 0:
-        num_splits = L.mv_tree_attn_pick_splits(rows, int(max_nodes), heads, kv_heads, d, cols * page, int(q.dtype == torch.float32))
-    need = L.mv_tree_attn_workspace_bytes(tokens, heads, d, num_splits)
-    if need and workspace is None:
-        workspace = torch.empty(need // 4, dtype=torch.float32, device=q.device)
-    scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
+        num_splits = L.mv_tree_attn_pick_splits(rows, max_nodes, heads, kv_heads, d, cols * page, f32)
+    ws = need = 0
+    if num_splits > 1:
+        need = L.mv_tree_attn_workspace_bytes(tokens, heads, d, num_splits)
+        if workspace is None:
+            workspace = torch.empty(need // 4, dtype=_F32, device=q.device)
+        assert workspace.get_device() == dev and workspace.is_contiguous()
+        ws, need = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     nv.check("mv_tree_attn", L.mv_tree_attn(
-        q.data_ptr(), q.stride(0) if tokens > 1 else heads * d, k_cache.data_ptr(), v_cache.data_ptr(), _i32(ctx_lens),
-        _i32(row_start, rows + 1), bt, bt_stride, cols, nv.ptr(mask), words, out.data_ptr(), out.stride(0) if tokens > 1 else heads * d,
-        workspace.data_ptr() if need else None, workspace.numel() * workspace.element_size() if need else 0, rows, tokens, int(max_nodes),
-        heads, kv_heads, d, page, pages, scale, int(num_splits), int(q.dtype == torch.float32), nv.stream_ptr()))
+        q_ptr, _heads(q, shape, dtype, dev, "q"), k_cache.data_ptr(), v_cache.data_ptr(), _vec(ctx_lens, rows, dev),
+        _vec(row_start, rows + 1, dev), bt, bt_stride, cols, m, words, out_ptr, _heads(out, shape, dtype, dev, "out"), ws or None, need, rows,
+        tokens, max_nodes, heads, kv_heads, d, page, pages, d ** -0.5 if softmax_scale is None else softmax_scale, num_splits, f32,
+        nv.stream_ptr()))
     return out
 
 
@@ -196,30 +217,45 @@ class TreeCaches:
     def __init__(self, k_caches, v_caches):
         k, v = list(k_caches), list(v_caches)
         assert len(k) == len(v) and len(k) > 0
-        self.pages, self.page, kv_heads, d = _cache(k[0], v[0])
+        self.device = k[0].get_device()
+        assert self.device >= 0, "device tensors expected"
+        self.pages, self.page, kv_heads, d = _cache(k[0], v[0], self.device)
         for a, b in zip(k, v):
-            assert a.is_cuda and _cache(a, b) == k[0].shape and a.dtype == k[0].dtype
-            assert a.get_device() == k[0].get_device() and b.get_device() == k[0].get_device(), "tensors on different devices"
+            assert _cache(a, b, self.device) == k[0].shape and a.dtype is k[0].dtype, "the layers' caches are of one shape and type"
         self.row_bytes = kv_heads * d * k[0].element_size()
         assert self.row_bytes % 16 == 0 and all(t.data_ptr() % 16 == 0 for t in k + v), "a token's keys must be whole 16-byte pieces"
-        self.layers, self.first = len(k), k[0]
+        self.layers = len(k)
         self._tensors = (k, v)
         self.k = (ctypes.c_void_p * len(k))(*[t.data_ptr() for t in k])
         self.v = (ctypes.c_void_p * len(v))(*[t.data_ptr() for t in v])
 
 
-class TreePath(NamedTuple):
+class TreePath:
     """What tree_accept leaves, per row: path [max_path] (accepted nodes, node 0 first, -1 behind them), ids [max_path] int64 (the target's
-    picks along it: the row's new tokens, the last of them not yet in the cache; -1 behind them), counts, lens (ctx_lens + counts)."""
-    path: torch.Tensor
-    ids: torch.Tensor
-    counts: torch.Tensor
-    lens: torch.Tensor
+    picks along it: the row's new tokens, the last of them not yet in the cache; -1 behind them), counts, lens (ctx_lens + counts).  The
+    buffers are checked once, here."""
+    __slots__ = ("_t", "_p", "n_rows", "max_path", "device")
+
+    def __init__(self, path: torch.Tensor, ids: torch.Tensor, counts: torch.Tensor, lens: torch.Tensor):
+        (self.n_rows, self.max_path), self.device = path.shape, path.get_device()
+        assert self.device >= 0, "device tensors expected"
+        assert path.dtype is _I32 and path.is_contiguous()
+        assert ids.shape == path.shape and ids.dtype is _I64 and ids.is_contiguous() and ids.get_device() == self.device
+        self._t = (path, ids, counts, lens)
+        self._p = (path.data_ptr(), ids.data_ptr(), _vec(counts, self.n_rows, self.device), _vec(lens, self.n_rows, self.device))
+
+    path = property(lambda self: self._t[0])
+    ids = property(lambda self: self._t[1])
+    counts = property(lambda self: self._t[2])
+    lens = property(lambda self: self._t[3])
+
+    def __iter__(self):
+        return iter(self._t)
 
     @classmethod
     def empty(cls, rows: int, max_path: int, device) -> "TreePath":
-        return cls(torch.empty(rows, max_path, dtype=torch.int32, device=device), torch.empty(rows, max_path, dtype=torch.int64, device=device),
-                   torch.empty(rows, dtype=torch.int32, device=device), torch.empty(rows, dtype=torch.int32, device=device))
+        return cls(torch.empty(rows, max_path, dtype=_I32, device=device), torch.empty(rows, max_path, dtype=_I64, device=device),
+                   torch.empty(rows, dtype=_I32, device=device), torch.empty(rows, dtype=_I32, device=device))
 
 
 def tree_accept(tokens: torch.Tensor, picks: torch.Tensor, row_start: torch.Tensor, ctx_lens: torch.Tensor, max_nodes: int,
@@ -230,27 +266,20 @@ def tree_accept(tokens: torch.Tensor, picks: torch.Tensor, row_start: torch.Tens
     max_path nodes (default: out's, else max_nodes).  With `caches` the keys and values of the path's j-th node are moved to index
     ctx_lens[b] + j of the sequence in every layer (places without a page: not moved), which is where a sequence of lens[b] tokens has
     them; all of it one launch for up to 64 layers.  A row without nodes has an empty path."""
-    n_tokens, rows = tokens.shape[0], ctx_lens.shape[0]
-    assert tokens.is_cuda and tokens.dtype == torch.int64 and tokens.dim() == 1 and tokens.is_contiguous()
-    assert picks.is_cuda and picks.dtype == torch.int64 and picks.shape == tokens.shape and picks.is_contiguous()
+    n_tokens, rows, dev = tokens.shape[0], ctx_lens.shape[0], _current(tokens)
     assert max_nodes <= MAX_NODES, f"trees go up to {MAX_NODES} nodes a row"
-    if max_path is None:
-        max_path = out.path.shape[1] if out is not None else max(1, max_nodes)
     if out is None:
-        out = TreePath.empty(rows, max_path, tokens.device)
-    assert out.path.shape == (rows, max_path) and out.path.dtype == torch.int32 and out.path.is_contiguous()
-    assert out.ids.shape == (rows, max_path) and out.ids.dtype == torch.int64 and out.ids.is_contiguous()
-    assert rows == 0 or out.lens.data_ptr() != ctx_lens.data_ptr(), "the new lengths may not overwrite the old ones"
-    bt = bt_stride = cols = layers = 0
-    if caches is not None:
-        assert block_table is not None, "moving keys and values takes the block table"
-        bt, bt_stride, cols = _table(block_table, rows)
-        layers = caches.layers
-    _same_device(tokens, picks, parents, row_start, ctx_lens, *out, None if caches is None else caches.first,
-                 None if caches is None else block_table)
+        out = TreePath.empty(rows, max(1, max_nodes) if max_path is None else max_path, tokens.device)
+    assert out.n_rows == rows and out.device == dev and (max_path is None or max_path == out.max_path), "out is of another step's sizes"
+    path, ids, counts, lens = out._p
+    ctx = _vec(ctx_lens, rows, dev)
+    assert lens != ctx or rows == 0, "the new lengths may not overwrite the old ones"
+    if caches is None:
+        move = (None, 0, 0, None, None, 0, 0, 0, 0)
+    else:
+        assert block_table is not None and caches.device == dev, "moving keys and values takes the block table, on the caches' device"
+        move = (*_table(block_table, rows, dev), caches.k, caches.v, caches.layers, caches.row_bytes, caches.page, caches.pages)
     nv.check("mv_tree_accept", nv.lib().mv_tree_accept(
-        tokens.data_ptr(), picks.data_ptr(), None if parents is None else _i32(parents, n_tokens), _i32(row_start, rows + 1),
-        _i32(ctx_lens), bt or None, bt_stride, cols, caches.k if layers else None, caches.v if layers else None, layers,
-        caches.row_bytes if layers else 0, caches.page if layers else 0, caches.pages if layers else 0, rows, n_tokens, int(max_nodes),
-        int(max_path), out.path.data_ptr(), out.ids.data_ptr(), _i32(out.counts, rows), _i32(out.lens, rows), nv.stream_ptr()))
+        _vec(tokens, n_tokens, dev, _I64), _vec(picks, n_tokens, dev, _I64), None if parents is None else _vec(parents, n_tokens, dev),
+        _vec(row_start, rows + 1, dev), ctx, *move, rows, n_tokens, max_nodes, out.max_path, path, ids, counts, lens, nv.stream_ptr()))
     return out
