@@ -65,11 +65,12 @@ FLAGS = [
 FLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
-# per-source additions.  attn_prefill.hip: the pipelined attention deals its vector work out slot
+# per-source additions.  attn_prefill.hip, tree_attn.hip: the pipelined attention deals its vector work out slot
 # by slot beside the MFMAs; the SLP vectoriser would gather the row-sum additions of many slots
 # into one chain of packed additions (slower beside MFMAs than the scalar form, and serial)
 FILE_FLAGS = {
     "attn_prefill.hip": ["-fno-slp-vectorize"],
+    "tree_attn.hip": ["-fno-slp-vectorize"],
 }
 
 

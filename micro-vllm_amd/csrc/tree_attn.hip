@@ -6,6 +6,8 @@
 // keep a softmax state each; the states meet in LDS, the splits' in a second launch that adds them in order.
 #include "common.h"
 
+#include <type_traits>
+
 namespace mv {
 
 constexpr float kTreeNegBig = -1.0e30f;        // a running maximum before any visible key
@@ -13,6 +15,7 @@ constexpr int kTreeMaxNodes = 256;
 constexpr int kTreeMaxWords = kTreeMaxNodes / 64;
 constexpr int kTreeBlock = 16;                 // pages hold whole runs of this many keys
 constexpr int kTreeMaxSplits = 64;
+constexpr int kTreeRunTiles = 4;               // no run of tiles is cut shorter
 
 struct TreeArgs {
     const void *q, *k_cache, *v_cache;
@@ -26,6 +29,7 @@ struct TreeArgs {
     float *part, *state;         // splits: sums [split][token][head][d], (maximum, denominator) [split][token][head]
     int bt_cols, rows, tokens, max_nodes, hq, hkv, g, page, page_shift, num_pages, nsplit, row_blocks;
     int round_keys;              // keys that a split's workgroup takes in one round
+    int wide;
     float scale_log2;
 };
 
@@ -40,10 +44,14 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int b) {
     s.total = (int)min((int64_t)s.ctx + s.n, (int64_t)a.bt_cols << a.page_shift);
     return s;
 }
-// Blocks are dealt to the splits in rounds of one for every wave of a workgroup, so which keys a wave asks for first does not depend on
-// a row's length.  Splits of a row that have any:
+// Up to 64 stacked rows (and fp32): blocks are dealt to the splits in rounds of one for every wave of a workgroup, so which keys a wave asks
+// for first does not depend on a row's length.  More: a split is a run of 64-key tiles.  Tiles of a run, and splits of a row that have any:
+__device__ __forceinline__ int run_tiles(const TreeArgs& a, int total) {
+    return max((((total + 63) >> 6) + a.nsplit - 1) / a.nsplit, kTreeRunTiles);
+}
 __device__ __forceinline__ int filled_splits_tree(const TreeArgs& a, int total) {
-    return max(1, min(a.nsplit, (total + a.round_keys - 1) / a.round_keys));
+    const int round = a.wide ? run_tiles(a, total) * 64 : a.round_keys;
+    return max(1, min(a.nsplit, (total + round - 1) / round));
 }
 // 64 bits of a node's mask from bit `first` (negative: cached tokens in front of the nodes, visible) on
 __device__ __forceinline__ uint64_t mask_from(const uint64_t (&w)[kTreeMaxWords], int first) {
@@ -114,35 +122,38 @@ __device__ __forceinline__ void leave_rows(const TreeArgs& a, const TreeSpan& s,
     }
 }
 
-// Values that are not finite, of keys that some row may not see, were left out of a split's products; here they are added to the sums of a
-// row that sees them: whatever its weight, the result is that infinity or NaN.  `block`: keys that the kernel takes together.  Rare, and
-// slow: a loop over the split's keys.
+// Values that are not finite, of keys that some row may not see, are left out of a split's products; here they are handed, key by key, to
+// the sums of a row that sees them: whatever its weight, the result is that infinity or NaN.  The keys: runs of `span` from `first` on, `step`
+// apart, up to `end`; `block` is how many the kernel takes together (one with nothing to hide went through the product whole).  Rare, and slow.
+template <bool F32, int D, class Take>
+__device__ __forceinline__ void odd_values(const TreeArgs& a, const TreeSpan& s, int b, int kvh, int node, int first, int step, int span,
+                                           int end, int block, Take&& take) {
+    const int32_t* bt = a.block_table + (int64_t)b * a.bt_stride;
+    for (; first < end; first = step > end - first ? end : first + step)
+        for (int key = first; key < min(first + span, end); ++key) {
+            const int pg = bt[key >> a.page_shift], kb = key / block * block;
+            if (pg < 0 || pg >= a.num_pages) continue;
+            if (kb + block <= s.ctx && kb + block <= s.total) {
+                bool there = true;
+                for (int k = kb; k < kb + block; k += kTreeBlock) there &= (unsigned)bt[k >> a.page_shift] < (unsigned)a.num_pages;
+                if (there) continue;
+            }
+            const int j = key - s.ctx;
+            if (j >= 0 && (a.mask ? !(a.mask[(int64_t)(s.start + node) * a.words + (j >> 6)] >> (j & 63) & 1) : j > node)) continue;
+            take((const typename TreeT<F32>::T*)a.v_cache + ((((int64_t)pg << a.page_shift) + (key & (a.page - 1))) * a.hkv + kvh) * D);
+        }
+}
+__device__ __forceinline__ bool is_odd(float x) { return !(fabsf(x) <= 3.4028235e38f); }
+// dimensions c .. c + 3 of a stacked row, of a kernel that deals its blocks
 template <bool F32, int D>
 __device__ __forceinline__ void add_odd(const TreeArgs& a, const TreeSpan& s, int b, int kvh, int split, int block, int sr, int c, f32x4_t& o) {
-    typedef TreeT<F32> X;
-    const int node = sr / a.g, waves = a.round_keys / block;
-    for (int first = split * a.round_keys; first < s.total; first += a.nsplit * a.round_keys)
-        for (int key = first; key < min(first + waves * block, s.total); ++key) {
-            const int pg = a.block_table[(int64_t)b * a.bt_stride + (key >> a.page_shift)];
-            if (pg < 0 || pg >= a.num_pages) continue;
-            const int kb = key / block * block;
-            if (kb + block <= s.ctx) {       // such a block was left out of the products' care only if one of its pages is missing
-                bool there = true;
-                for (int k = kb; k < kb + block; k += kTreeBlock) {
-                    const int p = a.block_table[(int64_t)b * a.bt_stride + min(k >> a.page_shift, a.bt_cols - 1)];
-                    there &= p >= 0 && p < a.num_pages;
-                }
-                if (there && kb + block <= s.total) continue;
-            } else if (key >= s.ctx) {
-                const int j = key - s.ctx;
-                if (a.mask ? !(a.mask[(int64_t)(s.start + node) * a.words + (j >> 6)] >> (j & 63) & 1) : j > node) continue;
-            }
-            const f32x4_t x = X::ld4((const typename X::T*)a.v_cache +
-                                     ((((int64_t)pg << a.page_shift) + (key & (a.page - 1))) * a.hkv + kvh) * D + c);
+    odd_values<F32, D>(a, s, b, kvh, sr / a.g, split * a.round_keys, a.nsplit * a.round_keys, a.round_keys, s.total, block,
+                       [&](const typename TreeT<F32>::T* v) {
+                           const f32x4_t x = TreeT<F32>::ld4(v + c);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (!(fabsf(x[j]) <= 3.4028235e38f)) o[j] += x[j];
-        }
+                           for (int j = 0; j < 4; ++j)
+                               if (is_odd(x[j])) o[j] += x[j];
+                       });
 }
 
 // ------------------------------------------------------------------ fp32
@@ -514,6 +525,416 @@ __global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs 
     }
 }
 
+// ------------------------------------------------------------------ bf16, more rows: 32 a wave, keys shared by the workgroup
+// 256 stacked rows against every 64-key tile in LDS (keys in a ring of three tiles, values of two), one barrier a tile.
+//   * v_mfma_f32_32x32x16_bf16: S^T = K . Q^T leaves a lane (row l & 31, half h = l >> 5) 16 scores of a 32-key block, keys (i & 3) + 8 (i >> 2) +
+//     4 h; registers 8 s .. 8 s + 7, rounded to bf16, are operand B of step s of O^T += V^T . P^T as they stand, and the transposing reads of
+//     V deliver those keys.
+//   * pipeline over 32-key blocks: while the matrix unit forms S of block u + 1 the vector unit turns S of u into weights, while it adds V^T P of
+//     u the vector unit takes the maxima of S of u + 1; LDS reads run a few matrix instructions ahead.  Pieces are dealt out slot by slot between
+//     scheduling fences.
+//   * a tile in which every key counts for every row (all but the one or two with nodes in them) takes no mask.
+// Waves without rows (short trees) only stage.
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+
+__device__ __forceinline__ float max3_tree(float a, float b, float c) {      // (fmaxf of a product's result is a self-maximum more)
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+template <int D>
+__global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
+    constexpr int NT = 512, KT = 64, KS = D / 16, DB = D / 32, NP = 2 * DB;
+    constexpr int PF = 3, PFV = NP - 1 < 7 ? NP - 1 : 7;        // reads of keys and values in front of their matrix instruction
+    constexpr int KROW = D * 2 + 16, VROW = D * 2 + 64, VPR = D / 8, NV = KT * VPR / NT;
+    __shared__ __attribute__((aligned(16))) unsigned char kL[3][KT * KROW];
+    __shared__ __attribute__((aligned(16))) unsigned char vL[2][KT * VROW];
+    __shared__ int oddL;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lq = lane & 31, hi = lane >> 5;
+
+    const int units = a.rows * a.hkv * a.row_blocks, split = blockIdx.x / units, unit = blockIdx.x % units;
+    const int kvh = unit % a.hkv, b = unit / a.hkv % a.rows, rb = unit / (a.hkv * a.rows);
+    const TreeSpan s = tree_span(a, b);
+    // a row's stacked rows in as few parts as 256 allow, of even size
+    const int stacked = s.n * a.g, parts = (stacked + 255) / 256;
+    if (rb >= parts || split >= filled_splits_tree(a, s.total)) return;
+    const int part_rows = ((stacked + parts - 1) / parts + 31) & ~31, row0 = rb * part_rows;
+    if (row0 >= stacked) return;
+    const int tiles = (s.total + KT - 1) / KT, per = run_tiles(a, s.total), t0 = split * per, t1 = min(t0 + per, tiles);
+    const int my_rows = min(part_rows, stacked - row0);
+    const bool active = wid * 32 < my_rows;                     // uniform over the wave
+    const int sr = min(row0 + wid * 32 + lq, stacked - 1), node = sr / a.g, head = kvh * a.g + sr - node * a.g;
+    const bool stored = wid * 32 + lq < my_rows;
+
+    bf16x8_t qf[KS];
+    {
+        const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.start + node) * a.ldq + (int64_t)head * D + hi * 8;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) qf[k] = __builtin_bit_cast(bf16x8_t, ld16(qp + k * 16));
+    }
+    // ---- pages: lane l asks for that of key l of a tile; which keys count is a ballot, a staged row's page an exchange
+    const int32_t* bt = a.block_table + (int64_t)b * a.bt_stride;
+    auto page_ids = [&](int t) __attribute__((always_inline)) {
+        return bt[min((min(t, t1 - 1) * KT + lane) >> a.page_shift, a.bt_cols - 1)];
+    };
+    auto counted = [&](int t, int pg) __attribute__((always_inline)) -> uint64_t {
+        return __builtin_amdgcn_ballot_w64(min(t, t1 - 1) * KT + lane < s.total && (unsigned)pg < (unsigned)a.num_pages);
+    };
+    const int srow0 = threadIdx.x / VPR, srow1 = srow0 + (NV - 1) * (NT / VPR), sch = (threadIdx.x % VPR) * 16;
+    const unsigned row_bytes = (unsigned)a.hkv * D * 2;
+    struct Place {
+        int64_t r0, r1;     // byte offsets of the thread's rows of a tile
+    };
+    auto place = [&](int t, int pg) __attribute__((always_inline)) {
+        const int inside = (unsigned)pg < (unsigned)a.num_pages ? pg : 0, kb = min(t, t1 - 1) * KT;
+        const int p0 = __shfl(inside, srow0, 64), p1 = NV > 1 ? __shfl(inside, srow1, 64) : p0;
+        auto at = [&](int p, int row) __attribute__((always_inline)) {
+            return (((int64_t)p << a.page_shift) + ((kb + row) & (a.page - 1))) * row_bytes + kvh * D * 2 + sch;
+        };
+        return Place{at(p0, srow0), at(p1, srow1)};
+    };
+    struct Stage {
+        u32x4_t r0, r1;
+    };
+    auto g_load = [&](Stage& st, const void* cache, const Place& p) __attribute__((always_inline)) {
+        st.r0 = *reinterpret_cast<const u32x4_t*>((const unsigned char*)cache + p.r0);
+        if constexpr (NV > 1) st.r1 = *reinterpret_cast<const u32x4_t*>((const unsigned char*)cache + p.r1);
+    };
+    auto k_store = [&](const Stage& st, int buf, int which) __attribute__((always_inline)) {
+        if (which == 0) *reinterpret_cast<u32x4_t*>(&kL[buf][srow0 * KROW + sch]) = st.r0;
+        if (NV > 1 && which == 1) *reinterpret_cast<u32x4_t*>(&kL[buf][srow1 * KROW + sch]) = st.r1;
+    };
+    auto v_store = [&](const Stage& st, int buf, int which) __attribute__((always_inline)) {
+        if (which == 0) *reinterpret_cast<u32x4_t*>(&vL[buf][srow0 * VROW + sch]) = st.r0;
+        if (NV > 1 && which == 1) *reinterpret_cast<u32x4_t*>(&vL[buf][srow1 * VROW + sch]) = st.r1;
+    };
+    // values of keys that do not count become zero, and what is not finite of the others is left for the end
+    bool odd = false;
+    auto clean = [&](Stage& st, uint64_t bits) __attribute__((always_inline)) {
+        auto one = [&](u32x4_t& v, int row) __attribute__((always_inline)) {
+            if (!(bits >> row & 1)) v = (u32x4_t){0, 0, 0, 0};
+            uint32_t w[4] = {v[0], v[1], v[2], v[3]};
+            const bool o0 = drop_odd(w[0]), o1 = drop_odd(w[1]), o2 = drop_odd(w[2]), o3 = drop_odd(w[3]);
+            odd |= o0 | o1 | o2 | o3;
+            v = (u32x4_t){w[0], w[1], w[2], w[3]};
+        };
+        one(st.r0, srow0);
+        if constexpr (NV > 1) one(st.r1, srow1);
+    };
+    auto open_tile = [&](int t, uint64_t bits) __attribute__((always_inline)) { return bits == ~0ull && (t + 1) * KT <= s.ctx; };
+    // which of a tile's keys the lane's row sees
+    auto visible = [&](int t, uint64_t bits) __attribute__((always_inline)) -> uint64_t {
+        const int first = t * KT - s.ctx;
+        if (first <= -KT) return bits;
+        if (!a.mask) {
+            const int up = node + 1 - first;
+            return bits & (up >= 64 ? ~0ull : (1ull << max(up, 0)) - 1);
+        }
+        const uint64_t* w = a.mask + (int64_t)(s.start + node) * a.words;
+        if (first < 0) return bits & ((w[0] << -first) | ((1ull << -first) - 1));
+        const int at = first >> 6, sh = first & 63;
+        uint64_t v = at < a.words ? w[at] >> sh : 0;
+        if (sh && at + 1 < a.words) v |= w[at + 1] << (64 - sh);
+        return bits & v;
+    };
+
+    // ---- fragments
+    const int k_off = lq * KROW + hi * 16, li = lane & 15;
+    const int tr_off = (4 * hi + (li >> 2)) * VROW + (16 * ((lane >> 4) & 1) + 4 * (li & 3)) * 2;
+    auto k_frag = [&](const unsigned char* kblock, int k) __attribute__((always_inline)) {
+        return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(kblock + k * 32 + k_off));
+    };
+    auto v_frag = [&](const unsigned char* vblock, int j) __attribute__((always_inline)) {      // step j / DB, rows 32 (j % DB) of O^T
+        const unsigned char* vb = vblock + (j / DB) * 16 * VROW + (j % DB) * 64 + tr_off;
+        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(vb));
+        const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(vb + 8 * VROW));
+        const s16x8_t both = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
+        return __builtin_bit_cast(bf16x8_t, both);
+    };
+
+    f32x16_t oacc[DB];
+    float mrun = kTreeNegBig, lrun0 = 0.f, lrun1 = 0.f, alpha = 1.f;
+    bool rescale = false;
+    uint32_t pw[8];
+    float fa[8][2], eb[8][2];
+    auto softmax_slot = [&](const f32x16_t& sc, int at) __attribute__((always_inline)) {      // three stages of a pair of scores, a slot apart
+        constexpr int kEnter128[8] = {1, 2, 3, 4, 5, 6, 7, 8}, kEnter64[8] = {1, 1, 1, 1, 2, 2, 3, 3};
+#pragma unroll
+        for (int pr = 0; pr < 8; ++pr)
+            if (at == (D == 128 ? kEnter128[pr] : kEnter64[pr]) + 2) {
+                lrun0 += eb[pr][0];
+                lrun1 += eb[pr][1];
+                pw[pr] = pack_bf16x2(eb[pr][0], eb[pr][1]);
+            }
+#pragma unroll
+        for (int pr = 0; pr < 8; ++pr)
+            if (at == (D == 128 ? kEnter128[pr] : kEnter64[pr]) + 1) {
+                eb[pr][0] = __builtin_amdgcn_exp2f(fa[pr][0]);
+                eb[pr][1] = __builtin_amdgcn_exp2f(fa[pr][1]);
+            }
+#pragma unroll
+        for (int pr = 0; pr < 8; ++pr)
+            if (at == (D == 128 ? kEnter128[pr] : kEnter64[pr])) {
+                fa[pr][0] = __builtin_fmaf(sc[2 * pr], a.scale_log2, -mrun);
+                fa[pr][1] = __builtin_fmaf(sc[2 * pr + 1], a.scale_log2, -mrun);
+            }
+    };
+    auto p_frag = [&](int st) __attribute__((always_inline)) {
+        return __builtin_bit_cast(bf16x8_t, make_uint4(pw[4 * st], pw[4 * st + 1], pw[4 * st + 2], pw[4 * st + 3]));
+    };
+    float m2[2];
+    // a quarter of a block's maximum; masked: `vis` (shifted by 4 hi) has the row's keys
+    auto max_piece = [&](f32x16_t& sn, int mi, uint32_t vis, auto masked) __attribute__((always_inline)) {
+        constexpr int from[5] = {0, 6, 10, 14, 16};
+        if constexpr (decltype(masked)::value) {
+#pragma unroll
+            for (int i = from[mi]; i < from[mi + 1]; ++i)
+                if (!(vis >> ((i & 3) + 8 * (i >> 2)) & 1)) sn[i] = -__builtin_inff();
+        }
+        if (mi == 0) {
+            m2[0] = max3_tree(sn[0], sn[1], sn[2]);
+            m2[1] = max3_tree(sn[3], sn[4], sn[5]);
+        } else if (mi == 1) {
+            m2[0] = max3_tree(m2[0], sn[6], sn[7]);
+            m2[1] = max3_tree(m2[1], sn[8], sn[9]);
+        } else if (mi == 2) {
+            m2[0] = max3_tree(m2[0], sn[10], sn[11]);
+            m2[1] = max3_tree(m2[1], sn[12], sn[13]);
+        } else {
+            m2[0] = max3_tree(m2[0], sn[14], sn[15]);
+        }
+    };
+    auto max_finish = [&]() __attribute__((always_inline)) {
+        const unsigned u = __float_as_uint(fmaxf(m2[0], m2[1]) * a.scale_log2);
+        const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const float mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        rescale = __builtin_amdgcn_ballot_w64(mloc > mrun) != 0;
+        if (rescale) {
+            const float mnew = fmaxf(mrun, mloc);
+            alpha = __builtin_amdgcn_exp2f(mrun - mnew);
+            mrun = mnew;
+        }
+    };
+    auto apply_rescale = [&]() __attribute__((always_inline)) {
+        if (rescale) {
+            lrun0 *= alpha;
+            lrun1 *= alpha;
+            typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+            const f32x2_t a2 = {alpha, alpha};
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const f32x2_t o2 = f32x2_t{oacc[db][i], oacc[db][i + 1]} * a2;
+                    oacc[db][i] = o2[0];
+                    oacc[db][i + 1] = o2[1];
+                }
+        }
+    };
+    // Block u (scores sc, maximum pieces taken): weights, O += V^T P; scores of block u + 1 (keys at kblock) into sn.  kpre: its first reads, made
+    // during the step before, refilled from kblock_after.  hook(slot) in every slot.
+    bf16x8_t kpre[PF];
+    auto block_step = [&](const f32x16_t& sc, f32x16_t& sn, const unsigned char* kblock, const unsigned char* vblock,
+                          const unsigned char* kblock_after, uint32_t vis_next, auto has_next, auto has_after, auto mask_next,
+                          auto&& hook) __attribute__((always_inline)) {
+        constexpr bool kNext = decltype(has_next)::value, kAfter = decltype(has_after)::value;
+        max_finish();
+        apply_rescale();
+        bf16x8_t kf[KS], vf[NP];
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (kNext) {
+                if (i < PF) kf[i] = kpre[i];
+                if (i + PF < KS) kf[i + PF] = k_frag(kblock, i + PF);
+                const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i], qf[i], i == 0 ? zero : sn, 0, 0, 0);
+            }
+            if (i + PFV >= KS) vf[i + PFV - KS] = v_frag(vblock, i + PFV - KS);
+            softmax_slot(sc, i);
+            hook(i);
+        }
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (j + PFV < NP) vf[j + PFV] = v_frag(vblock, j + PFV);
+            if constexpr (kAfter) {
+                if (j + PF >= NP) kpre[j + PF - NP] = k_frag(kblock_after, j + PF - NP);
+            }
+            oacc[j % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j], p_frag(j / DB), oacc[j % DB], 0, 0, 0);
+            softmax_slot(sc, KS + j);
+            if constexpr (kNext) {
+                if (j >= DB) {
+#pragma unroll
+                    for (int mi = (j - DB) * 4 / DB; mi < (j - DB + 1) * 4 / DB; ++mi) max_piece(sn, mi, vis_next, mask_next);
+                }
+            }
+            hook(KS + j);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto no_hook = [](int) __attribute__((always_inline)) {};
+    const std::true_type yes{};
+    const std::false_type no{};
+
+    // ---- prologue: K(t0), V(t0), K(t0 + 1) staged, S of the first block and its maxima
+    Stage sk, sv;
+    Place at1, at2;
+    uint64_t bits0, bits1, bits2;      // keys that count in tiles t, t + 1, t + 2
+    int open_end = min(t1, s.ctx / KT);      // tiles in front of this one take no mask, as far as their pages are known
+    int pg3;
+    {
+        const int p0 = page_ids(t0), p1 = page_ids(t0 + 1), p2 = page_ids(t0 + 2);
+        pg3 = page_ids(t0 + 3);
+        const Place at0 = place(t0, p0);
+        bits0 = counted(t0, p0);
+        at1 = place(t0 + 1, p1);
+        bits1 = counted(t0 + 1, p1);
+        at2 = place(t0 + 2, p2);
+        bits2 = counted(t0 + 2, p2);
+        if (bits2 != ~0ull) open_end = min(open_end, t0 + 2);
+        if (bits1 != ~0ull) open_end = min(open_end, t0 + 1);
+        if (bits0 != ~0ull) open_end = min(open_end, t0);
+        if (threadIdx.x == 0) oddL = 0;
+        Stage s2;
+        g_load(sk, a.k_cache, at0);
+        g_load(sv, a.v_cache, at0);
+        g_load(s2, a.k_cache, at1);
+        k_store(sk, 0, 0);
+        k_store(sk, 0, 1);
+        if (!open_tile(t0, bits0)) clean(sv, bits0);
+        v_store(sv, 0, 0);
+        v_store(sv, 0, 1);
+        k_store(s2, 1, 0);
+        k_store(s2, 1, 1);
+    }
+    __syncthreads();
+
+    int kc = 0, kn = 1, kw = 2;        // ring slots of K(t), K(t + 1), K(t + 2)
+    // K(t + 2), V(t + 1) and the page numbers of tile t + 4: a whole step to arrive
+    auto request = [&](int t) __attribute__((always_inline)) {
+        const int pg4 = page_ids(t + 4);
+        g_load(sk, a.k_cache, at2);
+        g_load(sv, a.v_cache, at1);
+        at1 = at2;
+        at2 = place(t + 3, pg3);
+        const uint64_t bits3 = counted(t + 3, pg3);
+        pg3 = pg4;
+        if (bits3 != ~0ull) open_end = min(open_end, t + 3);
+        return bits3;
+    };
+    auto turn = [&](uint64_t bits3) __attribute__((always_inline)) {
+        bits0 = bits1;
+        bits1 = bits2;
+        bits2 = bits3;
+        const int k_old = kc;
+        kc = kn;
+        kn = kw;
+        kw = k_old;
+        __syncthreads();
+    };
+    if (!active) {       // a wave without rows stages its part of every tile
+        for (int t = t0; t + 1 < t1; ++t) {
+            const uint64_t bits3 = request(t);
+            k_store(sk, kw, 0);
+            k_store(sk, kw, 1);
+            if (!open_tile(t + 1, bits1)) clean(sv, bits1);
+            v_store(sv, (t - t0 + 1) & 1, 0);
+            v_store(sv, (t - t0 + 1) & 1, 1);
+            turn(bits3);
+        }
+        if (odd) oddL = 1;
+        __syncthreads();
+        return;
+    }
+
+
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) oacc[db][i] = 0.f;
+    f32x16_t s0, s1;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s0[i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(&kL[0][0], k), qf[k], s0, 0, 0, 0);
+    {
+        const uint32_t vis = (uint32_t)visible(t0, bits0) >> (4 * hi);
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi) max_piece(s0, mi, vis, yes);
+    }
+#pragma unroll
+    for (int k = 0; k < PF; ++k) kpre[k] = k_frag(&kL[0][0] + 32 * KROW, k);
+    if (wid >= 4) __builtin_amdgcn_s_setprio(1);      // (the later waves of a SIMD lose every arbitration by age otherwise)
+    auto tile_step = [&](int t, auto masks) __attribute__((always_inline)) {
+        constexpr bool kMask = decltype(masks)::value;
+        const int buf = (t - t0) & 1;
+        const unsigned char *kcur = &kL[kc][0], *knext = &kL[kn][0], *vcur = &vL[buf][0];
+        const uint64_t bits3 = request(t);
+        uint32_t vis1 = 0, vis2 = 0;
+        if constexpr (kMask) {
+            vis1 = (uint32_t)(visible(t, bits0) >> 32) >> (4 * hi);
+            vis2 = (uint32_t)visible(t + 1, bits1) >> (4 * hi);
+        }
+        block_step(s0, s1, kcur + 32 * KROW, vcur, knext, vis1, yes, yes, masks, no_hook);
+        const int kdst = kw, vdst = buf ^ 1;
+        if constexpr (kMask) {
+            if (!open_tile(t + 1, bits1)) clean(sv, bits1);
+        }
+        block_step(s1, s0, knext, vcur + 32 * VROW, knext + 32 * KROW, vis2, yes, yes, masks, [&](int at) __attribute__((always_inline)) {
+            const int k = at - (KS + NP - 2 * NV);      // the stores beside the last matrix instructions
+            if (k >= 0 && k < NV) k_store(sk, kdst, k);
+            if (k >= NV && k < 2 * NV) v_store(sv, vdst, k - NV);
+        });
+        turn(bits3);
+    };
+    int t = t0;
+    for (; t + 1 < open_end; ++t) tile_step(t, no);
+    for (; t + 1 < t1; ++t) tile_step(t, yes);
+    {   // the last tile: nothing follows its second block
+        const uint32_t vis1 = (uint32_t)(visible(t, bits0) >> 32) >> (4 * hi);
+        const unsigned char* vcur = &vL[(t - t0) & 1][0];
+        block_step(s0, s1, &kL[kc][0] + 32 * KROW, vcur, nullptr, vis1, yes, no, yes, no_hook);
+        block_step(s1, s0, &kL[kc][0], vcur + 32 * VROW, nullptr, 0, no, no, no, no_hook);
+    }
+    if (odd) oddL = 1;
+    __syncthreads();
+    if (!stored) return;
+    // oacc[db][i] = O^T[32 db + (i & 3) + 8 (i >> 2) + 4 hi][row]
+    if (oddL)
+        odd_values<false, D>(a, s, b, kvh, node, t0 * KT, 1 << 30, 1 << 30, min(t1 * KT, s.total), KT, [&](const uint16_t* v) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f32x4_t x = TreeT<false>::ld4(v + 32 * db + 8 * k + 4 * hi);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (is_odd(x[j])) oacc[db][4 * k + j] += x[j];
+                }
+        });
+    const float den = lrun0 + lrun1 + __shfl_xor(lrun0 + lrun1, 32, 64);
+    const bool whole = filled_splits_tree(a, s.total) <= 1;
+    const int64_t tok = s.start + node;
+    const float inv = den != 0.f ? 1.0f / den : 0.f;
+    const int64_t at = ((int64_t)split * a.tokens + tok) * a.hq + head;
+    uint16_t* op = (uint16_t*)a.out + tok * a.ldo + (int64_t)head * D + 4 * hi;
+    float* pp = a.part + at * D + 4 * hi;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const f32x4_t o = {oacc[db][4 * k], oacc[db][4 * k + 1], oacc[db][4 * k + 2], oacc[db][4 * k + 3]};
+            if (whole) TreeT<false>::st4(op + 32 * db + 8 * k, o * inv);
+            else *reinterpret_cast<f32x4_t*>(pp + 32 * db + 8 * k) = o;
+        }
+    if (!whole && hi == 0) {
+        a.state[2 * at] = mrun;
+        a.state[2 * at + 1] = den;
+    }
+}
+
 // Splits added in order; rows that one split holds are written already.
 template <bool F32, int D>
 __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
@@ -541,14 +962,16 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
 
 // Rows, workgroups and keys of a launch
 struct TreeForm {
-    int row_tiles, row_blocks, round_keys;
+    int row_tiles, row_blocks, round_keys, wide;
 };
 static TreeForm tree_form(int max_nodes, int g, int d, int f32) {
     const int64_t stacked = (int64_t)max_nodes * g;
     TreeForm f;
+    f.wide = !f32 && stacked > 64;
     f.row_tiles = f32 ? 2 : stacked <= 16 ? 1 : stacked <= 32 ? 2 : 4;
-    f.row_blocks = (int)((stacked + 16 * f.row_tiles - 1) / (16 * f.row_tiles));
-    f.round_keys = f32 ? 64 : 128;
+    const int rows = f.wide ? 256 : 16 * f.row_tiles;
+    f.row_blocks = (int)((stacked + rows - 1) / rows);
+    f.round_keys = f.wide ? 64 * kTreeRunTiles : f32 ? 64 : 128;
     return f;
 }
 
@@ -620,6 +1043,7 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     const TreeForm f = tree_form(max_nodes, a.g, d, f32);
     a.row_blocks = f.row_blocks;
     a.round_keys = f.round_keys;
+    a.wide = f.wide;
     a.scale_log2 = scale * 1.4426950408889634f;
     const int64_t grid = (int64_t)rows * hkv * a.row_blocks * num_splits;
     if (grid > 0x7fffffff || rows > 65535) return MV_ERR_UNSUPPORTED;
@@ -628,6 +1052,8 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
 #define MV_TREE(K_, T_) hipLaunchKernelGGL((K_), g1, dim3(T_), 0, s, a)
     if (f32 && d == 64) MV_TREE((tree_attn_f32_kernel<64>), 256);
     else if (f32) MV_TREE((tree_attn_f32_kernel<128>), 256);
+    else if (f.wide && d == 64) MV_TREE((tree_attn_wide_kernel<64>), 512);
+    else if (f.wide) MV_TREE((tree_attn_wide_kernel<128>), 512);
     else if (d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<64, 1, 1>), 256);
     else if (d == 64 && f.row_tiles == 2) MV_TREE((tree_attn_narrow_kernel<64, 2, 1>), 256);
     else if (d == 64) MV_TREE((tree_attn_narrow_kernel<64, 4, 1>), 256);
