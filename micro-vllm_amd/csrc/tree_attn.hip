@@ -11,6 +11,10 @@
 namespace mv {
 
 constexpr float kTreeNegBig = -1.0e30f;        // a running maximum before any visible key
+// A row's running maximum is raised only when a score outgrows it by this many powers of two: weights are then up to 2^6 instead of up to
+// one, the sums have 32 bits for that, and a weight's rounding to bf16 is relative.  With the exact maximum some row of a wave outgrows its own
+// in most blocks, and every accumulator is multiplied for it.
+constexpr float kTreeRaise = 6.0f;
 constexpr int kTreeMaxNodes = 256;
 constexpr int kTreeMaxWords = kTreeMaxNodes / 64;
 constexpr int kTreeBlock = 16;                 // pages hold whole runs of this many keys
@@ -464,7 +468,7 @@ __global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs 
             float top = fmaxf(fmaxf(fmaxf(sc[i][0][0], sc[i][0][1]), fmaxf(sc[i][0][2], sc[i][0][3])),
                               fmaxf(fmaxf(sc[i][1][0], sc[i][1][1]), fmaxf(sc[i][1][2], sc[i][1][3]))) * a.scale_log2;
             top = max_of_quarters(top);
-            if (__builtin_amdgcn_ballot_w64(top > m[i]) != 0) {      // (else a factor of one for every row)
+            if (__builtin_amdgcn_ballot_w64(top > m[i] + kTreeRaise) != 0) {
                 const float mn = fmaxf(m[i], top), alpha = __builtin_amdgcn_exp2f(m[i] - mn);
                 m[i] = mn;
                 l[i] *= alpha;
@@ -526,7 +530,8 @@ __global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs 
 }
 
 // ------------------------------------------------------------------ bf16, more rows: 32 a wave, keys shared by the workgroup
-// 256 stacked rows against every 64-key tile in LDS (keys in a ring of three tiles, values of two), one barrier a tile.
+// 256 stacked rows against every 64-key tile in LDS, one barrier a tile.  Keys and values go there by global_load_lds, three and two whole
+// tiles' time ahead (rings of five and four tiles: no staging registers, and a trip to memory under load is one to two of those times).
 //   * v_mfma_f32_32x32x16_bf16: S^T = K . Q^T leaves a lane (row l & 31, half h = l >> 5) 16 scores of a 32-key block, keys (i & 3) + 8 (i >> 2) +
 //     4 h; registers 8 s .. 8 s + 7, rounded to bf16, are operand B of step s of O^T += V^T . P^T as they stand, and the transposing reads of
 //     V deliver those keys.
@@ -543,14 +548,20 @@ __device__ __forceinline__ float max3_tree(float a, float b, float c) {      // 
     return r;
 }
 
+// all but the youngest N requests have landed
+template <int N>
+__device__ __forceinline__ void wait_landed() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
 template <int D>
 __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
-    constexpr int NT = 512, KT = 64, KS = D / 16, DB = D / 32, NP = 2 * DB;
+    constexpr int KT = 64, KS = D / 16, DB = D / 32, NP = 2 * DB;
     constexpr int PF = 3, PFV = NP - 1 < 7 ? NP - 1 : 7;        // reads of keys and values in front of their matrix instruction
-    constexpr int KROW = D * 2 + 16, VROW = D * 2 + 64, VPR = D / 8, NV = KT * VPR / NT;
-    __shared__ __attribute__((aligned(16))) unsigned char kL[3][KT * KROW];
-    __shared__ __attribute__((aligned(16))) unsigned char vL[2][KT * VROW];
+    constexpr int KD = 4, VD = 3, RB = D * 2, TB = KT * RB, VPR = D / 8, NI = TB / 8192;      // NI: requests of a wave for a tile
+    __shared__ __attribute__((aligned(16))) unsigned char ring[(KD + 1 + VD + 1) * TB];
     __shared__ int oddL;
+    unsigned char *const kring = ring, *const vring = ring + (KD + 1) * TB;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lq = lane & 31, hi = lane >> 5;
 
     const int units = a.rows * a.hkv * a.row_blocks, split = blockIdx.x / units, unit = blockIdx.x % units;
@@ -573,54 +584,70 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
 #pragma unroll
         for (int k = 0; k < KS; ++k) qf[k] = __builtin_bit_cast(bf16x8_t, ld16(qp + k * 16));
     }
-    // ---- pages: lane l asks for that of key l of a tile; which keys count is a ballot, a staged row's page an exchange
-    const int32_t* bt = a.block_table + (int64_t)b * a.bt_stride;
+    // ---- pages: the four runs of 16 keys of a tile lie in a page each; a wave stages eight rows, of one run
+    typedef const int32_t __attribute__((address_space(4))) Entry;      // (nothing here writes the table: scalar loads)
+    Entry* bt = (Entry*)(uintptr_t)(a.block_table + (int64_t)b * a.bt_stride);
+    struct Pages {
+        int p[4];
+    };
     auto page_ids = [&](int t) __attribute__((always_inline)) {
-        return bt[min((min(t, t1 - 1) * KT + lane) >> a.page_shift, a.bt_cols - 1)];
+        Pages r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.p[i] = bt[min((min(t, t1 - 1) * KT + 16 * i) >> a.page_shift, a.bt_cols - 1)];
+        return r;
     };
-    auto counted = [&](int t, int pg) __attribute__((always_inline)) -> uint64_t {
-        return __builtin_amdgcn_ballot_w64(min(t, t1 - 1) * KT + lane < s.total && (unsigned)pg < (unsigned)a.num_pages);
+    auto counted = [&](int t, const Pages& g) __attribute__((always_inline)) {      // keys of a tile that count
+        uint64_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bits |= (unsigned)g.p[i] < (unsigned)a.num_pages ? 0xffffull << (16 * i) : 0;
+        const int left = s.total - min(t, t1 - 1) * KT;
+        return left < KT ? bits & ((1ull << left) - 1) : bits;
     };
-    const int srow0 = threadIdx.x / VPR, srow1 = srow0 + (NV - 1) * (NT / VPR), sch = (threadIdx.x % VPR) * 16;
-    const unsigned row_bytes = (unsigned)a.hkv * D * 2;
-    struct Place {
-        int64_t r0, r1;     // byte offsets of the thread's rows of a tile
+    const unsigned row_bytes = (unsigned)a.hkv * RB;
+    auto base_of = [&](int t, const Pages& g) __attribute__((always_inline)) {      // byte offset in either cache of the wave's first row
+        const int run = wid >> 1, pg = run == 0 ? g.p[0] : run == 1 ? g.p[1] : run == 2 ? g.p[2] : g.p[3];
+        const int64_t row = ((int64_t)((unsigned)pg < (unsigned)a.num_pages ? pg : 0) << a.page_shift) + ((min(t, t1 - 1) * KT + 8 * wid) & (a.page - 1));
+        return row * row_bytes + kvh * RB;
     };
-    auto place = [&](int t, int pg) __attribute__((always_inline)) {
-        const int inside = (unsigned)pg < (unsigned)a.num_pages ? pg : 0, kb = min(t, t1 - 1) * KT;
-        const int p0 = __shfl(inside, srow0, 64), p1 = NV > 1 ? __shfl(inside, srow1, 64) : p0;
-        auto at = [&](int p, int row) __attribute__((always_inline)) {
-            return (((int64_t)p << a.page_shift) + ((kb + row) & (a.page - 1))) * row_bytes + kvh * D * 2 + sch;
-        };
-        return Place{at(p0, srow0), at(p1, srow1)};
+    // The LDS image of a tile is its rows back to back; 16-byte piece c of row r stands at c ^ k_turn(r) (keys: operand reads of 16 rows) or
+    // c ^ v_turn(r) (values: transposing reads of four pieces of four rows), which keeps the reads free of bank conflicts.  A request of a
+    // wave is a KB of the image; the lanes ask for the pieces that belong there.
+    auto k_turn = [](int r) __attribute__((always_inline)) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+    auto v_turn = [](int r) __attribute__((always_inline)) { return D == 128 ? (r & 3) << 2 : (r >> 1 & 1) << 2; };
+    unsigned k_from[NI], v_from[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int r = 8 * wid + i * (64 / VPR) + lane / VPR, c = lane % VPR;
+        k_from[i] = (r & 7) * row_bytes + (c ^ k_turn(r)) * 16;
+        v_from[i] = (r & 7) * row_bytes + (c ^ v_turn(r)) * 16;
+    }
+    // (through inline assembly: seen by the compiler, these loads make it wait for all of them in front of every LDS read)
+    auto copy = [&](const void* cache, int64_t base, unsigned from, const unsigned char* to) __attribute__((always_inline)) {
+        const unsigned dst = (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned char*)to;
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                     : : "v"(from), "s"((const unsigned char*)cache + base), "s"(dst) : "memory");
     };
-    struct Stage {
-        u32x4_t r0, r1;
+    auto copy_k = [&](int64_t base, int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) copy(a.k_cache, base, k_from[i], kring + slot * TB + wid * 8 * RB + i * 1024);
     };
-    auto g_load = [&](Stage& st, const void* cache, const Place& p) __attribute__((always_inline)) {
-        st.r0 = *reinterpret_cast<const u32x4_t*>((const unsigned char*)cache + p.r0);
-        if constexpr (NV > 1) st.r1 = *reinterpret_cast<const u32x4_t*>((const unsigned char*)cache + p.r1);
+    auto copy_v = [&](int64_t base, int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) copy(a.v_cache, base, v_from[i], vring + slot * TB + wid * 8 * RB + i * 1024);
     };
-    auto k_store = [&](const Stage& st, int buf, int which) __attribute__((always_inline)) {
-        if (which == 0) *reinterpret_cast<u32x4_t*>(&kL[buf][srow0 * KROW + sch]) = st.r0;
-        if (NV > 1 && which == 1) *reinterpret_cast<u32x4_t*>(&kL[buf][srow1 * KROW + sch]) = st.r1;
-    };
-    auto v_store = [&](const Stage& st, int buf, int which) __attribute__((always_inline)) {
-        if (which == 0) *reinterpret_cast<u32x4_t*>(&vL[buf][srow0 * VROW + sch]) = st.r0;
-        if (NV > 1 && which == 1) *reinterpret_cast<u32x4_t*>(&vL[buf][srow1 * VROW + sch]) = st.r1;
-    };
-    // values of keys that do not count become zero, and what is not finite of the others is left for the end
+    // values of keys that do not count become zero, and what is not finite of the others is left for the end: in the pieces that this wave asked
+    // for, once they are there
     bool odd = false;
-    auto clean = [&](Stage& st, uint64_t bits) __attribute__((always_inline)) {
-        auto one = [&](u32x4_t& v, int row) __attribute__((always_inline)) {
-            if (!(bits >> row & 1)) v = (u32x4_t){0, 0, 0, 0};
-            uint32_t w[4] = {v[0], v[1], v[2], v[3]};
-            const bool o0 = drop_odd(w[0]), o1 = drop_odd(w[1]), o2 = drop_odd(w[2]), o3 = drop_odd(w[3]);
+    auto clean = [&](int slot, uint64_t bits) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            uint4* at = reinterpret_cast<uint4*>(vring + slot * TB + wid * 8 * RB + i * 1024 + lane * 16);
+            uint4 v = *at;
+            if (!(bits >> (8 * wid + i * (64 / VPR) + lane / VPR) & 1)) v = make_uint4(0, 0, 0, 0);
+            const bool o0 = drop_odd(v.x), o1 = drop_odd(v.y), o2 = drop_odd(v.z), o3 = drop_odd(v.w);
             odd |= o0 | o1 | o2 | o3;
-            v = (u32x4_t){w[0], w[1], w[2], w[3]};
-        };
-        one(st.r0, srow0);
-        if constexpr (NV > 1) one(st.r1, srow1);
+            *at = v;
+        }
     };
     auto open_tile = [&](int t, uint64_t bits) __attribute__((always_inline)) { return bits == ~0ull && (t + 1) * KT <= s.ctx; };
     // which of a tile's keys the lane's row sees
@@ -640,15 +667,16 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
     };
 
     // ---- fragments
-    const int k_off = lq * KROW + hi * 16, li = lane & 15;
-    const int tr_off = (4 * hi + (li >> 2)) * VROW + (16 * ((lane >> 4) & 1) + 4 * (li & 3)) * 2;
+    const int li = lane & 15, v_row = 4 * hi + (li >> 2);
+    const unsigned k_at = lq * RB + ((hi ^ k_turn(lq)) * 16);
+    const unsigned v_at = v_row * RB + ((2 * ((lane >> 4) & 1) + ((li & 3) >> 1)) ^ v_turn(v_row)) * 16 + (li & 1) * 8;
     auto k_frag = [&](const unsigned char* kblock, int k) __attribute__((always_inline)) {
-        return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(kblock + k * 32 + k_off));
+        return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(kblock + (k_at ^ (32 * k))));
     };
     auto v_frag = [&](const unsigned char* vblock, int j) __attribute__((always_inline)) {      // step j / DB, rows 32 (j % DB) of O^T
-        const unsigned char* vb = vblock + (j / DB) * 16 * VROW + (j % DB) * 64 + tr_off;
+        const unsigned char* vb = vblock + (j / DB) * 16 * RB + (v_at ^ (64 * (j % DB)));
         const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(vb));
-        const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(vb + 8 * VROW));
+        const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(vb + 8 * RB));
         const s16x8_t both = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
         return __builtin_bit_cast(bf16x8_t, both);
     };
@@ -709,7 +737,7 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
         const unsigned u = __float_as_uint(fmaxf(m2[0], m2[1]) * a.scale_log2);
         const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
         const float mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-        rescale = __builtin_amdgcn_ballot_w64(mloc > mrun) != 0;
+        rescale = __builtin_amdgcn_ballot_w64(mloc > mrun + kTreeRaise) != 0;
         if (rescale) {
             const float mnew = fmaxf(mrun, mloc);
             alpha = __builtin_amdgcn_exp2f(mrun - mnew);
@@ -733,11 +761,11 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
         }
     };
     // Block u (scores sc, maximum pieces taken): weights, O += V^T P; scores of block u + 1 (keys at kblock) into sn.  kpre: its first reads, made
-    // during the step before, refilled from kblock_after.  hook(slot) in every slot.
+    // during the step before, refilled from kblock_after.
     bf16x8_t kpre[PF];
     auto block_step = [&](const f32x16_t& sc, f32x16_t& sn, const unsigned char* kblock, const unsigned char* vblock,
-                          const unsigned char* kblock_after, uint32_t vis_next, auto has_next, auto has_after, auto mask_next,
-                          auto&& hook) __attribute__((always_inline)) {
+                          const unsigned char* kblock_after, uint32_t vis_next, auto has_next, auto has_after,
+                          auto mask_next) __attribute__((always_inline)) {
         constexpr bool kNext = decltype(has_next)::value, kAfter = decltype(has_after)::value;
         max_finish();
         apply_rescale();
@@ -753,7 +781,6 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
             }
             if (i + PFV >= KS) vf[i + PFV - KS] = v_frag(vblock, i + PFV - KS);
             softmax_slot(sc, i);
-            hook(i);
         }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
@@ -770,85 +797,75 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
                     for (int mi = (j - DB) * 4 / DB; mi < (j - DB + 1) * 4 / DB; ++mi) max_piece(sn, mi, vis_next, mask_next);
                 }
             }
-            hook(KS + j);
         }
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto no_hook = [](int) __attribute__((always_inline)) {};
     const std::true_type yes{};
     const std::false_type no{};
 
-    // ---- prologue: K(t0), V(t0), K(t0 + 1) staged, S of the first block and its maxima
-    Stage sk, sv;
-    Place at1, at2;
-    uint64_t bits0, bits1, bits2;      // keys that count in tiles t, t + 1, t + 2
-    int open_end = min(t1, s.ctx / KT);      // tiles in front of this one take no mask, as far as their pages are known
-    int pg3;
+    // ---- prologue: keys of KD and values of VD tiles asked for, S of the first block and its maxima
+    // bits[i]: keys that count in tile t + i.  open_end: tiles in front of this one take no mask, as far as their pages are known
+    uint64_t bits[KD];
+    int64_t v_base[KD - VD];           // of tiles t + VD .., whose keys have been asked for
+    int open_end = min(t1, s.ctx / KT);
+    if (threadIdx.x == 0) oddL = 0;
     {
-        const int p0 = page_ids(t0), p1 = page_ids(t0 + 1), p2 = page_ids(t0 + 2);
-        pg3 = page_ids(t0 + 3);
-        const Place at0 = place(t0, p0);
-        bits0 = counted(t0, p0);
-        at1 = place(t0 + 1, p1);
-        bits1 = counted(t0 + 1, p1);
-        at2 = place(t0 + 2, p2);
-        bits2 = counted(t0 + 2, p2);
-        if (bits2 != ~0ull) open_end = min(open_end, t0 + 2);
-        if (bits1 != ~0ull) open_end = min(open_end, t0 + 1);
-        if (bits0 != ~0ull) open_end = min(open_end, t0);
-        if (threadIdx.x == 0) oddL = 0;
-        Stage s2;
-        g_load(sk, a.k_cache, at0);
-        g_load(sv, a.v_cache, at0);
-        g_load(s2, a.k_cache, at1);
-        k_store(sk, 0, 0);
-        k_store(sk, 0, 1);
-        if (!open_tile(t0, bits0)) clean(sv, bits0);
-        v_store(sv, 0, 0);
-        v_store(sv, 0, 1);
-        k_store(s2, 1, 0);
-        k_store(s2, 1, 1);
+        Pages g[KD];
+#pragma unroll
+        for (int i = 0; i < KD; ++i) g[i] = page_ids(t0 + i);
+#pragma unroll
+        for (int i = 0; i < KD; ++i) {
+            const int64_t base = base_of(t0 + i, g[i]);
+            copy_k(base, i);
+            if (i < VD) copy_v(base, i);
+            else v_base[i - VD] = base;
+            bits[i] = counted(t0 + i, g[i]);
+        }
+#pragma unroll
+        for (int i = KD - 1; i >= 0; --i)
+            if (bits[i] != ~0ull) open_end = min(open_end, t0 + i);
     }
+    Pages ahead = page_ids(t0 + KD);
+    // (the query rows' loads are waited for with the first tiles)
+    wait_landed<(KD - 2) * NI + (VD - 1) * NI>();
+    if (!open_tile(t0, bits[0])) clean(0, bits[0]);
     __syncthreads();
-
-    int kc = 0, kn = 1, kw = 2;        // ring slots of K(t), K(t + 1), K(t + 2)
-    // K(t + 2), V(t + 1) and the page numbers of tile t + 4: a whole step to arrive
+    int kslot = 0, vslot = 0;          // of tile t
+    auto after = [](int slot, int step, int n) __attribute__((always_inline)) { return slot + step < n ? slot + step : slot + step - n; };
+    // K(t + KD) and V(t + VD) into the slots that K(t - 1) and V(t - 1) left, page numbers of the tile behind
     auto request = [&](int t) __attribute__((always_inline)) {
-        const int pg4 = page_ids(t + 4);
-        g_load(sk, a.k_cache, at2);
-        g_load(sv, a.v_cache, at1);
-        at1 = at2;
-        at2 = place(t + 3, pg3);
-        const uint64_t bits3 = counted(t + 3, pg3);
-        pg3 = pg4;
-        if (bits3 != ~0ull) open_end = min(open_end, t + 3);
-        return bits3;
+        const int64_t base = base_of(t + KD, ahead);
+        copy_k(base, after(kslot, KD, KD + 1));
+        copy_v(v_base[0], after(vslot, VD, VD + 1));
+#pragma unroll
+        for (int i = 0; i + 1 < KD - VD; ++i) v_base[i] = v_base[i + 1];
+        v_base[KD - VD - 1] = base;
+        const uint64_t last = counted(t + KD, ahead);
+        if (last != ~0ull) open_end = min(open_end, t + KD);
+        ahead = page_ids(t + KD + 1);
+        return last;
     };
-    auto turn = [&](uint64_t bits3) __attribute__((always_inline)) {
-        bits0 = bits1;
-        bits1 = bits2;
-        bits2 = bits3;
-        const int k_old = kc;
-        kc = kn;
-        kn = kw;
-        kw = k_old;
+    // the end of a tile: K(t + 2) and V(t + 1) have landed (what was asked for since the tile before may be on its way), values cleaned if need be
+    auto turn = [&](int t, uint64_t last, bool masks) __attribute__((always_inline)) {
+        wait_landed<(KD - 2) * NI + (VD - 1) * NI>();
+        vslot = after(vslot, 1, VD + 1);
+        kslot = after(kslot, 1, KD + 1);
+        if (masks && !open_tile(t + 1, bits[1])) clean(vslot, bits[1]);
+#pragma unroll
+        for (int i = 0; i + 1 < KD; ++i) bits[i] = bits[i + 1];
+        bits[KD - 1] = last;
         __syncthreads();
     };
     if (!active) {       // a wave without rows stages its part of every tile
         for (int t = t0; t + 1 < t1; ++t) {
-            const uint64_t bits3 = request(t);
-            k_store(sk, kw, 0);
-            k_store(sk, kw, 1);
-            if (!open_tile(t + 1, bits1)) clean(sv, bits1);
-            v_store(sv, (t - t0 + 1) & 1, 0);
-            v_store(sv, (t - t0 + 1) & 1, 1);
-            turn(bits3);
+            const uint64_t last = request(t);
+            turn(t, last, true);
         }
         if (odd) oddL = 1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in LDS after this workgroup is gone
         __syncthreads();
         return;
     }
-
 
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -858,47 +875,39 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s0[i] = 0.f;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(&kL[0][0], k), qf[k], s0, 0, 0, 0);
+    for (int k = 0; k < KS; ++k) s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(kring, k), qf[k], s0, 0, 0, 0);
     {
-        const uint32_t vis = (uint32_t)visible(t0, bits0) >> (4 * hi);
+        const uint32_t vis = (uint32_t)visible(t0, bits[0]) >> (4 * hi);
 #pragma unroll
         for (int mi = 0; mi < 4; ++mi) max_piece(s0, mi, vis, yes);
     }
 #pragma unroll
-    for (int k = 0; k < PF; ++k) kpre[k] = k_frag(&kL[0][0] + 32 * KROW, k);
+    for (int k = 0; k < PF; ++k) kpre[k] = k_frag(kring + 32 * RB, k);
     if (wid >= 4) __builtin_amdgcn_s_setprio(1);      // (the later waves of a SIMD lose every arbitration by age otherwise)
     auto tile_step = [&](int t, auto masks) __attribute__((always_inline)) {
         constexpr bool kMask = decltype(masks)::value;
-        const int buf = (t - t0) & 1;
-        const unsigned char *kcur = &kL[kc][0], *knext = &kL[kn][0], *vcur = &vL[buf][0];
-        const uint64_t bits3 = request(t);
+        const unsigned char *kcur = kring + kslot * TB, *knext = kring + after(kslot, 1, KD + 1) * TB, *vcur = vring + vslot * TB;
+        const uint64_t last = request(t);
         uint32_t vis1 = 0, vis2 = 0;
         if constexpr (kMask) {
-            vis1 = (uint32_t)(visible(t, bits0) >> 32) >> (4 * hi);
-            vis2 = (uint32_t)visible(t + 1, bits1) >> (4 * hi);
+            vis1 = (uint32_t)(visible(t, bits[0]) >> 32) >> (4 * hi);
+            vis2 = (uint32_t)visible(t + 1, bits[1]) >> (4 * hi);
         }
-        block_step(s0, s1, kcur + 32 * KROW, vcur, knext, vis1, yes, yes, masks, no_hook);
-        const int kdst = kw, vdst = buf ^ 1;
-        if constexpr (kMask) {
-            if (!open_tile(t + 1, bits1)) clean(sv, bits1);
-        }
-        block_step(s1, s0, knext, vcur + 32 * VROW, knext + 32 * KROW, vis2, yes, yes, masks, [&](int at) __attribute__((always_inline)) {
-            const int k = at - (KS + NP - 2 * NV);      // the stores beside the last matrix instructions
-            if (k >= 0 && k < NV) k_store(sk, kdst, k);
-            if (k >= NV && k < 2 * NV) v_store(sv, vdst, k - NV);
-        });
-        turn(bits3);
+        block_step(s0, s1, kcur + 32 * RB, vcur, knext, vis1, yes, yes, masks);
+        block_step(s1, s0, knext, vcur + 32 * RB, knext + 32 * RB, vis2, yes, yes, masks);
+        turn(t, last, kMask);
     };
     int t = t0;
     for (; t + 1 < open_end; ++t) tile_step(t, no);
     for (; t + 1 < t1; ++t) tile_step(t, yes);
     {   // the last tile: nothing follows its second block
-        const uint32_t vis1 = (uint32_t)(visible(t, bits0) >> 32) >> (4 * hi);
-        const unsigned char* vcur = &vL[(t - t0) & 1][0];
-        block_step(s0, s1, &kL[kc][0] + 32 * KROW, vcur, nullptr, vis1, yes, no, yes, no_hook);
-        block_step(s1, s0, &kL[kc][0], vcur + 32 * VROW, nullptr, 0, no, no, no, no_hook);
+        const uint32_t vis1 = (uint32_t)(visible(t, bits[0]) >> 32) >> (4 * hi);
+        const unsigned char *kcur = kring + kslot * TB, *vcur = vring + vslot * TB;
+        block_step(s0, s1, kcur + 32 * RB, vcur, nullptr, vis1, yes, no, yes);
+        block_step(s1, s0, kcur, vcur + 32 * RB, nullptr, 0, no, no, no);
     }
     if (odd) oddL = 1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (!stored) return;
     // oacc[db][i] = O^T[32 db + (i & 3) + 8 (i >> 2) + 4 hi][row]
