@@ -530,8 +530,9 @@ __global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs 
 }
 
 // ------------------------------------------------------------------ bf16, more rows: 32 a wave, keys shared by the workgroup
-// 256 stacked rows against every 64-key tile in LDS, one barrier a tile.  Keys and values go there by global_load_lds, three and two whole
-// tiles' time ahead (rings of five and four tiles: no staging registers, and a trip to memory under load is one to two of those times).
+// 128 stacked rows against every 64-key tile in LDS, one barrier a tile, two workgroups a compute unit (two waves a SIMD that do not wait for each
+// other's barriers, and shorter trees leave less idle than in one of 256 rows).  Keys and values go to LDS by global_load_lds, KD - 1 and VD tiles'
+// time ahead (no staging registers).
 //   * v_mfma_f32_32x32x16_bf16: S^T = K . Q^T leaves a lane (row l & 31, half h = l >> 5) 16 scores of a 32-key block, keys (i & 3) + 8 (i >> 2) +
 //     4 h; registers 8 s .. 8 s + 7, rounded to bf16, are operand B of step s of O^T += V^T . P^T as they stand, and the transposing reads of
 //     V deliver those keys.
@@ -555,20 +556,22 @@ __device__ __forceinline__ void wait_landed() {
 }
 
 template <int D>
-__global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
+__global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     constexpr int KT = 64, KS = D / 16, DB = D / 32, NP = 2 * DB;
     constexpr int PF = 3, PFV = NP - 1 < 7 ? NP - 1 : 7;        // reads of keys and values in front of their matrix instruction
-    constexpr int KD = 4, VD = 3, RB = D * 2, TB = KT * RB, VPR = D / 8, NI = TB / 8192;      // NI: requests of a wave for a tile
+    constexpr int KD = D == 128 ? 2 : 4, VD = KD - 1, RB = D * 2, TB = KT * RB, VPR = D / 8, NI = TB / 4096;      // NI: requests of a wave for a tile
     __shared__ __attribute__((aligned(16))) unsigned char ring[(KD + 1 + VD + 1) * TB];
-    __shared__ int oddL;
     unsigned char *const kring = ring, *const vring = ring + (KD + 1) * TB;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lq = lane & 31, hi = lane >> 5;
 
-    const int units = a.rows * a.hkv * a.row_blocks, split = blockIdx.x / units, unit = blockIdx.x % units;
-    const int kvh = unit % a.hkv, b = unit / a.hkv % a.rows, rb = unit / (a.hkv * a.rows);
+    // parts of the same rows' keys eight workgroups apart, on one XCD: what one asks for the others find in its L2
+    const int units = a.rows * a.hkv, each = (units + 7) / 8 * 8 * a.row_blocks, split = blockIdx.x / each, within = blockIdx.x % each;
+    const int unit = within / (8 * a.row_blocks) * 8 + within % 8, rb = within / 8 % a.row_blocks;
+    if (unit >= units) return;
+    const int kvh = unit % a.hkv, b = unit / a.hkv;
     const TreeSpan s = tree_span(a, b);
-    // a row's stacked rows in as few parts as 256 allow, of even size
-    const int stacked = s.n * a.g, parts = (stacked + 255) / 256;
+    // a row's stacked rows in as few parts as 128 allow, of even size
+    const int stacked = s.n * a.g, parts = (stacked + 127) / 128;
     if (rb >= parts || split >= filled_splits_tree(a, s.total)) return;
     const int part_rows = ((stacked + parts - 1) / parts + 31) & ~31, row0 = rb * part_rows;
     if (row0 >= stacked) return;
@@ -584,7 +587,7 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
 #pragma unroll
         for (int k = 0; k < KS; ++k) qf[k] = __builtin_bit_cast(bf16x8_t, ld16(qp + k * 16));
     }
-    // ---- pages: the four runs of 16 keys of a tile lie in a page each; a wave stages eight rows, of one run
+    // ---- pages: the four runs of 16 keys of a tile lie in a page each; a wave stages one of them
     typedef const int32_t __attribute__((address_space(4))) Entry;      // (nothing here writes the table: scalar loads)
     Entry* bt = (Entry*)(uintptr_t)(a.block_table + (int64_t)b * a.bt_stride);
     struct Pages {
@@ -605,8 +608,8 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
     };
     const unsigned row_bytes = (unsigned)a.hkv * RB;
     auto base_of = [&](int t, const Pages& g) __attribute__((always_inline)) {      // byte offset in either cache of the wave's first row
-        const int run = wid >> 1, pg = run == 0 ? g.p[0] : run == 1 ? g.p[1] : run == 2 ? g.p[2] : g.p[3];
-        const int64_t row = ((int64_t)((unsigned)pg < (unsigned)a.num_pages ? pg : 0) << a.page_shift) + ((min(t, t1 - 1) * KT + 8 * wid) & (a.page - 1));
+        const int pg = wid == 0 ? g.p[0] : wid == 1 ? g.p[1] : wid == 2 ? g.p[2] : g.p[3];
+        const int64_t row = ((int64_t)((unsigned)pg < (unsigned)a.num_pages ? pg : 0) << a.page_shift) + ((min(t, t1 - 1) * KT + 16 * wid) & (a.page - 1));
         return row * row_bytes + kvh * RB;
     };
     // The LDS image of a tile is its rows back to back; 16-byte piece c of row r stands at c ^ k_turn(r) (keys: operand reads of 16 rows) or
@@ -617,9 +620,9 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
     unsigned k_from[NI], v_from[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-        const int r = 8 * wid + i * (64 / VPR) + lane / VPR, c = lane % VPR;
-        k_from[i] = (r & 7) * row_bytes + (c ^ k_turn(r)) * 16;
-        v_from[i] = (r & 7) * row_bytes + (c ^ v_turn(r)) * 16;
+        const int r = i * (64 / VPR) + lane / VPR, c = lane % VPR;      // (a run's first row turns nothing: r for 16 wid + r)
+        k_from[i] = r * row_bytes + (c ^ k_turn(r)) * 16;
+        v_from[i] = r * row_bytes + (c ^ v_turn(r)) * 16;
     }
     // (through inline assembly: seen by the compiler, these loads make it wait for all of them in front of every LDS read)
     auto copy = [&](const void* cache, int64_t base, unsigned from, const unsigned char* to) __attribute__((always_inline)) {
@@ -629,11 +632,11 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
     };
     auto copy_k = [&](int64_t base, int slot) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) copy(a.k_cache, base, k_from[i], kring + slot * TB + wid * 8 * RB + i * 1024);
+        for (int i = 0; i < NI; ++i) copy(a.k_cache, base, k_from[i], kring + slot * TB + wid * 16 * RB + i * 1024);
     };
     auto copy_v = [&](int64_t base, int slot) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) copy(a.v_cache, base, v_from[i], vring + slot * TB + wid * 8 * RB + i * 1024);
+        for (int i = 0; i < NI; ++i) copy(a.v_cache, base, v_from[i], vring + slot * TB + wid * 16 * RB + i * 1024);
     };
     // values of keys that do not count become zero, and what is not finite of the others is left for the end: in the pieces that this wave asked
     // for, once they are there
@@ -641,9 +644,9 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
     auto clean = [&](int slot, uint64_t bits) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            uint4* at = reinterpret_cast<uint4*>(vring + slot * TB + wid * 8 * RB + i * 1024 + lane * 16);
+            uint4* at = reinterpret_cast<uint4*>(vring + slot * TB + wid * 16 * RB + i * 1024 + lane * 16);
             uint4 v = *at;
-            if (!(bits >> (8 * wid + i * (64 / VPR) + lane / VPR) & 1)) v = make_uint4(0, 0, 0, 0);
+            if (!(bits >> (16 * wid + i * (64 / VPR) + lane / VPR) & 1)) v = make_uint4(0, 0, 0, 0);
             const bool o0 = drop_odd(v.x), o1 = drop_odd(v.y), o2 = drop_odd(v.z), o3 = drop_odd(v.w);
             odd |= o0 | o1 | o2 | o3;
             *at = v;
@@ -808,7 +811,6 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
     uint64_t bits[KD];
     int64_t v_base[KD - VD];           // of tiles t + VD .., whose keys have been asked for
     int open_end = min(t1, s.ctx / KT);
-    if (threadIdx.x == 0) oddL = 0;
     {
         Pages g[KD];
 #pragma unroll
@@ -856,14 +858,23 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
         bits[KD - 1] = last;
         __syncthreads();
     };
+    // behind the last tile: whether any wave left a value out (the word is the ring's first, which nothing reads any more)
+    auto report_odd = [&]() __attribute__((always_inline)) {
+        __syncthreads();
+        volatile int* flag = reinterpret_cast<volatile int*>(ring);
+        if (threadIdx.x == 0) *flag = 0;
+        __syncthreads();
+        if (odd) *flag = 1;
+        __syncthreads();
+        return *flag != 0;
+    };
     if (!active) {       // a wave without rows stages its part of every tile
         for (int t = t0; t + 1 < t1; ++t) {
             const uint64_t last = request(t);
             turn(t, last, true);
         }
-        if (odd) oddL = 1;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in LDS after this workgroup is gone
-        __syncthreads();
+        report_odd();
         return;
     }
 
@@ -883,7 +894,6 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < PF; ++k) kpre[k] = k_frag(kring + 32 * RB, k);
-    if (wid >= 4) __builtin_amdgcn_s_setprio(1);      // (the later waves of a SIMD lose every arbitration by age otherwise)
     auto tile_step = [&](int t, auto masks) __attribute__((always_inline)) {
         constexpr bool kMask = decltype(masks)::value;
         const unsigned char *kcur = kring + kslot * TB, *knext = kring + after(kslot, 1, KD + 1) * TB, *vcur = vring + vslot * TB;
@@ -906,12 +916,11 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
         block_step(s0, s1, kcur + 32 * RB, vcur, nullptr, vis1, yes, no, yes);
         block_step(s1, s0, kcur, vcur + 32 * RB, nullptr, 0, no, no, no);
     }
-    if (odd) oddL = 1;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    const bool any_odd = report_odd();
     if (!stored) return;
     // oacc[db][i] = O^T[32 db + (i & 3) + 8 (i >> 2) + 4 hi][row]
-    if (oddL)
+    if (any_odd)
         odd_values<false, D>(a, s, b, kvh, node, t0 * KT, 1 << 30, 1 << 30, min(t1 * KT, s.total), KT, [&](const uint16_t* v) {
 #pragma unroll
             for (int db = 0; db < DB; ++db)
@@ -944,27 +953,70 @@ __global__ __launch_bounds__(512, 1) void tree_attn_wide_kernel(TreeArgs a) {
     }
 }
 
-// Splits added in order; rows that one split holds are written already.
+// Splits added in order; rows that one split holds are written already.  A (node, head) is 2^shift groups of D / 4 lanes, each of which adds every
+// 2^shift-th split with all its requests out at once (64 splits in one group: 32 dependent trips, 17 us where this takes 3).
 template <bool F32, int D>
-__global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
+__global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a, int shift) {
     typedef TreeT<F32> X;
-    constexpr int LPR = D / 4;                 // lanes of a (node, head)
-    const int b = blockIdx.y;
+    constexpr int LPR = D / 4, GROUPS = 256 / LPR, MOST = 4;
+    __shared__ float topL[GROUPS], denL[GROUPS];
+    __shared__ f32x4_t oL[256];
+    const int b = blockIdx.y, group = threadIdx.x / LPR, part = group & ((1 << shift) - 1), c = threadIdx.x % LPR * 4;
     const TreeSpan s = tree_span(a, b);
     const int filled = filled_splits_tree(a, s.total);
-    const int64_t item = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-    const int node = (int)(item / a.hq), head = (int)(item % a.hq), c = threadIdx.x % LPR * 4;
-    if (filled <= 1 || node >= s.n) return;
-    const int64_t t = s.start + node, step = (int64_t)a.tokens * a.hq, at = t * a.hq + head;
-    float top = kTreeNegBig;
-    for (int i = 0; i < filled; ++i) top = fmaxf(top, a.state[2 * (at + i * step)]);
-    float den = 0.f;
+    if (filled <= 1 || (int64_t)blockIdx.x * (GROUPS >> shift) >= (int64_t)s.n * a.hq) return;
+    const int64_t item = (int64_t)blockIdx.x * (GROUPS >> shift) + (group >> shift), step = (int64_t)a.tokens * a.hq;
+    const int node = (int)min(item / a.hq, (int64_t)s.n - 1), head = (int)(item % a.hq);
+    const int64_t t = s.start + node, at = t * a.hq + head;
+    float top = kTreeNegBig, den = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < filled; ++i) {
-        const float f = __builtin_amdgcn_exp2f(a.state[2 * (at + i * step)] - top);
-        den = fmaf(a.state[2 * (at + i * step) + 1], f, den);
-        o += *reinterpret_cast<const f32x4_t*>(a.part + (at + i * step) * D + c) * f;
+    for (int first = part; first < filled; first += MOST << shift) {
+        float m[MOST], l[MOST];
+        f32x4_t x[MOST];
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+            m[i] = -__builtin_inff();
+            if (first + (i << shift) >= filled) continue;
+            const int64_t from = at + (first + (i << shift)) * step;
+            m[i] = a.state[2 * from];
+            l[i] = a.state[2 * from + 1];
+            x[i] = *reinterpret_cast<const f32x4_t*>(a.part + from * D + c);
+        }
+        float up = top;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) up = fmaxf(up, m[i]);
+        const float f0 = __builtin_amdgcn_exp2f(top - up);
+        den *= f0;
+        o *= f0;
+        top = up;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+            if (first + (i << shift) >= filled) break;
+            const float f = __builtin_amdgcn_exp2f(m[i] - top);
+            den = fmaf(l[i], f, den);
+            o += x[i] * f;
+        }
     }
+    if (shift > 0) {
+        if (c == 0) {
+            topL[group] = top;
+            denL[group] = den;
+        }
+        oL[threadIdx.x] = o;
+        __syncthreads();
+        if (part != 0) return;
+        float up = top;
+        for (int i = 1; i < 1 << shift; ++i) up = fmaxf(up, topL[group + i]);
+        const float f0 = __builtin_amdgcn_exp2f(top - up);
+        den *= f0;
+        o *= f0;
+        for (int i = 1; i < 1 << shift; ++i) {
+            const float f = __builtin_amdgcn_exp2f(topL[group + i] - up);
+            den = fmaf(denL[group + i], f, den);
+            o += oL[threadIdx.x + i * LPR] * f;
+        }
+    }
+    if (item >= (int64_t)s.n * a.hq) return;
     const float inv = den != 0.f ? 1.0f / den : 0.f;
     X::st4((typename X::T*)a.out + t * a.ldo + (int64_t)head * D + c, o * inv);
 }
@@ -978,7 +1030,7 @@ static TreeForm tree_form(int max_nodes, int g, int d, int f32) {
     TreeForm f;
     f.wide = !f32 && stacked > 64;
     f.row_tiles = f32 ? 2 : stacked <= 16 ? 1 : stacked <= 32 ? 2 : 4;
-    const int rows = f.wide ? 256 : 16 * f.row_tiles;
+    const int rows = f.wide ? 128 : 16 * f.row_tiles;
     f.row_blocks = (int)((stacked + rows - 1) / rows);
     f.round_keys = f.wide ? 64 * kTreeRunTiles : f32 ? 64 : 128;
     return f;
@@ -1054,15 +1106,15 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     a.round_keys = f.round_keys;
     a.wide = f.wide;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const int64_t grid = (int64_t)rows * hkv * a.row_blocks * num_splits;
+    const int64_t grid = ((int64_t)rows * hkv + (f.wide ? 7 : 0)) / (f.wide ? 8 : 1) * (f.wide ? 8 : 1) * a.row_blocks * num_splits;
     if (grid > 0x7fffffff || rows > 65535) return MV_ERR_UNSUPPORTED;
     hipStream_t s = (hipStream_t)stream;
     const dim3 g1((unsigned)grid);
 #define MV_TREE(K_, T_) hipLaunchKernelGGL((K_), g1, dim3(T_), 0, s, a)
     if (f32 && d == 64) MV_TREE((tree_attn_f32_kernel<64>), 256);
     else if (f32) MV_TREE((tree_attn_f32_kernel<128>), 256);
-    else if (f.wide && d == 64) MV_TREE((tree_attn_wide_kernel<64>), 512);
-    else if (f.wide) MV_TREE((tree_attn_wide_kernel<128>), 512);
+    else if (f.wide && d == 64) MV_TREE((tree_attn_wide_kernel<64>), 256);
+    else if (f.wide) MV_TREE((tree_attn_wide_kernel<128>), 256);
     else if (d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<64, 1, 1>), 256);
     else if (d == 64 && f.row_tiles == 2) MV_TREE((tree_attn_narrow_kernel<64, 2, 1>), 256);
     else if (d == 64) MV_TREE((tree_attn_narrow_kernel<64, 4, 1>), 256);
@@ -1071,11 +1123,14 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     else MV_TREE((tree_attn_narrow_kernel<128, 2, 2>), 512);
 #undef MV_TREE
     if (num_splits > 1) {
-        const dim3 g2((unsigned)(((int64_t)max_nodes * hq + 1024 / d - 1) / (1024 / d)), (unsigned)rows);
-        if (f32 && d == 64) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 64>), g2, dim3(256), 0, s, a);
-        else if (f32) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 128>), g2, dim3(256), 0, s, a);
-        else if (d == 64) hipLaunchKernelGGL((tree_attn_merge_kernel<false, 64>), g2, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((tree_attn_merge_kernel<false, 128>), g2, dim3(256), 0, s, a);
+        const int groups = 1024 / d;
+        int shift = 0;
+        while ((4 << shift) < num_splits && (1 << shift) < groups) ++shift;
+        const dim3 g2((unsigned)(((int64_t)max_nodes * hq + (groups >> shift) - 1) / (groups >> shift)), (unsigned)rows);
+        if (f32 && d == 64) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 64>), g2, dim3(256), 0, s, a, shift);
+        else if (f32) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 128>), g2, dim3(256), 0, s, a, shift);
+        else if (d == 64) hipLaunchKernelGGL((tree_attn_merge_kernel<false, 64>), g2, dim3(256), 0, s, a, shift);
+        else hipLaunchKernelGGL((tree_attn_merge_kernel<false, 128>), g2, dim3(256), 0, s, a, shift);
     }
     return check_launch();
 }
