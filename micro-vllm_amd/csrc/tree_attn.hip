@@ -536,9 +536,12 @@ __global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs 
 //   * v_mfma_f32_32x32x16_bf16: S^T = K . Q^T leaves a lane (row l & 31, half h = l >> 5) 16 scores of a 32-key block, keys (i & 3) + 8 (i >> 2) +
 //     4 h; registers 8 s .. 8 s + 7, rounded to bf16, are operand B of step s of O^T += V^T . P^T as they stand, and the transposing reads of
 //     V deliver those keys.
-//   * pipeline over 32-key blocks: while the matrix unit forms S of block u + 1 the vector unit turns S of u into weights, while it adds V^T P of
-//     u the vector unit takes the maxima of S of u + 1; LDS reads run a few matrix instructions ahead.  Pieces are dealt out slot by slot between
-//     scheduling fences.
+//   * pipeline over 32-key blocks: while the matrix unit forms S of block u + 1 the vector unit turns S of u into weights, the matrix unit then adds
+//     V^T P of u; LDS reads run a few matrix instructions ahead.  Pieces are dealt out slot by slot between scheduling fences.
+//   * no running maximum: weights are 2^(s - m) with m the maximum of the row's first block.  Their size does not touch their precision (bf16 and
+//     the fp32 sums are relative), only their range, so a row whose denominator or sums leave the range that is safe - scores 44 nats above those of
+//     its first block - makes the workgroup do its keys again with a running maximum.  (The maximum of every block, its exchange between lanes and
+//     the test for a rescale were a fifth of the vector unit's work: 32 rows of 4096 and 64 nodes 188 -> 165 us.)
 //   * a tile in which every key counts for every row (all but the one or two with nodes in them) takes no mask.
 // Waves without rows (short trees) only stage.
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
@@ -591,25 +594,30 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     typedef const int32_t __attribute__((address_space(4))) Entry;      // (nothing here writes the table: scalar loads)
     Entry* bt = (Entry*)(uintptr_t)(a.block_table + (int64_t)b * a.bt_stride);
     struct Pages {
-        int p[4];
+        int own;               // of the wave's run
+        uint64_t there;        // keys of the tile that lie in a page
     };
+    const bool small = a.page_shift < 6;      // pages of less than a tile
     auto page_ids = [&](int t) __attribute__((always_inline)) {
+        const int kb = min(t, t1 - 1) * KT;
         Pages r;
+        r.own = bt[min((kb + 16 * wid) >> a.page_shift, a.bt_cols - 1)];
+        r.there = (unsigned)r.own < (unsigned)a.num_pages ? ~0ull : 0;
+        if (small) {
+            r.there = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r.p[i] = bt[min((min(t, t1 - 1) * KT + 16 * i) >> a.page_shift, a.bt_cols - 1)];
+            for (int i = 0; i < 4; ++i)
+                if ((unsigned)bt[min((kb + 16 * i) >> a.page_shift, a.bt_cols - 1)] < (unsigned)a.num_pages) r.there |= 0xffffull << (16 * i);
+        }
         return r;
     };
     auto counted = [&](int t, const Pages& g) __attribute__((always_inline)) {      // keys of a tile that count
-        uint64_t bits = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bits |= (unsigned)g.p[i] < (unsigned)a.num_pages ? 0xffffull << (16 * i) : 0;
         const int left = s.total - min(t, t1 - 1) * KT;
-        return left < KT ? bits & ((1ull << left) - 1) : bits;
+        return left < KT ? g.there & ((1ull << left) - 1) : g.there;
     };
     const unsigned row_bytes = (unsigned)a.hkv * RB;
     auto base_of = [&](int t, const Pages& g) __attribute__((always_inline)) {      // byte offset in either cache of the wave's first row
-        const int pg = wid == 0 ? g.p[0] : wid == 1 ? g.p[1] : wid == 2 ? g.p[2] : g.p[3];
-        const int64_t row = ((int64_t)((unsigned)pg < (unsigned)a.num_pages ? pg : 0) << a.page_shift) + ((min(t, t1 - 1) * KT + 16 * wid) & (a.page - 1));
+        const int64_t row = ((int64_t)((unsigned)g.own < (unsigned)a.num_pages ? g.own : 0) << a.page_shift) + ((min(t, t1 - 1) * KT + 16 * wid) & (a.page - 1));
         return row * row_bytes + kvh * RB;
     };
     // The LDS image of a tile is its rows back to back; 16-byte piece c of row r stands at c ^ k_turn(r) (keys: operand reads of 16 rows) or
@@ -685,8 +693,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     };
 
     f32x16_t oacc[DB];
-    float mrun = kTreeNegBig, lrun0 = 0.f, lrun1 = 0.f, alpha = 1.f;
-    bool rescale = false;
+    float mrun = kTreeNegBig, lrun0 = 0.f, lrun1 = 0.f;
+    bool saw = false;                  // any key
     uint32_t pw[8];
     float fa[8][2], eb[8][2];
     auto softmax_slot = [&](const f32x16_t& sc, int at) __attribute__((always_inline)) {      // three stages of a pair of scores, a slot apart
@@ -714,64 +722,45 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     auto p_frag = [&](int st) __attribute__((always_inline)) {
         return __builtin_bit_cast(bf16x8_t, make_uint4(pw[4 * st], pw[4 * st + 1], pw[4 * st + 2], pw[4 * st + 3]));
     };
-    float m2[2];
-    // a quarter of a block's maximum; masked: `vis` (shifted by 4 hi) has the row's keys
-    auto max_piece = [&](f32x16_t& sn, int mi, uint32_t vis, auto masked) __attribute__((always_inline)) {
-        constexpr int from[5] = {0, 6, 10, 14, 16};
-        if constexpr (decltype(masked)::value) {
+    // scores of keys that the row does not see (`vis`, shifted by 4 hi, has those it does): a quarter of a block's
+    auto mask_piece = [&](f32x16_t& sn, int mi, uint32_t vis) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = from[mi]; i < from[mi + 1]; ++i)
-                if (!(vis >> ((i & 3) + 8 * (i >> 2)) & 1)) sn[i] = -__builtin_inff();
-        }
-        if (mi == 0) {
-            m2[0] = max3_tree(sn[0], sn[1], sn[2]);
-            m2[1] = max3_tree(sn[3], sn[4], sn[5]);
-        } else if (mi == 1) {
-            m2[0] = max3_tree(m2[0], sn[6], sn[7]);
-            m2[1] = max3_tree(m2[1], sn[8], sn[9]);
-        } else if (mi == 2) {
-            m2[0] = max3_tree(m2[0], sn[10], sn[11]);
-            m2[1] = max3_tree(m2[1], sn[12], sn[13]);
-        } else {
-            m2[0] = max3_tree(m2[0], sn[14], sn[15]);
-        }
+        for (int i = 4 * mi; i < 4 * mi + 4; ++i)
+            if (!(vis >> ((i & 3) + 8 * (i >> 2)) & 1)) sn[i] = -__builtin_inff();
     };
-    auto max_finish = [&]() __attribute__((always_inline)) {
-        const unsigned u = __float_as_uint(fmaxf(m2[0], m2[1]) * a.scale_log2);
+    auto block_max = [&](const f32x16_t& sc) __attribute__((always_inline)) {      // of a row, times the scale
+        float x = max3_tree(sc[0], sc[1], sc[2]), y = max3_tree(sc[3], sc[4], sc[5]);
+        x = max3_tree(x, sc[6], sc[7]);
+        y = max3_tree(y, sc[8], sc[9]);
+        x = max3_tree(x, sc[10], sc[11]);
+        y = max3_tree(y, sc[12], sc[13]);
+        x = max3_tree(x, sc[14], sc[15]);
+        const unsigned u = __float_as_uint(fmaxf(x, y) * a.scale_log2);
         const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-        const float mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-        rescale = __builtin_amdgcn_ballot_w64(mloc > mrun + kTreeRaise) != 0;
-        if (rescale) {
-            const float mnew = fmaxf(mrun, mloc);
-            alpha = __builtin_amdgcn_exp2f(mrun - mnew);
-            mrun = mnew;
-        }
+        return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
     };
-    auto apply_rescale = [&]() __attribute__((always_inline)) {
-        if (rescale) {
+    bool exact = false;                // with a running maximum
+    auto raise = [&](const f32x16_t& sc) __attribute__((always_inline)) {
+        const float mloc = block_max(sc);
+        if (__builtin_amdgcn_ballot_w64(mloc > mrun) != 0) {
+            const float mnew = fmaxf(mrun, mloc), alpha = __builtin_amdgcn_exp2f(mrun - mnew);
+            mrun = mnew;
             lrun0 *= alpha;
             lrun1 *= alpha;
-            typedef __attribute__((ext_vector_type(2))) float f32x2_t;
-            const f32x2_t a2 = {alpha, alpha};
 #pragma unroll
             for (int db = 0; db < DB; ++db)
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const f32x2_t o2 = f32x2_t{oacc[db][i], oacc[db][i + 1]} * a2;
-                    oacc[db][i] = o2[0];
-                    oacc[db][i + 1] = o2[1];
-                }
+                for (int i = 0; i < 16; ++i) oacc[db][i] *= alpha;
         }
     };
-    // Block u (scores sc, maximum pieces taken): weights, O += V^T P; scores of block u + 1 (keys at kblock) into sn.  kpre: its first reads, made
+    // Block u (scores sc, masked): weights, O += V^T P; scores of block u + 1 (keys at kblock) into sn.  kpre: its first reads, made
     // during the step before, refilled from kblock_after.
     bf16x8_t kpre[PF];
     auto block_step = [&](const f32x16_t& sc, f32x16_t& sn, const unsigned char* kblock, const unsigned char* vblock,
                           const unsigned char* kblock_after, uint32_t vis_next, auto has_next, auto has_after,
                           auto mask_next) __attribute__((always_inline)) {
         constexpr bool kNext = decltype(has_next)::value, kAfter = decltype(has_after)::value;
-        max_finish();
-        apply_rescale();
+        if (exact) raise(sc);
         bf16x8_t kf[KS], vf[NP];
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
@@ -794,10 +783,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
             }
             oacc[j % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j], p_frag(j / DB), oacc[j % DB], 0, 0, 0);
             softmax_slot(sc, KS + j);
-            if constexpr (kNext) {
+            if constexpr (kNext && decltype(mask_next)::value) {
                 if (j >= DB) {
 #pragma unroll
-                    for (int mi = (j - DB) * 4 / DB; mi < (j - DB + 1) * 4 / DB; ++mi) max_piece(sn, mi, vis_next, mask_next);
+                    for (int mi = (j - DB) * 4 / DB; mi < (j - DB + 1) * 4 / DB; ++mi) mask_piece(sn, mi, vis_next);
                 }
             }
         }
@@ -806,12 +795,15 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     const std::true_type yes{};
     const std::false_type no{};
 
-    // ---- prologue: keys of KD and values of VD tiles asked for, S of the first block and its maxima
+    // ---- prologue: keys of KD and values of VD tiles asked for
     // bits[i]: keys that count in tile t + i.  open_end: tiles in front of this one take no mask, as far as their pages are known
     uint64_t bits[KD];
     int64_t v_base[KD - VD];           // of tiles t + VD .., whose keys have been asked for
-    int open_end = min(t1, s.ctx / KT);
-    {
+    int open_end, kslot, vslot;        // slots: of tile t
+    Pages ahead;
+    auto begin = [&]() __attribute__((always_inline)) {
+        open_end = min(t1, s.ctx / KT);
+        kslot = vslot = 0;
         Pages g[KD];
 #pragma unroll
         for (int i = 0; i < KD; ++i) g[i] = page_ids(t0 + i);
@@ -826,13 +818,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
 #pragma unroll
         for (int i = KD - 1; i >= 0; --i)
             if (bits[i] != ~0ull) open_end = min(open_end, t0 + i);
-    }
-    Pages ahead = page_ids(t0 + KD);
-    // (the query rows' loads are waited for with the first tiles)
-    wait_landed<(KD - 2) * NI + (VD - 1) * NI>();
-    if (!open_tile(t0, bits[0])) clean(0, bits[0]);
-    __syncthreads();
-    int kslot = 0, vslot = 0;          // of tile t
+        ahead = page_ids(t0 + KD);
+        // (the query rows' loads are waited for with the first tiles)
+        wait_landed<(KD - 2) * NI + (VD - 1) * NI>();
+        if (!open_tile(t0, bits[0])) clean(0, bits[0]);
+        __syncthreads();
+    };
     auto after = [](int slot, int step, int n) __attribute__((always_inline)) { return slot + step < n ? slot + step : slot + step - n; };
     // K(t + KD) and V(t + VD) into the slots that K(t - 1) and V(t - 1) left, page numbers of the tile behind
     auto request = [&](int t) __attribute__((always_inline)) {
@@ -858,69 +849,99 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
         bits[KD - 1] = last;
         __syncthreads();
     };
-    // behind the last tile: whether any wave left a value out (the word is the ring's first, which nothing reads any more)
-    auto report_odd = [&]() __attribute__((always_inline)) {
+    // behind the last tile: whether any wave left a value out (1), and whether any row left the safe range (2).  The word is the ring's first, which
+    // nothing reads or writes any more
+    auto report = [&](bool bad) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in LDS behind this
         __syncthreads();
-        volatile int* flag = reinterpret_cast<volatile int*>(ring);
+        int* flag = reinterpret_cast<int*>(ring);
         if (threadIdx.x == 0) *flag = 0;
         __syncthreads();
-        if (odd) *flag = 1;
+        if (odd || bad) atomicOr(flag, (odd ? 1 : 0) | (bad ? 2 : 0));
         __syncthreads();
-        return *flag != 0;
+        const int all = *flag;
+        __syncthreads();
+        return all;
     };
     if (!active) {       // a wave without rows stages its part of every tile
-        for (int t = t0; t + 1 < t1; ++t) {
-            const uint64_t last = request(t);
-            turn(t, last, true);
+        for (int pass = 0; pass < 2; ++pass) {
+            begin();
+            for (int t = t0; t + 1 < t1; ++t) {
+                const uint64_t last = request(t);
+                turn(t, last, true);
+            }
+            if (!(report(false) & 2)) break;
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in LDS after this workgroup is gone
-        report_odd();
         return;
     }
 
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) oacc[db][i] = 0.f;
     f32x16_t s0, s1;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s0[i] = 0.f;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(kring, k), qf[k], s0, 0, 0, 0);
-    {
-        const uint32_t vis = (uint32_t)visible(t0, bits[0]) >> (4 * hi);
-#pragma unroll
-        for (int mi = 0; mi < 4; ++mi) max_piece(s0, mi, vis, yes);
-    }
-#pragma unroll
-    for (int k = 0; k < PF; ++k) kpre[k] = k_frag(kring + 32 * RB, k);
     auto tile_step = [&](int t, auto masks) __attribute__((always_inline)) {
         constexpr bool kMask = decltype(masks)::value;
         const unsigned char *kcur = kring + kslot * TB, *knext = kring + after(kslot, 1, KD + 1) * TB, *vcur = vring + vslot * TB;
         const uint64_t last = request(t);
         uint32_t vis1 = 0, vis2 = 0;
         if constexpr (kMask) {
-            vis1 = (uint32_t)(visible(t, bits[0]) >> 32) >> (4 * hi);
-            vis2 = (uint32_t)visible(t + 1, bits[1]) >> (4 * hi);
+            const uint64_t here = visible(t, bits[0]), there = visible(t + 1, bits[1]);
+            saw |= (here | there) != 0;
+            vis1 = (uint32_t)(here >> 32) >> (4 * hi);
+            vis2 = (uint32_t)there >> (4 * hi);
         }
         block_step(s0, s1, kcur + 32 * RB, vcur, knext, vis1, yes, yes, masks);
         block_step(s1, s0, knext, vcur + 32 * RB, knext + 32 * RB, vis2, yes, yes, masks);
         turn(t, last, kMask);
     };
-    int t = t0;
-    for (; t + 1 < open_end; ++t) tile_step(t, no);
-    for (; t + 1 < t1; ++t) tile_step(t, yes);
-    {   // the last tile: nothing follows its second block
-        const uint32_t vis1 = (uint32_t)(visible(t, bits[0]) >> 32) >> (4 * hi);
-        const unsigned char *kcur = kring + kslot * TB, *vcur = vring + vslot * TB;
-        block_step(s0, s1, kcur + 32 * RB, vcur, nullptr, vis1, yes, no, yes);
-        block_step(s1, s0, kcur, vcur + 32 * RB, nullptr, 0, no, no, no);
+    int flags;
+    while (true) {
+        begin();
+        mrun = kTreeNegBig;
+        lrun0 = lrun1 = 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) oacc[db][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s0[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(kring, k), qf[k], s0, 0, 0, 0);
+        const uint64_t first = visible(t0, bits[0]);
+        saw = first != 0;
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi) mask_piece(s0, mi, (uint32_t)first >> (4 * hi));
+        if (!exact) {
+            mrun = block_max(s0);
+            if (!(fabsf(mrun) <= 3.4028235e38f)) mrun = 0.f;      // nothing seen yet
+        }
+#pragma unroll
+        for (int k = 0; k < PF; ++k) kpre[k] = k_frag(kring + 32 * RB, k);
+        int t = t0;
+        for (; t + 1 < open_end; ++t) tile_step(t, no);
+        for (; t + 1 < t1; ++t) tile_step(t, yes);
+        {   // the last tile: nothing follows its second block
+            const uint32_t vis1 = (uint32_t)(visible(t, bits[0]) >> 32) >> (4 * hi);
+            const unsigned char *kcur = kring + kslot * TB, *vcur = vring + vslot * TB;
+            block_step(s0, s1, kcur + 32 * RB, vcur, nullptr, vis1, yes, no, yes);
+            block_step(s1, s0, kcur, vcur + 32 * RB, nullptr, 0, no, no, no);
+        }
+        bool bad = false;
+        if (!exact) {
+            const float l = lrun0 + lrun1 + __shfl_xor(lrun0 + lrun1, 32, 64);
+            bad = saw && !(l >= 0x1p-20f && l <= 0x1p64f);
+            float none = 0.f;      // zero unless a sum is not finite
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) none = fmaf(oacc[db][i], 0.f, none);
+            bad |= none != 0.f;
+        }
+        flags = report(bad);
+        if (exact || !(flags & 2)) break;
+        exact = true;
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const bool any_odd = report_odd();
+    if (!saw) mrun = kTreeNegBig;
     if (!stored) return;
     // oacc[db][i] = O^T[32 db + (i & 3) + 8 (i >> 2) + 4 hi][row]
-    if (any_odd)
+    if (flags & 1)
         odd_values<false, D>(a, s, b, kvh, node, t0 * KT, 1 << 30, 1 << 30, min(t1 * KT, s.total), KT, [&](const uint16_t* v) {
 #pragma unroll
             for (int db = 0; db < DB; ++db)
