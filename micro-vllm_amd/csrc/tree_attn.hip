@@ -19,7 +19,6 @@ constexpr int kTreeMaxNodes = 256;
 constexpr int kTreeMaxWords = kTreeMaxNodes / 64;
 constexpr int kTreeBlock = 16;                 // pages hold whole runs of this many keys
 constexpr int kTreeMaxSplits = 64;
-constexpr int kTreeRunTiles = 4;               // no run of tiles is cut shorter
 
 struct TreeArgs {
     const void *q, *k_cache, *v_cache;
@@ -33,7 +32,7 @@ struct TreeArgs {
     float *part, *state;         // splits: sums [split][token][head][d], (maximum, denominator) [split][token][head]
     int bt_cols, rows, tokens, max_nodes, hq, hkv, g, page, page_shift, num_pages, nsplit, row_blocks;
     int round_keys;              // keys that a split's workgroup takes in one round
-    int wide;
+    int row_part, slots, least;  // stacked rows of a workgroup, workgroups that run at once, rounds below which nothing is cut
     float scale_log2;
 };
 
@@ -48,14 +47,31 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int b) {
     s.total = (int)min((int64_t)s.ctx + s.n, (int64_t)a.bt_cols << a.page_shift);
     return s;
 }
-// Up to 64 stacked rows (and fp32): blocks are dealt to the splits in rounds of one for every wave of a workgroup, so which keys a wave asks
-// for first does not depend on a row's length.  More: a split is a run of 64-key tiles.  Tiles of a run, and splits of a row that have any:
-__device__ __forceinline__ int run_tiles(const TreeArgs& a, int total) {
-    return max((((total + 63) >> 6) + a.nsplit - 1) / a.nsplit, kTreeRunTiles);
+// How many of the launch's splits a row of `total` keys takes.  A piece of work is a round (round_keys keys of up to row_part stacked rows of one
+// key/value head); rows are cut so that no split has more than its share of the step's rounds over `slots` workgroups: where rows differ in
+// length the long ones take more splits, and where there are rounds enough for every slot none is cut.  In two halves, the rounds that a lane
+// counts (its loads go out with a kernel's first) and their sum; all lanes of a wave call them together.
+__device__ __forceinline__ int step_rounds(const TreeArgs& a) {
+    int work = 0;
+    if (a.nsplit > 1)
+        for (int i = threadIdx.x & 63; i < a.rows; i += 64) {
+            const int from = min(max(a.row_start[i], 0), a.tokens);
+            const int n = min(min(max(a.row_start[i + 1], from), a.tokens) - from, a.max_nodes);
+            const int keys = (int)min((int64_t)max(a.ctx[i], 0) + n, (int64_t)a.bt_cols << a.page_shift);
+            work += ((n * a.g + a.row_part - 1) / a.row_part) * ((keys + a.round_keys - 1) / a.round_keys);
+        }
+    return work;
 }
-__device__ __forceinline__ int filled_splits_tree(const TreeArgs& a, int total) {
-    const int round = a.wide ? run_tiles(a, total) * 64 : a.round_keys;
-    return max(1, min(a.nsplit, (total + round - 1) / round));
+__device__ __forceinline__ int row_splits(const TreeArgs& a, int total, int work) {
+    if (a.nsplit == 1) return 1;
+    work += __builtin_amdgcn_update_dpp(0, work, 0x111, 0xf, 0xf, true);      // row_shr 1, 2, 4, 8: a row's sum in its lane 15
+    work += __builtin_amdgcn_update_dpp(0, work, 0x112, 0xf, 0xf, true);
+    work += __builtin_amdgcn_update_dpp(0, work, 0x114, 0xf, 0xf, true);
+    work += __builtin_amdgcn_update_dpp(0, work, 0x118, 0xf, 0xf, true);
+    const int64_t sum = (int64_t)__builtin_amdgcn_readlane(work, 15) + __builtin_amdgcn_readlane(work, 31) + __builtin_amdgcn_readlane(work, 47) +
+                        __builtin_amdgcn_readlane(work, 63);
+    const int share = max((int)((sum * a.hkv + a.slots - 1) / a.slots), a.least), rounds = (total + a.round_keys - 1) / a.round_keys;
+    return max(1, min(a.nsplit, (rounds + share - 1) / share));
 }
 // 64 bits of a node's mask from bit `first` (negative: cached tokens in front of the nodes, visible) on
 __device__ __forceinline__ uint64_t mask_from(const uint64_t (&w)[kTreeMaxWords], int first) {
@@ -150,8 +166,9 @@ __device__ __forceinline__ void odd_values(const TreeArgs& a, const TreeSpan& s,
 __device__ __forceinline__ bool is_odd(float x) { return !(fabsf(x) <= 3.4028235e38f); }
 // dimensions c .. c + 3 of a stacked row, of a kernel that deals its blocks
 template <bool F32, int D>
-__device__ __forceinline__ void add_odd(const TreeArgs& a, const TreeSpan& s, int b, int kvh, int split, int block, int sr, int c, f32x4_t& o) {
-    odd_values<F32, D>(a, s, b, kvh, sr / a.g, split * a.round_keys, a.nsplit * a.round_keys, a.round_keys, s.total, block,
+__device__ __forceinline__ void add_odd(const TreeArgs& a, const TreeSpan& s, int b, int kvh, int split, int splits, int block, int sr, int c,
+                                        f32x4_t& o) {
+    odd_values<F32, D>(a, s, b, kvh, sr / a.g, split * a.round_keys, splits * a.round_keys, a.round_keys, s.total, block,
                        [&](const typename TreeT<F32>::T* v) {
                            const f32x4_t x = TreeT<F32>::ld4(v + c);
 #pragma unroll
@@ -174,12 +191,16 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
     __shared__ __attribute__((aligned(16))) float oL[W][RT * 16][D];
     __shared__ float mL[W][RT * 16], lL[W][RT * 16];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
-    const int split = blockIdx.x % a.nsplit, rest = blockIdx.x / a.nsplit;
+    // (splits slowest: neighbouring workgroups go to different XCDs, and where no row is cut only the first split has work)
+    const int units = a.rows * a.hkv * a.row_blocks, split = blockIdx.x / units, rest = blockIdx.x % units;
     const int rb = rest % a.row_blocks, bh = rest / a.row_blocks, kvh = bh % a.hkv, b = bh / a.hkv;
+    const int rounds = step_rounds(a);
     const TreeSpan s = tree_span(a, b);
     const int stacked = s.n * a.g, row0 = rb * RT * 16;
     const int blocks = (s.total + kTreeBlock - 1) / kTreeBlock;
-    if (row0 >= stacked || split >= filled_splits_tree(a, s.total)) return;
+    if (row0 >= stacked || (split > 0 && split * a.round_keys >= s.total)) return;
+    const int splits = row_splits(a, s.total, rounds);
+    if (split >= splits) return;
 
     f32x4_t qf[RT][KG];
     uint64_t words[RT][kTreeMaxWords];
@@ -212,7 +233,7 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
     }
     const int64_t stride = (int64_t)a.hkv * D;
     bool odd = false;
-    for (int blk = split * W + wid; blk < blocks; blk += a.nsplit * W) {
+    for (int blk = split * W + wid; blk < blocks; blk += splits * W) {
         const int kb = blk * kTreeBlock, pg = a.block_table[(int64_t)b * a.bt_stride + (kb >> a.page_shift)];
         if (pg < 0 || pg >= a.num_pages) continue;      // a place without a page: its keys do not count
         const int64_t row = ((int64_t)pg << a.page_shift) + (kb & (a.page - 1));
@@ -295,7 +316,7 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
                     (f32x4_t){acc[i][h][0][e], acc[i][h][1][e], acc[i][h][2][e], acc[i][h][3][e]};
     }
     const bool any_odd = __syncthreads_or(odd);
-    const bool whole = filled_splits_tree(a, s.total) <= 1;
+    const bool whole = splits == 1;
 #pragma unroll 1
     for (int it = threadIdx.x; it < RT * 16 * (D / 4); it += 256) {
         const int rr = it / (D / 4), c = it % (D / 4) * 4, sr = row0 + rr;
@@ -311,34 +332,32 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
             den = fmaf(lL[w][rr], f, den);
             o += *reinterpret_cast<const f32x4_t*>(&oL[w][rr][c]) * f;
         }
-        if (any_odd) add_odd<F32, D>(a, s, b, kvh, split, 16, sr, c, o);
+        if (any_odd) add_odd<F32, D>(a, s, b, kvh, split, splits, 16, sr, c, o);
         leave_rows<F32, D>(a, s, whole, split, kvh, sr, c, top, den, o);
     }
 }
 
-// ------------------------------------------------------------------ bf16, up to 64 stacked rows a workgroup
+// ------------------------------------------------------------------ bf16, up to 64 stacked rows (heads of 128: 32)
 // Every wave has keys of its own (32 at a time) and all the rows: nothing is shared until the end, no barrier in the loop.
 //   S^T = K . Q^T   v_mfma_f32_16x16x32_bf16, operand A = key rows as they lie in memory (lane (r, q): row r, dimensions 32 k + 8 q ..);
 //   O^T = V^T . P^T operand B = P as S^T left it, rounded to bf16 (keys 4 q + j and 16 + 4 q + j), operand A through the wave's own piece of
 //                   LDS with the transposing read, which delivers those keys.
 // The normaliser sums the unrounded weights; rounding a weight to bf16 (2^-8 of it) is what the matrix instruction asks for, and half of what
 // the rounding of the output costs anyway.  The next block's keys and values are requested into the registers that this one leaves.
-// RG groups of four waves take 16 RT stacked rows each and the same keys: more rows in one wave are more than 256 registers (heads of 128), and what
-// the groups ask for twice comes out of the L1 cache.
-template <int D, int RT, int RG>
+template <int D, int RT>
 constexpr size_t kNarrowLds = [] {
-    constexpr size_t stage = RG * 4 * 32 * (D * 2 + 32), merge = RG * 4 * RT * 16 * (D + 4) * sizeof(float);
+    constexpr size_t stage = 4 * 32 * (D * 2 + 32), merge = 4 * RT * 16 * (D + 4) * sizeof(float);
     return stage > merge ? stage : merge;
 }();
 
-template <int D, int RT, int RG>
-__global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs a) {
-    constexpr int W = 4, KS = D / 32, DT = D / 16, VROW = D * 2 + 32, VPR = D / 8, NV = 32 * VPR / 64, OROW = D + 4, ROWS = RG * RT * 16;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kNarrowLds<D, RT, RG>];
+template <int D, int RT>
+__global__ __launch_bounds__(256, 2) void tree_attn_narrow_kernel(TreeArgs a) {
+    constexpr int W = 4, KS = D / 32, DT = D / 16, VROW = D * 2 + 32, VPR = D / 8, NV = 32 * VPR / 64, OROW = D + 4, ROWS = RT * 16;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kNarrowLds<D, RT>];
     __shared__ float mL[W][ROWS], lL[W][ROWS];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
-    const int wid = wave & 3, rg = wave >> 2;
-    const int split = blockIdx.x % a.nsplit, rest = blockIdx.x / a.nsplit;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+    // (splits slowest: neighbouring workgroups go to different XCDs, and where no row is cut only the first split has work)
+    const int units = a.rows * a.hkv * a.row_blocks, split = blockIdx.x / units, rest = blockIdx.x % units;
     const int rb = rest % a.row_blocks, bh = rest / a.row_blocks, kvh = bh % a.hkv, b = bh / a.hkv;
     typedef const int32_t __attribute__((address_space(4))) Entry;      // (nothing here writes the table: scalar loads)
     Entry* bt = (Entry*)(uintptr_t)(a.block_table + (int64_t)b * a.bt_stride);
@@ -349,9 +368,12 @@ __global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs 
     int blk = split * W + wid, pg[2];
     bool odd = false;
     pages_of(blk, pg);
+    const int rounds = step_rounds(a);
     const TreeSpan s = tree_span(a, b);
     const int stacked = s.n * a.g, row0 = rb * ROWS, blocks = (s.total + 31) / 32;
-    if (row0 >= stacked || split >= filled_splits_tree(a, s.total)) return;
+    if (row0 >= stacked || (split > 0 && split * a.round_keys >= s.total)) return;
+    const int splits = row_splits(a, s.total, rounds);
+    if (split >= splits) return;
 
     // (a request = a base that is the same for the wave, in scalar registers, and a lane's offset of 32 bits that never changes)
     const unsigned row_bytes = (unsigned)a.hkv * D * 2, k_at = r * row_bytes + 16 * q, v_from = (lane / VPR) * row_bytes + (lane % VPR) * 16;
@@ -384,7 +406,7 @@ __global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs 
     uint64_t word0[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        const int sr = min(row0 + rg * RT * 16 + i * 16 + r, stacked - 1);
+        const int sr = min(row0 + i * 16 + r, stacked - 1);
         node[i] = sr / a.g;
         const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.start + node[i]) * a.ldq + (int64_t)(kvh * a.g + sr % a.g) * D + 8 * q;
 #pragma unroll
@@ -415,11 +437,11 @@ __global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs 
 #pragma unroll
         for (int t = 0; t < DT; ++t) acc[i][t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
-    unsigned char* vst = lds + wave * (32 * VROW);
+    unsigned char* vst = lds + wid * (32 * VROW);
     const int v_at = (lane / VPR) * VROW + (lane % VPR) * 16, tr_at = (4 * q + (r >> 2)) * VROW + (r & 3) * 8;
 
     while (blk < blocks) {
-        const int kb = blk * 32, next = blk + a.nsplit * W;
+        const int kb = blk * 32, next = blk + splits * W;
         uint32_t valid = (pg[0] >= 0 && pg[0] < a.num_pages ? 0xffffu : 0) | (pg[1] >= 0 && pg[1] < a.num_pages ? 0xffff0000u : 0);
         if (s.total - kb < 32) valid &= (1u << (s.total - kb)) - 1;
         const bool open = valid == ~0u && kb + 32 <= s.ctx;       // every key there and visible to every row (uniform)
@@ -501,16 +523,16 @@ __global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs 
         l[i] += __shfl_xor(l[i], 16, 64);
         l[i] += __shfl_xor(l[i], 32, 64);
         if (q == 0) {
-            mL[wid][(rg * RT + i) * 16 + r] = m[i];
-            lL[wid][(rg * RT + i) * 16 + r] = l[i];
+            mL[wid][i * 16 + r] = m[i];
+            lL[wid][i * 16 + r] = l[i];
         }
 #pragma unroll
-        for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4_t*>(oL + (wid * ROWS + (rg * RT + i) * 16 + r) * OROW + 16 * t + 4 * q) = acc[i][t];
+        for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4_t*>(oL + (wid * ROWS + i * 16 + r) * OROW + 16 * t + 4 * q) = acc[i][t];
     }
     const bool any_odd = __syncthreads_or(odd);
-    const bool whole = filled_splits_tree(a, s.total) <= 1;
+    const bool whole = splits == 1;
 #pragma unroll 1
-    for (int it = threadIdx.x; it < ROWS * (D / 4); it += RG * 256) {
+    for (int it = threadIdx.x; it < ROWS * (D / 4); it += 256) {
         const int rr = it / (D / 4), c = it % (D / 4) * 4, sr = row0 + rr;
         if (sr >= stacked) break;
         float top = mL[0][rr];
@@ -524,7 +546,7 @@ __global__ __launch_bounds__(RG * 256, 2) void tree_attn_narrow_kernel(TreeArgs 
             den = fmaf(lL[w][rr], f, den);
             o += *reinterpret_cast<const f32x4_t*>(oL + (w * ROWS + rr) * OROW + c) * f;
         }
-        if (any_odd) add_odd<false, D>(a, s, b, kvh, split, 32, sr, c, o);
+        if (any_odd) add_odd<false, D>(a, s, b, kvh, split, splits, 32, sr, c, o);
         leave_rows<false, D>(a, s, whole, split, kvh, sr, c, top, den, o);
     }
 }
@@ -572,13 +594,16 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     const int unit = within / (8 * a.row_blocks) * 8 + within % 8, rb = within / 8 % a.row_blocks;
     if (unit >= units) return;
     const int kvh = unit % a.hkv, b = unit / a.hkv;
+    const int rounds = step_rounds(a);
     const TreeSpan s = tree_span(a, b);
     // a row's stacked rows in as few parts as 128 allow, of even size
     const int stacked = s.n * a.g, parts = (stacked + 127) / 128;
-    if (rb >= parts || split >= filled_splits_tree(a, s.total)) return;
+    if (rb >= parts || (split > 0 && split * 64 * a.least >= s.total)) return;
+    const int splits = row_splits(a, s.total, rounds);
+    if (split >= splits) return;
     const int part_rows = ((stacked + parts - 1) / parts + 31) & ~31, row0 = rb * part_rows;
     if (row0 >= stacked) return;
-    const int tiles = (s.total + KT - 1) / KT, per = run_tiles(a, s.total), t0 = split * per, t1 = min(t0 + per, tiles);
+    const int tiles = (s.total + KT - 1) / KT, per = (tiles + splits - 1) / splits, t0 = split * per, t1 = min(t0 + per, tiles);
     const int my_rows = min(part_rows, stacked - row0);
     const bool active = wid * 32 < my_rows;                     // uniform over the wave
     const int sr = min(row0 + wid * 32 + lq, stacked - 1), node = sr / a.g, head = kvh * a.g + sr - node * a.g;
@@ -954,7 +979,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
                 }
         });
     const float den = lrun0 + lrun1 + __shfl_xor(lrun0 + lrun1, 32, 64);
-    const bool whole = filled_splits_tree(a, s.total) <= 1;
+    const bool whole = splits == 1;
     const int64_t tok = s.start + node;
     const float inv = den != 0.f ? 1.0f / den : 0.f;
     const int64_t at = ((int64_t)split * a.tokens + tok) * a.hq + head;
@@ -984,7 +1009,7 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a, int sh
     __shared__ f32x4_t oL[256];
     const int b = blockIdx.y, group = threadIdx.x / LPR, part = group & ((1 << shift) - 1), c = threadIdx.x % LPR * 4;
     const TreeSpan s = tree_span(a, b);
-    const int filled = filled_splits_tree(a, s.total);
+    const int filled = row_splits(a, s.total, step_rounds(a));
     if (filled <= 1 || (int64_t)blockIdx.x * (GROUPS >> shift) >= (int64_t)s.n * a.hq) return;
     const int64_t item = (int64_t)blockIdx.x * (GROUPS >> shift) + (group >> shift), step = (int64_t)a.tokens * a.hq;
     const int node = (int)min(item / a.hq, (int64_t)s.n - 1), head = (int)(item % a.hq);
@@ -1042,18 +1067,36 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a, int sh
     X::st4((typename X::T*)a.out + t * a.ldo + (int64_t)head * D + c, o * inv);
 }
 
-// Rows, workgroups and keys of a launch
+// Which kernel a launch takes, with rows, workgroups and keys of its workgroups.
+// Where few workgroups have short rows, latency counts: a workgroup of 16 rows is the quickest through its keys, and as many of them as the chip has
+// units ask for the same keys again out of L2 (us, rows 1, 32 heads of 64 on 4, 7 nodes behind 45 keys: 16 rows a workgroup 5.1, 32 6.2, 64 8.1, the wide
+// form 6.9; 500 keys 6.9, 8.7, 11.6; 32 heads of 128 on 8, 64 nodes behind 300 keys 11.1, 12.3, -, 16.7).  Past `reach` (workgroups times keys) that
+// traffic is what they take: 4 rows of 4000 keys, 16 nodes, heads of 64 18.5, 15.5, 17.8, 17.1; heads of 128 45.6, 31.1, -, 24.3.  Then a workgroup
+// takes the rows it can: 64 of heads of 64 (32 rows of 4096 and 8 nodes 34.5, wide 36.9), 32 of heads of 128 (107; 64 in two groups of waves 183, wide 120),
+// and what is more goes to the wide form.
 struct TreeForm {
-    int row_tiles, row_blocks, round_keys, wide;
+    int row_tiles, row_part, row_blocks, round_keys, wide, slots, least;
 };
-static TreeForm tree_form(int max_nodes, int g, int d, int f32) {
-    const int64_t stacked = (int64_t)max_nodes * g;
+static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f32, int64_t max_keys) {
+    const int64_t stacked = (int64_t)max_nodes * g, heads = (int64_t)rows * hkv;
+    auto fits = [&](int tiles, int most, int64_t reach) {
+        const int64_t wgs = heads * ((stacked + 16 * tiles - 1) / (16 * tiles));
+        return wgs <= most && wgs * max_keys <= reach;
+    };
     TreeForm f;
-    f.wide = !f32 && stacked > 64;
-    f.row_tiles = f32 ? 2 : stacked <= 16 ? 1 : stacked <= 32 ? 2 : 4;
-    const int rows = f.wide ? 128 : 16 * f.row_tiles;
-    f.row_blocks = (int)((stacked + rows - 1) / rows);
-    f.round_keys = f.wide ? 64 * kTreeRunTiles : f32 ? 64 : 128;
+    f.wide = 0;
+    if (f32) f.row_tiles = 2;
+    else if (stacked <= 16 || fits(1, num_cus(), d == 64 ? 200000 : 50000)) f.row_tiles = 1;
+    else if (stacked <= 32 || fits(2, d == 64 ? num_cus() : num_cus() / 2, d == 64 ? 300000 : 64000)) f.row_tiles = 2;
+    else f.row_tiles = 4, f.wide = d == 128 || stacked > 64;
+    f.row_part = f.wide ? 128 : 16 * f.row_tiles;
+    f.row_blocks = (int)((stacked + f.row_part - 1) / f.row_part);
+    f.round_keys = f.wide || f32 ? 64 : 128;
+    // Work for one workgroup a unit, or for two where there are two without any cut (wide, us with one and two: 32 uneven rows of up to 8191, 64 nodes
+    // of 8B heads 211, 205; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4)
+    const bool two = f.wide ? heads * f.row_blocks >= 2 * num_cus() : f32 && d == 64;
+    f.slots = num_cus() * (two ? 2 : 1);
+    f.least = f.wide ? 6 : 1;
     return f;
 }
 
@@ -1069,10 +1112,12 @@ size_t mv_tree_attn_workspace_bytes(int tokens, int hq, int d, int num_splits) {
 int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, int max_keys, int f32) {
     using namespace mv;
     if (rows <= 0 || max_nodes <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || max_keys <= 0) return 1;
-    const TreeForm f = tree_form(max_nodes, hq / hkv, d, f32);
-    const int64_t units = (int64_t)rows * hkv * f.row_blocks;
-    int64_t splits = (num_cus() + units - 1) / units;
-    const int64_t most = ((int64_t)max_keys + f.round_keys - 1) / f.round_keys;
+    const TreeForm f = tree_form(rows, max_nodes, hkv, hq / hkv, d, f32, max_keys);
+    // the launch that joins the splits costs some 3 us, a round of a workgroup 0.5 (heads of 64) to 1.2 (of 128): short rows are not cut
+    if (max_keys <= (f32 ? 384 : d == 64 ? 1152 : 512)) return 1;
+    // (as many as the kernels may want: they cut a row in fewer where its keys or the step's rows do not ask for them)
+    const int64_t units = (int64_t)rows * hkv * f.row_blocks, most = ((int64_t)max_keys + f.round_keys * f.least - 1) / (f.round_keys * f.least);
+    int64_t splits = units < f.slots ? (f.slots + units - 1) / units * (rows > 1 ? 2 : 1) : rows > 1 && max_keys >= 2048 ? 4 : 1;
     if (splits > most) splits = most;
     return (int)(splits < 1 ? 1 : splits > kTreeMaxSplits ? kTreeMaxSplits : splits);
 }
@@ -1122,26 +1167,27 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     a.page_shift = __builtin_ctz((unsigned)page);
     a.num_pages = num_pages;
     a.nsplit = num_splits;
-    const TreeForm f = tree_form(max_nodes, a.g, d, f32);
+    const TreeForm f = tree_form(rows, max_nodes, hkv, a.g, d, f32, (int64_t)bt_cols << a.page_shift);
     a.row_blocks = f.row_blocks;
     a.round_keys = f.round_keys;
-    a.wide = f.wide;
+    a.row_part = f.row_part;
+    a.slots = f.slots;
+    a.least = f.least;
     a.scale_log2 = scale * 1.4426950408889634f;
     const int64_t grid = ((int64_t)rows * hkv + (f.wide ? 7 : 0)) / (f.wide ? 8 : 1) * (f.wide ? 8 : 1) * a.row_blocks * num_splits;
     if (grid > 0x7fffffff || rows > 65535) return MV_ERR_UNSUPPORTED;
     hipStream_t s = (hipStream_t)stream;
     const dim3 g1((unsigned)grid);
-#define MV_TREE(K_, T_) hipLaunchKernelGGL((K_), g1, dim3(T_), 0, s, a)
-    if (f32 && d == 64) MV_TREE((tree_attn_f32_kernel<64>), 256);
-    else if (f32) MV_TREE((tree_attn_f32_kernel<128>), 256);
-    else if (f.wide && d == 64) MV_TREE((tree_attn_wide_kernel<64>), 256);
-    else if (f.wide) MV_TREE((tree_attn_wide_kernel<128>), 256);
-    else if (d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<64, 1, 1>), 256);
-    else if (d == 64 && f.row_tiles == 2) MV_TREE((tree_attn_narrow_kernel<64, 2, 1>), 256);
-    else if (d == 64) MV_TREE((tree_attn_narrow_kernel<64, 4, 1>), 256);
-    else if (f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<128, 1, 1>), 256);
-    else if (f.row_tiles == 2) MV_TREE((tree_attn_narrow_kernel<128, 2, 1>), 256);
-    else MV_TREE((tree_attn_narrow_kernel<128, 2, 2>), 512);
+#define MV_TREE(K_) hipLaunchKernelGGL((K_), g1, dim3(256), 0, s, a)
+    if (f32 && d == 64) MV_TREE((tree_attn_f32_kernel<64>));
+    else if (f32) MV_TREE((tree_attn_f32_kernel<128>));
+    else if (f.wide && d == 64) MV_TREE((tree_attn_wide_kernel<64>));
+    else if (f.wide) MV_TREE((tree_attn_wide_kernel<128>));
+    else if (d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<64, 1>));
+    else if (d == 64 && f.row_tiles == 2) MV_TREE((tree_attn_narrow_kernel<64, 2>));
+    else if (d == 64) MV_TREE((tree_attn_narrow_kernel<64, 4>));
+    else if (f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<128, 1>));
+    else MV_TREE((tree_attn_narrow_kernel<128, 2>));
 #undef MV_TREE
     if (num_splits > 1) {
         const int groups = 1024 / d;

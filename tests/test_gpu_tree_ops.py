@@ -298,14 +298,45 @@ def test_places_without_a_page_do_not_count(ops, dtype):
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_scores_of_any_size(ops, dtype):
     """Scores of hundreds on either side of zero, and one key that outweighs all others wherever it lies."""
-    case = AttnCase([130], [24], 4, 2, 64, 64, dtype, seed=11, scale_q=30.0)
-    case.check(run_attn(ops, case), "large scores")
-    for at in (0, 15, 16, 63, 64, 129, 131):
-        case = AttnCase([130], [24], 4, 2, 64, 64, dtype, seed=12)
-        p, s = case.table[0][at // 64], at % 64
-        case.k[p, s] = case.q[5, ::2].to(F32).to(dtype) * 4
-        for splits in (1, 3):
-            case.check(run_attn(ops, case, splits), f"key {at}")
+    for hq, hkv in ((4, 2), (8, 1)):
+        case = AttnCase([130], [24], hq, hkv, 64, 64, dtype, seed=11, scale_q=30.0)
+        case.check(run_attn(ops, case), "large scores")
+        for at in (0, 15, 16, 63, 64, 129, 131):
+            case = AttnCase([130], [24], hq, hkv, 64, 64, dtype, seed=12)
+            p, s = case.table[0][at // 64], at % 64
+            case.k[p, s] = case.q[5, ::hq // hkv].to(F32).to(dtype) * 4
+            for splits in (1, 3):
+                case.check(run_attn(ops, case, splits), f"key {at}")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (8, 1)])
+@pytest.mark.parametrize("step", [-1.0, 1.0])
+def test_scores_that_rise_or_fall_along_the_keys(ops, d, hq, hkv, step):
+    """Scores that climb (fall) by one per key, over hundreds: no key of the first block says anything about the last ones', and nothing before
+    them has a weight left.  The second half of the keys is out of reach of the first by more than fp32's range."""
+    case = AttnCase([700, 0, 90], [20, 30, 24], hq, hkv, d, 64, BF16, seed=13)
+    case.q.zero_()
+    case.q[:, :, 0], case.q[:, :, 1] = d ** 0.5, 1.0
+    for b, (c, n) in enumerate(zip(case.ctx, case.counts)):
+        for j in range(c + n):
+            p, s = case.table[b][j // 64], j % 64
+            case.k[p, s, :, 0] = step * j
+    for splits in (0, 1, 2):
+        case.check(run_attn(ops, case, splits), f"splits {splits}")
+
+
+def test_values_near_the_end_of_the_range(ops):
+    """Values of 2^100 and scores 30 above those of the first keys: no sum may overflow on the way."""
+    case = AttnCase([400], [24], 8, 1, 64, 64, BF16, seed=14)
+    case.v.mul_(2.0 ** 100)
+    for j in (200, 390, 405):
+        p, s = case.table[0][j // 64], j % 64
+        case.k[p, s] = case.q[7, ::8].to(F32).to(BF16) * 4
+    for splits in (0, 1, 2):
+        out = run_attn(ops, case, splits)
+        assert torch.isfinite(out[:case.T].float()).all()
+        case.check(out, f"splits {splits}")
 
 
 def test_a_long_cache_past_32_bit_offsets(ops):
