@@ -565,7 +565,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn_narrow_kernel(TreeArgs a) {
 //     its first block - makes the workgroup do its keys again with a running maximum.  (The maximum of every block, its exchange between lanes and
 //     the test for a rescale were a fifth of the vector unit's work: 32 rows of 4096 and 64 nodes 188 -> 165 us.)
 //   * a tile in which every key counts for every row (all but the one or two with nodes in them) takes no mask.
-// Waves without rows (short trees) only stage.
+// Waves without rows (short trees) only stage.  KW 2, for up to 64 rows: two waves take the two 32-key blocks of a tile for the same 32 rows and join
+// their states at the end.
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 
 __device__ __forceinline__ float max3_tree(float a, float b, float c) {      // (fmaxf of a product's result is a self-maximum more)
@@ -580,7 +581,7 @@ __device__ __forceinline__ void wait_landed() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
-template <int D>
+template <int D, int KW>
 __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     constexpr int KT = 64, KS = D / 16, DB = D / 32, NP = 2 * DB;
     constexpr int PF = 3, PFV = NP - 1 < 7 ? NP - 1 : 7;        // reads of keys and values in front of their matrix instruction
@@ -596,8 +597,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     const int kvh = unit % a.hkv, b = unit / a.hkv;
     const int rounds = step_rounds(a);
     const TreeSpan s = tree_span(a, b);
-    // a row's stacked rows in as few parts as 128 allow, of even size
-    const int stacked = s.n * a.g, parts = (stacked + 127) / 128;
+    // a row's stacked rows in as few parts as 128 (64) allow, of even size
+    const int stacked = s.n * a.g, parts = (stacked + 128 / KW - 1) / (128 / KW);
     if (rb >= parts || (split > 0 && split * 64 * a.least >= s.total)) return;
     const int splits = row_splits(a, s.total, rounds);
     if (split >= splits) return;
@@ -605,9 +606,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     if (row0 >= stacked) return;
     const int tiles = (s.total + KT - 1) / KT, per = (tiles + splits - 1) / splits, t0 = split * per, t1 = min(t0 + per, tiles);
     const int my_rows = min(part_rows, stacked - row0);
-    const bool active = wid * 32 < my_rows;                     // uniform over the wave
-    const int sr = min(row0 + wid * 32 + lq, stacked - 1), node = sr / a.g, head = kvh * a.g + sr - node * a.g;
-    const bool stored = wid * 32 + lq < my_rows;
+    const int rg = KW == 1 ? wid : wid & 1, kh = KW == 1 ? 0 : wid >> 1;      // the wave's rows, and its block of a tile
+    const bool active = rg * 32 < my_rows;                      // uniform over the wave
+    const int sr = min(row0 + rg * 32 + lq, stacked - 1), node = sr / a.g, head = kvh * a.g + sr - node * a.g;
+    const bool stored = rg * 32 + lq < my_rows;
 
     bf16x8_t qf[KS];
     {
@@ -897,8 +899,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
             }
             if (!(report(false) & 2)) break;
         }
+        if (KW == 2) __syncthreads();
         return;
     }
+    auto mine = [&](uint64_t keys) __attribute__((always_inline)) -> uint64_t { return KW == 1 ? keys : keys >> (32 * kh) & 0xffffffffull; };
 
     f32x16_t s0, s1;
     auto tile_step = [&](int t, auto masks) __attribute__((always_inline)) {
@@ -907,13 +911,20 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
         const uint64_t last = request(t);
         uint32_t vis1 = 0, vis2 = 0;
         if constexpr (kMask) {
-            const uint64_t here = visible(t, bits[0]), there = visible(t + 1, bits[1]);
+            const uint64_t here = mine(visible(t, bits[0])), there = mine(visible(t + 1, bits[1]));
             saw |= (here | there) != 0;
             vis1 = (uint32_t)(here >> 32) >> (4 * hi);
             vis2 = (uint32_t)there >> (4 * hi);
         }
-        block_step(s0, s1, kcur + 32 * RB, vcur, knext, vis1, yes, yes, masks);
-        block_step(s1, s0, knext, vcur + 32 * RB, knext + 32 * RB, vis2, yes, yes, masks);
+        if constexpr (KW == 1) {
+            block_step(s0, s1, kcur + 32 * RB, vcur, knext, vis1, yes, yes, masks);
+            block_step(s1, s0, knext, vcur + 32 * RB, knext + 32 * RB, vis2, yes, yes, masks);
+        } else {
+#pragma unroll
+            for (int k = 0; k < PF; ++k) kpre[k] = k_frag(knext + kh * 32 * RB, k);
+            block_step(s0, s1, knext + kh * 32 * RB, vcur + kh * 32 * RB, nullptr, vis2, yes, no, masks);
+            s0 = s1;
+        }
         turn(t, last, kMask);
     };
     int flags;
@@ -928,8 +939,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s0[i] = 0.f;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(kring, k), qf[k], s0, 0, 0, 0);
-        const uint64_t first = visible(t0, bits[0]);
+        for (int k = 0; k < KS; ++k) s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(kring + kh * 32 * RB, k), qf[k], s0, 0, 0, 0);
+        const uint64_t first = mine(visible(t0, bits[0]));
         saw = first != 0;
 #pragma unroll
         for (int mi = 0; mi < 4; ++mi) mask_piece(s0, mi, (uint32_t)first >> (4 * hi));
@@ -937,12 +948,16 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
             mrun = block_max(s0);
             if (!(fabsf(mrun) <= 3.4028235e38f)) mrun = 0.f;      // nothing seen yet
         }
+        if constexpr (KW == 1) {
 #pragma unroll
-        for (int k = 0; k < PF; ++k) kpre[k] = k_frag(kring + 32 * RB, k);
+            for (int k = 0; k < PF; ++k) kpre[k] = k_frag(kring + 32 * RB, k);
+        }
         int t = t0;
         for (; t + 1 < open_end; ++t) tile_step(t, no);
         for (; t + 1 < t1; ++t) tile_step(t, yes);
-        {   // the last tile: nothing follows its second block
+        if constexpr (KW == 2) {
+            block_step(s0, s1, nullptr, vring + vslot * TB + kh * 32 * RB, nullptr, 0, no, no, no);
+        } else {   // the last tile: nothing follows its second block
             const uint32_t vis1 = (uint32_t)(visible(t, bits[0]) >> 32) >> (4 * hi);
             const unsigned char *kcur = kring + kslot * TB, *vcur = vring + vslot * TB;
             block_step(s0, s1, kcur + 32 * RB, vcur, nullptr, vis1, yes, no, yes);
@@ -964,6 +979,33 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
         exact = true;
     }
     if (!saw) mrun = kTreeNegBig;
+    float den = lrun0 + lrun1 + __shfl_xor(lrun0 + lrun1, 32, 64);
+    if constexpr (KW == 2) {       // the states of a row's two waves: lane by lane through the ring
+        constexpr int EACH = DB * 16 + 4;
+        float* at = reinterpret_cast<float*>(ring) + (rg * 64 + lane) * EACH;
+        if (kh == 1) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<f32x4_t*>(at + db * 16 + i) = (f32x4_t){oacc[db][i], oacc[db][i + 1], oacc[db][i + 2], oacc[db][i + 3]};
+            at[DB * 16] = mrun;
+            at[DB * 16 + 1] = den;
+        }
+        __syncthreads();
+        if (kh == 1) return;
+        const float m1 = at[DB * 16], top = fmaxf(mrun, m1), f0 = __builtin_amdgcn_exp2f(mrun - top), f1 = __builtin_amdgcn_exp2f(m1 - top);
+        den = fmaf(at[DB * 16 + 1], f1, den * f0);
+        mrun = top;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4_t o = *reinterpret_cast<const f32x4_t*>(at + db * 16 + i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) oacc[db][i + j] = fmaf(o[j], f1, oacc[db][i + j] * f0);
+            }
+    }
     if (!stored) return;
     // oacc[db][i] = O^T[32 db + (i & 3) + 8 (i >> 2) + 4 hi][row]
     if (flags & 1)
@@ -978,7 +1020,6 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
                         if (is_odd(x[j])) oacc[db][4 * k + j] += x[j];
                 }
         });
-    const float den = lrun0 + lrun1 + __shfl_xor(lrun0 + lrun1, 32, 64);
     const bool whole = splits == 1;
     const int64_t tok = s.start + node;
     const float inv = den != 0.f ? 1.0f / den : 0.f;
@@ -1089,7 +1130,7 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     else if (stacked <= 16 || fits(1, num_cus(), d == 64 ? 200000 : 50000)) f.row_tiles = 1;
     else if (stacked <= 32 || fits(2, d == 64 ? num_cus() : num_cus() / 2, d == 64 ? 300000 : 64000)) f.row_tiles = 2;
     else f.row_tiles = 4, f.wide = d == 128 || stacked > 64;
-    f.row_part = f.wide ? 128 : 16 * f.row_tiles;
+    f.row_part = f.wide ? (stacked <= 64 ? 64 : 128) : 16 * f.row_tiles;
     f.row_blocks = (int)((stacked + f.row_part - 1) / f.row_part);
     f.round_keys = f.wide || f32 ? 64 : 128;
     // Work for one workgroup a unit, or for two where there are two without any cut (wide, us with one and two: 32 uneven rows of up to 8191, 64 nodes
@@ -1181,8 +1222,9 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
 #define MV_TREE(K_) hipLaunchKernelGGL((K_), g1, dim3(256), 0, s, a)
     if (f32 && d == 64) MV_TREE((tree_attn_f32_kernel<64>));
     else if (f32) MV_TREE((tree_attn_f32_kernel<128>));
-    else if (f.wide && d == 64) MV_TREE((tree_attn_wide_kernel<64>));
-    else if (f.wide) MV_TREE((tree_attn_wide_kernel<128>));
+    else if (f.wide && d == 64) MV_TREE((tree_attn_wide_kernel<64, 1>));      // (64 rows of such heads: the narrow form)
+    else if (f.wide && f.row_part == 64) MV_TREE((tree_attn_wide_kernel<128, 2>));
+    else if (f.wide) MV_TREE((tree_attn_wide_kernel<128, 1>));
     else if (d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<64, 1>));
     else if (d == 64 && f.row_tiles == 2) MV_TREE((tree_attn_narrow_kernel<64, 2>));
     else if (d == 64) MV_TREE((tree_attn_narrow_kernel<64, 4>));
