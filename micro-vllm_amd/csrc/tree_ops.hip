@@ -236,6 +236,109 @@ __global__ __launch_bounds__(256) void slot_store_any_kernel(SlotStoreArgs a) {
     }
 }
 
+// The forms of a head that are read as they lie: d / 8 = LPH lanes of eight values, whole pieces of the rotated part.  Workgroup = (token, some of its
+// heads): it forms the angles' sines and cosines once, for all of them, and leaves them with the weights in LDS; a lane asks for its own eight
+// values and (pairs half a head apart) for its partners', which a neighbour has too, out of L1: no exchange.  Bound by memory: 2048 tokens of 32 + 2 x 8
+// heads of 128 in bf16, 50 MB, 13 us (3.9 TB/s; a wave per head and value by value 39).
+template <bool F32>
+__device__ __forceinline__ void ld8(const void* base, int64_t at, float (&v)[8]) {
+    if constexpr (F32) {
+        const f32x4_t a = *reinterpret_cast<const f32x4_t*>((const float*)base + at), b = *reinterpret_cast<const f32x4_t*>((const float*)base + at + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+    } else {
+        const uint4 w = ld16((const uint16_t*)base + at);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(u[i]), v[2 * i + 1] = bf16_hi(u[i]);
+    }
+}
+template <bool F32>
+__device__ __forceinline__ void st8(void* base, int64_t at, const float (&v)[8]) {
+    if constexpr (F32) {
+        *reinterpret_cast<f32x4_t*>((float*)base + at) = (f32x4_t){v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_t*>((float*)base + at + 4) = (f32x4_t){v[4], v[5], v[6], v[7]};
+    } else {
+        st16((uint16_t*)base + at, make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])));
+    }
+}
+
+template <bool SF32, bool DF32, int LPH>
+__global__ __launch_bounds__(256) void slot_store_kernel(SlotStoreArgs a, int heads_per_wg) {
+    constexpr int D = LPH * 8, HP = 256 / LPH;
+    __shared__ __attribute__((aligned(16))) float wL[2][D], csL[D / 2], snL[D / 2];
+    const int units = a.hq + 2 * a.hkv, groups = (units + heads_per_wg - 1) / heads_per_wg, tid = threadIdx.x, half = a.rot / 2;
+    const int64_t t = blockIdx.x / groups;
+    const int u0 = (int)(blockIdx.x % groups) * heads_per_wg, u1 = min(u0 + heads_per_wg, units), e = tid % LPH * 8;
+    const int64_t slot = a.slots[t];
+    const bool turned = e < a.rot, low = e < half;
+    const int partner = a.adjacent || !turned ? e : low ? e + half : e - half;
+    const int64_t row = t * a.ld;
+    float x[8], y[8];
+    auto fetch = [&](int u) {
+        const int h = min(u, units - 1);
+        ld8<SF32>(a.qkv, row + (int64_t)h * D + e, x);
+        ld8<SF32>(a.qkv, row + (int64_t)h * D + partner, y);
+    };
+    fetch(u0 + tid / LPH);
+    for (int i = tid; i < half; i += 256) {
+        float sn, cs;
+        sincos_turn(a.positions[t], a.inv_freq[i], sn, cs);
+        csL[i] = cs;
+        snL[i] = sn;
+    }
+    for (int i = tid; i < D; i += 256) {
+        wL[0][i] = a.q_norm ? a.q_norm[i] : 1.f;
+        wL[1][i] = a.k_norm ? a.k_norm[i] : 1.f;
+    }
+    __syncthreads();
+    for (int first = u0; first < u1; first += HP) {       // (the same trips for every lane: exchanges below)
+        const int u = first + tid / LPH;
+        if (first > u0) fetch(u);
+        const bool is_q = u < a.hq, is_v = u >= a.hq + a.hkv;
+        float o[8];
+        if (is_v) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = x[i];
+        } else {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+            for (int k = 1; k < LPH; k <<= 1) ss += __shfl_xor(ss, k, 64);      // (a head's lanes go the same way)
+            const float inv = (is_q ? a.q_norm : a.k_norm) ? 1.0f / sqrtf(ss / (float)D + a.eps) : 1.f;
+            const float* w = wL[is_q ? 0 : 1];
+            float xw[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) xw[i] = x[i] * inv * w[e + i];
+            if (!turned) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = xw[i];
+            } else if (a.adjacent) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float cs = csL[e / 2 + i], sn = snL[e / 2 + i];
+                    o[2 * i] = xw[2 * i] * cs - xw[2 * i + 1] * sn;
+                    o[2 * i + 1] = xw[2 * i + 1] * cs + xw[2 * i] * sn;
+                }
+            } else {
+                const int at = low ? e : e - half;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float yw = y[i] * inv * w[partner + i], sn = snL[at + i];
+                    o[i] = xw[i] * csL[at + i] + yw * (low ? -sn : sn);
+                }
+            }
+        }
+        if (u >= u1) continue;
+        if (is_q) {
+            st8<DF32>(a.q_out, t * a.ldq + (int64_t)u * D + e, o);
+        } else if (slot >= 0 && slot < a.slots_n) {
+            st8<DF32>(is_v ? a.v_cache : a.k_cache, (slot * a.hkv + (u - a.hq - (is_v ? a.hkv : 0))) * D + e, o);
+        }
+    }
+}
+
 // ------------------------------------------------------------------ accept
 
 constexpr int kAcceptLayers = 64;      // layers of one launch: their addresses travel in its arguments
@@ -247,7 +350,7 @@ struct AcceptArgs {
     int row_vecs;                      // 16-byte pieces of one token's keys in a layer
     int64_t* ids;
     int32_t *path, *counts, *lens;     // NULL behind the first launch
-    uint4* cache[2 * kAcceptLayers];   // keys of the layers, then values
+    u32x4_t* cache[2 * kAcceptLayers];   // keys of the layers, then values
 };
 
 // Workgroup = (row, 256 of its pieces: a piece is 16 bytes of a token's keys or values in a layer).  Each workgroup walks for itself:
@@ -314,16 +417,25 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(AcceptArgs a) {
         };
         const int64_t s = place(ctx + pathL[tid]), e = place(ctx + tid);
         srcL[tid] = s;
-        dstL[tid] = s < 0 ? -1 : e;
+        dstL[tid] = s < 0 || pathL[tid] == tid ? -1 : e;
     }
     __syncthreads();
     const int64_t item = (int64_t)blockIdx.y * 256 + tid;
     if (item >= (int64_t)2 * a.layers * a.row_vecs) return;
     const int which = (int)(item / a.row_vecs), vec = (int)(item % a.row_vecs);
-    uint4* cache = a.cache[which < a.layers ? which : kAcceptLayers + which - a.layers] + vec;
-    for (int j = 0; j < count; ++j) {
-        if (pathL[j] == j || dstL[j] < 0) continue;
-        cache[dstL[j]] = cache[srcL[j]];
+    u32x4_t* cache = a.cache[which < a.layers ? which : kAcceptLayers + which - a.layers] + vec;
+    // eight moves at a time, all read before the first is written: sources lie behind every place that was written in front of them
+    for (int first = 0; first < count; first += 8) {
+        u32x4_t v[8];
+        int64_t to[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            to[i] = first + i < count ? dstL[first + i] : -1;
+            if (to[i] >= 0) v[i] = cache[srcL[first + i]];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (to[i] >= 0) cache[to[i]] = v[i];
     }
 }
 
@@ -367,10 +479,31 @@ int mv_qkv_norm_rotary_slots(const void* qkv, int64_t ld, const float* q_norm, c
         return MV_ERR_INVALID_ARG;
     SlotStoreArgs a{qkv, ld, q_norm, k_norm, eps, inv_freq, rot, adjacent, positions, slots, q_out, ldq, k_cache, v_cache, tokens, heads,
                     kv_heads, d, cache_slots};
-    const int64_t blocks = ((int64_t)tokens * (heads + 2 * kv_heads) + 3) / 4;
+    hipStream_t s = (hipStream_t)stream;
+    const int units = heads + 2 * kv_heads, sv = src_f32 ? 4 : 8, dv = dst_f32 ? 4 : 8;
+    const bool pieces = (d == 64 || d == 128 || d == 256) && rot % (adjacent ? 8 : 16) == 0 && ld % sv == 0 && ldq % dv == 0 && aligned16(qkv) &&
+                        aligned16(q_out) && aligned16(k_cache) && aligned16(v_cache);
+    if (pieces) {
+        // a token's heads in one workgroup where there are tokens for the chip, else in as many as there are rounds of 256 lanes
+        const int round = 256 / (d / 8), hpw = tokens >= 4 * num_cus() ? (units + round - 1) / round * round : round;
+        const int64_t blocks = (int64_t)tokens * ((units + hpw - 1) / hpw);
+        if (blocks > 0x7fffffff) return MV_ERR_UNSUPPORTED;
+        const dim3 grid((unsigned)blocks);
+#define MV_STORE(S_, D_)                                                                                                      \
+    do {                                                                                                                     \
+        if (d == 64) hipLaunchKernelGGL((slot_store_kernel<S_, D_, 8>), grid, dim3(256), 0, s, a, hpw);                         \
+        else if (d == 128) hipLaunchKernelGGL((slot_store_kernel<S_, D_, 16>), grid, dim3(256), 0, s, a, hpw);                  \
+        else hipLaunchKernelGGL((slot_store_kernel<S_, D_, 32>), grid, dim3(256), 0, s, a, hpw);                               \
+    } while (0)
+        if (src_f32 && dst_f32) MV_STORE(true, true);
+        else if (src_f32) MV_STORE(true, false);
+        else MV_STORE(false, false);
+#undef MV_STORE
+        return check_launch();
+    }
+    const int64_t blocks = ((int64_t)tokens * units + 3) / 4;
     if (blocks > 0x7fffffff) return MV_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)blocks);
-    hipStream_t s = (hipStream_t)stream;
     if (src_f32 && dst_f32) hipLaunchKernelGGL((slot_store_any_kernel<true, true>), grid, dim3(256), 0, s, a);
     else if (src_f32) hipLaunchKernelGGL((slot_store_any_kernel<true, false>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((slot_store_any_kernel<false, false>), grid, dim3(256), 0, s, a);
@@ -399,8 +532,8 @@ int mv_tree_accept(const int64_t* tokens, const int64_t* picks, const int32_t* p
     for (int first = 0; first == 0 || first < layers; first += kAcceptLayers) {
         a.layers = layers - first < kAcceptLayers ? layers - first : kAcceptLayers;
         for (int i = 0; i < a.layers; ++i) {
-            a.cache[i] = (uint4*)k_caches[first + i];
-            a.cache[kAcceptLayers + i] = (uint4*)v_caches[first + i];
+            a.cache[i] = (u32x4_t*)k_caches[first + i];
+            a.cache[kAcceptLayers + i] = (u32x4_t*)v_caches[first + i];
         }
         const int64_t items = (int64_t)2 * a.layers * a.row_vecs, parts = items > 0 ? (items + 255) / 256 : 1;
         if (parts > 65535) return MV_ERR_UNSUPPORTED;
