@@ -73,18 +73,19 @@ __device__ __forceinline__ int row_splits(const TreeArgs& a, int total, int work
     const int share = max((int)((sum * a.hkv + a.slots - 1) / a.slots), a.least), rounds = (total + a.round_keys - 1) / a.round_keys;
     return max(1, min(a.nsplit, (rounds + share - 1) / share));
 }
-// 64 bits of a node's mask from bit `first` (negative: cached tokens in front of the nodes, visible) on
-__device__ __forceinline__ uint64_t mask_from(const uint64_t (&w)[kTreeMaxWords], int first) {
-    if (first <= -64) return ~0ull;
-    if (first < 0) return (w[0] << -first) | ((1ull << -first) - 1);
-    uint64_t lo = 0, hi = 0;
-    const int at = first >> 6, sh = first & 63;
-#pragma unroll
-    for (int i = 0; i < kTreeMaxWords; ++i) {
-        if (i == at) lo = w[i];
-        if (i == at + 1) hi = w[i];
+// Which of the 32 keys from kb on a node sees (bit i: key kb + i): cached tokens all, nodes by its mask, whose first word is given
+__device__ __forceinline__ uint32_t visible_keys(const TreeArgs& a, const TreeSpan& s, int node, uint64_t word0, int kb) {
+    const int first = kb - s.ctx;
+    if (!a.mask) {
+        const int up = node + 1 - first;
+        return up >= 32 ? ~0u : up > 0 ? (1u << up) - 1 : 0;
     }
-    return sh ? (lo >> sh) | (hi << (64 - sh)) : lo;
+    if (first < 0) return first <= -32 ? ~0u : (uint32_t)(word0 << -first) | ((1u << -first) - 1);
+    const int at = first >> 6, sh = first & 63;
+    const uint64_t* w = a.mask + (int64_t)(s.start + node) * a.words;
+    uint64_t v = (at == 0 ? word0 : at < a.words ? w[at] : 0) >> sh;
+    if (sh > 32 && at + 1 < a.words) v |= w[at + 1] << (64 - sh);
+    return (uint32_t)v;
 }
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
@@ -181,19 +182,22 @@ __device__ __forceinline__ void add_odd(const TreeArgs& a, const TreeSpan& s, in
 // Both products on v_mfma_f32_16x16x4_f32 (operand A lane (r, q) = A[r][slot q], B likewise, result lane (r, q) = C[4 q + j][r]); the
 // contraction's slots are labels.  S^T = K . Q^T: slot q of step j of a group of 16 dimensions is dimension 4 q + j, so a key's and a
 // query's values are read 16 (8) bytes a lane.  O^T = V^T . P^T: slot q of step j is key 4 q + j, which is where S^T left its score;
-// row r of output block c is dimension 64 h + 4 r + c, so a value row too is read as it lies.  Nothing goes through LDS until the end.
-template <int D>
-__global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
+// row r of output block c is dimension 64 h + 4 r + c, so a value row too is read as it lies.  Nothing goes through LDS until the end.  The
+// next block's keys are requested into the registers that the scores leave, its values into those that the sums leave.
+template <int D, int RT>
+__global__ __launch_bounds__(256, 2) void tree_attn_f32_kernel(TreeArgs a) {
     constexpr bool F32 = true;
-    typedef TreeT<F32> X;
-    typedef typename X::T T;
-    constexpr int RT = 2, W = 4, KG = D / 16, H = D / 64;
-    __shared__ __attribute__((aligned(16))) float oL[W][RT * 16][D];
+    constexpr int W = 4, KG = D / 16, H = D / 64;
+    __shared__ __attribute__((aligned(16))) float oL[W][RT * 16][D + 4];
     __shared__ float mL[W][RT * 16], lL[W][RT * 16];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
     // (splits slowest: neighbouring workgroups go to different XCDs, and where no row is cut only the first split has work)
     const int units = a.rows * a.hkv * a.row_blocks, split = blockIdx.x / units, rest = blockIdx.x % units;
     const int rb = rest % a.row_blocks, bh = rest / a.row_blocks, kvh = bh % a.hkv, b = bh / a.hkv;
+    typedef const int32_t __attribute__((address_space(4))) Entry;      // (nothing here writes the table: scalar loads)
+    Entry* bt = (Entry*)(uintptr_t)(a.block_table + (int64_t)b * a.bt_stride);
+    auto page_of = [&](int blk) { return bt[min((blk * kTreeBlock) >> a.page_shift, a.bt_cols - 1)]; };
+    int blk = split * W + wid, pg = page_of(blk);
     const int rounds = step_rounds(a);
     const TreeSpan s = tree_span(a, b);
     const int stacked = s.n * a.g, row0 = rb * RT * 16;
@@ -202,23 +206,38 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
     const int splits = row_splits(a, s.total, rounds);
     if (split >= splits) return;
 
+    const unsigned row_bytes = (unsigned)a.hkv * D * 4, k_at = r * row_bytes + 16 * q, v_at = 4 * q * row_bytes + 16 * r;
+    auto base_of = [&](const void* cache, int at, int page) {
+        const int64_t row = ((int64_t)(page >= 0 && page < a.num_pages ? page : 0) << a.page_shift) + ((at * kTreeBlock) & (a.page - 1));
+        return (const unsigned char*)cache + row * row_bytes + kvh * D * 4;
+    };
+    f32x4_t kf[KG], vf[4][H];
+    auto load_k = [&](int at, int page) {
+        const unsigned char* p = base_of(a.k_cache, at, page);
+#pragma unroll
+        for (int k = 0; k < KG; ++k) kf[k] = *reinterpret_cast<const f32x4_t*>(p + 64 * k + k_at);
+    };
+    auto load_v = [&](int at, int page) {
+        const unsigned char* p = base_of(a.v_cache, at, page);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int h = 0; h < H; ++h) vf[j][h] = *reinterpret_cast<const f32x4_t*>(p + j * row_bytes + 256 * h + v_at);
+    };
+    load_k(blk, pg);
+    load_v(blk, pg);
+
     f32x4_t qf[RT][KG];
-    uint64_t words[RT][kTreeMaxWords];
+    int node[RT];
+    uint64_t word0[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        const int sr = min(row0 + i * 16 + r, stacked - 1), node = sr / a.g;
-        const T* qp = (const T*)a.q + (int64_t)(s.start + node) * a.ldq + (int64_t)(kvh * a.g + sr % a.g) * D + 4 * q;
+        const int sr = min(row0 + i * 16 + r, stacked - 1);
+        node[i] = sr / a.g;
+        const float* qp = (const float*)a.q + (int64_t)(s.start + node[i]) * a.ldq + (int64_t)(kvh * a.g + sr % a.g) * D + 4 * q;
 #pragma unroll
-        for (int k = 0; k < KG; ++k) qf[i][k] = X::ld4(qp + 16 * k);
-#pragma unroll
-        for (int w = 0; w < kTreeMaxWords; ++w) {
-            if (a.mask) {
-                words[i][w] = w < a.words ? a.mask[(int64_t)(s.start + node) * a.words + w] : 0;
-            } else {
-                const int up = node + 1 - 64 * w;
-                words[i][w] = up >= 64 ? ~0ull : up > 0 ? (1ull << up) - 1 : 0;
-            }
-        }
+        for (int k = 0; k < KG; ++k) qf[i][k] = *reinterpret_cast<const f32x4_t*>(qp + 16 * k);
+        word0[i] = a.mask ? a.mask[(int64_t)(s.start + node[i]) * a.words] : 0;
     }
     f32x4_t acc[RT][H][4];
     float m[RT], l[RT];
@@ -231,24 +250,49 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[i][h][c] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
-    const int64_t stride = (int64_t)a.hkv * D;
     bool odd = false;
-    for (int blk = split * W + wid; blk < blocks; blk += splits * W) {
-        const int kb = blk * kTreeBlock, pg = a.block_table[(int64_t)b * a.bt_stride + (kb >> a.page_shift)];
-        if (pg < 0 || pg >= a.num_pages) continue;      // a place without a page: its keys do not count
-        const int64_t row = ((int64_t)pg << a.page_shift) + (kb & (a.page - 1));
-        const T* kp = (const T*)a.k_cache + (row + r) * stride + (int64_t)kvh * D + 4 * q;
-        const T* vp = (const T*)a.v_cache + (row + 4 * q) * stride + (int64_t)kvh * D + 4 * r;
-        f32x4_t kf[KG], vf[4][H];
+    while (blk < blocks) {
+        const int kb = blk * kTreeBlock, next = blk + splits * W, left = s.total - kb;
+        const uint32_t valid = pg < 0 || pg >= a.num_pages ? 0 : left < 16 ? (1u << left) - 1 : 0xffffu;
+        const bool open = valid == 0xffffu && kb + kTreeBlock <= s.ctx;      // every key there and visible to every row (uniform)
+        const int pn = next < blocks ? page_of(next) : -1;
+        f32x4_t sc[RT];
 #pragma unroll
-        for (int k = 0; k < KG; ++k) kf[k] = X::ld4(kp + 16 * k);
+        for (int i = 0; i < RT; ++i) sc[i] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int k = 0; k < KG; ++k)
 #pragma unroll
-            for (int h = 0; h < H; ++h) vf[j][h] = X::ld4(vp + j * stride + 64 * h);
-        const bool open = kb + kTreeBlock <= s.ctx;      // every key visible to every row (uniform)
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < RT; ++i) sc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[k][j], qf[i][k][j], sc[i], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (next < blocks) load_k(next, pn);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4_t p[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            if (!open) {
+                const uint32_t seen = visible_keys(a, s, node[i], word0[i], kb) & valid;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (!(seen >> (4 * q + j) & 1)) sc[i][j] = -__builtin_inff();
+            }
+            const float top = max_of_quarters(fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])) * a.scale_log2);
+            if (__builtin_amdgcn_ballot_w64(top > m[i] + kTreeRaise) != 0) {
+                const float mn = fmaxf(m[i], top), alpha = __builtin_amdgcn_exp2f(m[i] - mn);
+                m[i] = mn;
+                l[i] *= alpha;
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[i][h][c] *= alpha;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[i][j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], a.scale_log2, -m[i]));
+            l[i] += (p[i][0] + p[i][1]) + (p[i][2] + p[i][3]);
+        }
         // Where a row may not see a key, its weight is zero and the product would still hand on a value that is not finite: such
-        // values are left out here and added at the end (add_odd); behind the last key everything is left out.
+        // values are left out here and added at the end (add_odd); of keys that do not count everything is left out.
         if (!open) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -256,48 +300,27 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(TreeArgs a) {
                 for (int h = 0; h < H; ++h)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        if (kb + 4 * q + j >= s.total) vf[j][h][c] = 0.f;
-                        if (!(fabsf(vf[j][h][c]) <= 3.4028235e38f)) {
+                        if (!(valid >> (4 * q + j) & 1)) vf[j][h][c] = 0.f;
+                        if (is_odd(vf[j][h][c])) {
                             vf[j][h][c] = 0.f;
                             odd = true;
                         }
                     }
         }
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            if (row0 + i * 16 >= stacked) break;         // uniform
-            f32x4_t sc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < KG; ++k)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[k][j], qf[i][k][j], sc, 0, 0, 0);
-            uint32_t seen = 0xffff;
-            if (!open) {
-                seen = (uint32_t)mask_from(words[i], kb - s.ctx);
-                if (s.total - kb < 16) seen &= (1u << (s.total - kb)) - 1;
-                seen &= 0xffff;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (!(seen >> (4 * q + j) & 1)) sc[j] = -__builtin_inff();
-            }
-            float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])) * a.scale_log2;
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = fmaxf(m[i], top), alpha = __builtin_amdgcn_exp2f(m[i] - mn);
-            m[i] = mn;
-            f32x4_t p;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(sc[j], a.scale_log2, -mn));
-            l[i] = l[i] * alpha + ((p[0] + p[1]) + (p[2] + p[3]));
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int h = 0; h < H; ++h)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    acc[i][h][c] *= alpha;
+                for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][h][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[j][h][c], p[j], acc[i][h][c], 0, 0, 0);
-                }
-        }
+                    for (int i = 0; i < RT; ++i)
+                        acc[i][h][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[j][h][c], p[i][j], acc[i][h][c], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (next < blocks) load_v(next, pn);
+        __builtin_amdgcn_sched_barrier(0);
+        blk = next;
+        pg = pn;
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -413,21 +436,6 @@ __global__ __launch_bounds__(256, 2) void tree_attn_narrow_kernel(TreeArgs a) {
         for (int k = 0; k < KS; ++k) qf[i][k] = __builtin_bit_cast(bf16x8_t, ld16(qp + 32 * k));
         word0[i] = a.mask ? a.mask[(int64_t)(s.start + node[i]) * a.words] : 0;
     }
-    // what row i sees of the 32 keys from kb on
-    auto visible = [&](int i, int kb) -> uint32_t {
-        const int first = kb - s.ctx;
-        if (!a.mask) {
-            const int up = node[i] + 1 - first;
-            return up >= 32 ? ~0u : up > 0 ? (1u << up) - 1 : 0;
-        }
-        if (first < 0) return first <= -32 ? ~0u : (uint32_t)(word0[i] << -first) | ((1u << -first) - 1);
-        const int at = first >> 6, sh = first & 63;
-        const uint64_t* w = a.mask + (int64_t)(s.start + node[i]) * a.words;
-        uint64_t v = (at == 0 ? word0[i] : at < a.words ? w[at] : 0) >> sh;
-        if (sh > 32 && at + 1 < a.words) v |= w[at + 1] << (64 - sh);
-        return (uint32_t)v;
-    };
-
     f32x4_t acc[RT][DT];
     float m[RT], l[RT];
 #pragma unroll
@@ -480,7 +488,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_narrow_kernel(TreeArgs a) {
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             if (!open) {
-                const uint32_t seen = visible(i, kb) & valid;
+                const uint32_t seen = visible_keys(a, s, node[i], word0[i], kb) & valid;
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -1114,7 +1122,8 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a, int sh
 // form 6.9; 500 keys 6.9, 8.7, 11.6; 32 heads of 128 on 8, 64 nodes behind 300 keys 11.1, 12.3, -, 16.7).  Past `reach` (workgroups times keys) that
 // traffic is what they take: 4 rows of 4000 keys, 16 nodes, heads of 64 18.5, 15.5, 17.8, 17.1; heads of 128 45.6, 31.1, -, 24.3.  Then a workgroup
 // takes the rows it can: 64 of heads of 64 (32 rows of 4096 and 8 nodes 34.5, wide 36.9), 32 of heads of 128 (107; 64 in two groups of waves 183, wide 120),
-// and what is more goes to the wide form.
+// and what is more goes to the wide form.  fp32, whose blocks are bound by their matrix instructions, 16 or 32 rows by the same rule (one row of 4000, 24
+// nodes, 8 heads of 64 on 2 12.9, 14.8; 16 rows, 16 nodes, 16 on 4 54, 49).
 struct TreeForm {
     int row_tiles, row_part, row_blocks, round_keys, wide, slots, least;
 };
@@ -1126,7 +1135,7 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     };
     TreeForm f;
     f.wide = 0;
-    if (f32) f.row_tiles = 2;
+    if (f32) f.row_tiles = stacked <= 16 || fits(1, num_cus(), 400000) ? 1 : 2;
     else if (stacked <= 16 || fits(1, num_cus(), d == 64 ? 200000 : 50000)) f.row_tiles = 1;
     else if (stacked <= 32 || fits(2, d == 64 ? num_cus() : num_cus() / 2, d == 64 ? 300000 : 64000)) f.row_tiles = 2;
     else f.row_tiles = 4, f.wide = d == 128 || stacked > 64;
@@ -1135,7 +1144,7 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     f.round_keys = f.wide || f32 ? 64 : 128;
     // Work for one workgroup a unit, or for two where there are two without any cut (wide, us with one and two: 32 uneven rows of up to 8191, 64 nodes
     // of 8B heads 211, 205; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4)
-    const bool two = f.wide ? heads * f.row_blocks >= 2 * num_cus() : f32 && d == 64;
+    const bool two = f.wide ? heads * f.row_blocks >= 2 * num_cus() : f32 && (d == 64 || f.row_tiles == 1);
     f.slots = num_cus() * (two ? 2 : 1);
     f.least = f.wide ? 6 : 1;
     return f;
@@ -1220,8 +1229,10 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     hipStream_t s = (hipStream_t)stream;
     const dim3 g1((unsigned)grid);
 #define MV_TREE(K_) hipLaunchKernelGGL((K_), g1, dim3(256), 0, s, a)
-    if (f32 && d == 64) MV_TREE((tree_attn_f32_kernel<64>));
-    else if (f32) MV_TREE((tree_attn_f32_kernel<128>));
+    if (f32 && d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_f32_kernel<64, 1>));
+    else if (f32 && d == 64) MV_TREE((tree_attn_f32_kernel<64, 2>));
+    else if (f32 && f.row_tiles == 1) MV_TREE((tree_attn_f32_kernel<128, 1>));
+    else if (f32) MV_TREE((tree_attn_f32_kernel<128, 2>));
     else if (f.wide && d == 64) MV_TREE((tree_attn_wide_kernel<64, 1>));      // (64 rows of such heads: the narrow form)
     else if (f.wide && f.row_part == 64) MV_TREE((tree_attn_wide_kernel<128, 2>));
     else if (f.wide) MV_TREE((tree_attn_wide_kernel<128, 1>));
