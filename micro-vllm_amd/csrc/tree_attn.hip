@@ -1051,69 +1051,76 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
 // Splits added in order; rows that one split holds are written already.  A (node, head) is 2^shift groups of D / 4 lanes, each of which adds every
 // 2^shift-th split with all its requests out at once (64 splits in one group: 32 dependent trips, 17 us where this takes 3).
 template <bool F32, int D>
-__global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a, int shift) {
+__global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
     typedef TreeT<F32> X;
     constexpr int LPR = D / 4, GROUPS = 256 / LPR, MOST = 4;
     __shared__ float topL[GROUPS], denL[GROUPS];
     __shared__ f32x4_t oL[256];
-    const int b = blockIdx.y, group = threadIdx.x / LPR, part = group & ((1 << shift) - 1), c = threadIdx.x % LPR * 4;
+    const int b = blockIdx.y, group = threadIdx.x / LPR, c = threadIdx.x % LPR * 4;
+    const int rounds = step_rounds(a);
     const TreeSpan s = tree_span(a, b);
-    const int filled = row_splits(a, s.total, step_rounds(a));
-    if (filled <= 1 || (int64_t)blockIdx.x * (GROUPS >> shift) >= (int64_t)s.n * a.hq) return;
-    const int64_t item = (int64_t)blockIdx.x * (GROUPS >> shift) + (group >> shift), step = (int64_t)a.tokens * a.hq;
-    const int node = (int)min(item / a.hq, (int64_t)s.n - 1), head = (int)(item % a.hq);
-    const int64_t t = s.start + node, at = t * a.hq + head;
-    float top = kTreeNegBig, den = 0.f;
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int first = part; first < filled; first += MOST << shift) {
-        float m[MOST], l[MOST];
-        f32x4_t x[MOST];
+    const int filled = row_splits(a, s.total, rounds);
+    if (filled <= 1) return;
+    int shift = 0;
+    while ((MOST << shift) < filled && (1 << shift) < GROUPS) ++shift;
+    const int part = group & ((1 << shift) - 1), each = GROUPS >> shift, items = s.n * a.hq;
+    const int64_t step = (int64_t)a.tokens * a.hq;
+    for (int base = blockIdx.x * each; base < items; base += gridDim.x * each) {      // (the same trips for the whole workgroup)
+        const int item = base + (group >> shift), node = min(item / a.hq, s.n - 1), head = item % a.hq;
+        const int64_t t = s.start + node, at = t * a.hq + head;
+        float top = kTreeNegBig, den = 0.f;
+        f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+        for (int first = part; first < filled; first += MOST << shift) {
+            float m[MOST], l[MOST];
+            f32x4_t x[MOST];
 #pragma unroll
-        for (int i = 0; i < MOST; ++i) {
-            m[i] = -__builtin_inff();
-            if (first + (i << shift) >= filled) continue;
-            const int64_t from = at + (first + (i << shift)) * step;
-            m[i] = a.state[2 * from];
-            l[i] = a.state[2 * from + 1];
-            x[i] = *reinterpret_cast<const f32x4_t*>(a.part + from * D + c);
+            for (int i = 0; i < MOST; ++i) {
+                m[i] = -__builtin_inff();
+                if (first + (i << shift) >= filled) continue;
+                const int64_t from = at + (first + (i << shift)) * step;
+                m[i] = a.state[2 * from];
+                l[i] = a.state[2 * from + 1];
+                x[i] = *reinterpret_cast<const f32x4_t*>(a.part + from * D + c);
+            }
+            float up = top;
+#pragma unroll
+            for (int i = 0; i < MOST; ++i) up = fmaxf(up, m[i]);
+            const float f0 = __builtin_amdgcn_exp2f(top - up);
+            den *= f0;
+            o *= f0;
+            top = up;
+#pragma unroll
+            for (int i = 0; i < MOST; ++i) {
+                if (first + (i << shift) >= filled) break;
+                const float f = __builtin_amdgcn_exp2f(m[i] - top);
+                den = fmaf(l[i], f, den);
+                o += x[i] * f;
+            }
         }
-        float up = top;
-#pragma unroll
-        for (int i = 0; i < MOST; ++i) up = fmaxf(up, m[i]);
-        const float f0 = __builtin_amdgcn_exp2f(top - up);
-        den *= f0;
-        o *= f0;
-        top = up;
-#pragma unroll
-        for (int i = 0; i < MOST; ++i) {
-            if (first + (i << shift) >= filled) break;
-            const float f = __builtin_amdgcn_exp2f(m[i] - top);
-            den = fmaf(l[i], f, den);
-            o += x[i] * f;
+        if (shift > 0) {
+            if (c == 0) {
+                topL[group] = top;
+                denL[group] = den;
+            }
+            oL[threadIdx.x] = o;
+            __syncthreads();
+            float up = top;
+            for (int i = 1; i < 1 << shift; ++i) up = fmaxf(up, topL[min(group + i, GROUPS - 1)]);
+            const float f0 = __builtin_amdgcn_exp2f(top - up);
+            den *= f0;
+            o *= f0;
+            for (int i = 1; i < 1 << shift; ++i) {
+                const int from = min(group + i, GROUPS - 1);
+                const float f = __builtin_amdgcn_exp2f(topL[from] - up);
+                den = fmaf(denL[from], f, den);
+                o += oL[from * LPR + threadIdx.x % LPR] * f;
+            }
+            __syncthreads();      // (the next items' states go to the same places)
         }
+        if (part != 0 || item >= items) continue;
+        const float inv = den != 0.f ? 1.0f / den : 0.f;
+        X::st4((typename X::T*)a.out + t * a.ldo + (int64_t)head * D + c, o * inv);
     }
-    if (shift > 0) {
-        if (c == 0) {
-            topL[group] = top;
-            denL[group] = den;
-        }
-        oL[threadIdx.x] = o;
-        __syncthreads();
-        if (part != 0) return;
-        float up = top;
-        for (int i = 1; i < 1 << shift; ++i) up = fmaxf(up, topL[group + i]);
-        const float f0 = __builtin_amdgcn_exp2f(top - up);
-        den *= f0;
-        o *= f0;
-        for (int i = 1; i < 1 << shift; ++i) {
-            const float f = __builtin_amdgcn_exp2f(topL[group + i] - up);
-            den = fmaf(denL[group + i], f, den);
-            o += oL[threadIdx.x + i * LPR] * f;
-        }
-    }
-    if (item >= (int64_t)s.n * a.hq) return;
-    const float inv = den != 0.f ? 1.0f / den : 0.f;
-    X::st4((typename X::T*)a.out + t * a.ldo + (int64_t)head * D + c, o * inv);
 }
 
 // Which kernel a launch takes, with rows, workgroups and keys of its workgroups.
@@ -1245,12 +1252,14 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     if (num_splits > 1) {
         const int groups = 1024 / d;
         int shift = 0;
-        while ((4 << shift) < num_splits && (1 << shift) < groups) ++shift;
-        const dim3 g2((unsigned)(((int64_t)max_nodes * hq + (groups >> shift) - 1) / (groups >> shift)), (unsigned)rows);
-        if (f32 && d == 64) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 64>), g2, dim3(256), 0, s, a, shift);
-        else if (f32) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 128>), g2, dim3(256), 0, s, a, shift);
-        else if (d == 64) hipLaunchKernelGGL((tree_attn_merge_kernel<false, 64>), g2, dim3(256), 0, s, a, shift);
-        else hipLaunchKernelGGL((tree_attn_merge_kernel<false, 128>), g2, dim3(256), 0, s, a, shift);
+        while ((4 << shift) < num_splits && (1 << shift) < groups) ++shift;      // (as the kernel at most)
+        // (rows that are not cut leave at once, but a workgroup that leaves has asked for lengths too: no more of them than twice what the chip holds)
+        const int64_t most = ((int64_t)max_nodes * hq + (groups >> shift) - 1) / (groups >> shift), fair = (16 * num_cus() + rows - 1) / rows;
+        const dim3 g2((unsigned)(most < fair ? most : fair), (unsigned)rows);
+        if (f32 && d == 64) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 64>), g2, dim3(256), 0, s, a);
+        else if (f32) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 128>), g2, dim3(256), 0, s, a);
+        else if (d == 64) hipLaunchKernelGGL((tree_attn_merge_kernel<false, 64>), g2, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((tree_attn_merge_kernel<false, 128>), g2, dim3(256), 0, s, a);
     }
     return check_launch();
 }
