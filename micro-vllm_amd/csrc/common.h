@@ -109,6 +109,15 @@ inline int check_launch() {
     return MV_OK;
 }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Whether `rows` rows of wa bytes, lda bytes apart from a on, share memory with rows of wb bytes, ldb apart from b on (lda >= wa, ldb >= wb).  Rows
+// of one stride may lie in between each other; of two strides, none may begin before the others' last ends.
+inline bool rows_meet(const void* a, int64_t lda, int64_t wa, const void* b, int64_t ldb, int64_t wb, int64_t rows) {
+    const int64_t at = (int64_t)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));
+    if (rows <= 0 || at >= (rows - 1) * lda + wa || at + (rows - 1) * ldb + wb <= 0) return false;
+    if (rows == 1 || lda != ldb) return true;
+    const int64_t in = (at % lda + lda) % lda;
+    return in < wa || in + wb > lda;
+}
 int num_cus();  // compute units of the current device (cached)
 // Opt a kernel in to `lds` bytes of dynamic LDS (needed past 64 KiB) on the current device.
 // `done` is the caller's per-kernel record of what each device was last configured for.

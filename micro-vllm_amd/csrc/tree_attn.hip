@@ -2,15 +2,16 @@
 // the nodes whose bits its mask has, o = sum_j softmax_j(q . k_j scale) v_j.  The nodes' own keys and values are in the cache already.
 //
 // The g query heads that share a key/value head are stacked: stacked row r = node * g + head, so every key read serves n * g rows.
-// Workgroup = (row, key/value head, run of stacked rows, split of the keys).  Waves take 16-key blocks of the split in turn and
-// keep a softmax state each; the states meet in LDS, the splits' in a second launch that adds them in order.
+// Workgroup = (row, key/value head, run of stacked rows, split of the keys), one pass over the keys with a softmax state per stacked row.
+// Three forms: fp32 and bf16 with few rows, where every wave takes blocks of keys of its own and the states meet in LDS at the end, and bf16 with many
+// rows, where the waves share the keys.  The splits' states are added in order by a second launch.
 #include "common.h"
 
 #include <type_traits>
 
 namespace mv {
 
-constexpr float kTreeNegBig = -1.0e30f;        // a running maximum before any visible key
+constexpr float kTreeNegBig = -3.4028235e38f;  // a running maximum before any visible key: below any score
 // A row's running maximum is raised only when a score outgrows it by this many powers of two: weights are then up to 2^6 instead of up to
 // one, the sums have 32 bits for that, and a weight's rounding to bf16 is relative.  With the exact maximum some row of a wave outgrows its own
 // in most blocks, and every accumulator is multiplied for it.
@@ -646,9 +647,9 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
         }
         return r;
     };
-    auto counted = [&](int t, const Pages& g) __attribute__((always_inline)) {      // keys of a tile that count
-        const int left = s.total - min(t, t1 - 1) * KT;
-        return left < KT ? g.there & ((1ull << left) - 1) : g.there;
+    auto counted = [&](int t, const Pages& g) __attribute__((always_inline)) {      // keys of a tile that count (the last splits may have no tile)
+        const int left = s.total - t * KT;
+        return left < KT ? g.there & ((1ull << max(left, 0)) - 1) : g.there;
     };
     const unsigned row_bytes = (unsigned)a.hkv * RB;
     auto base_of = [&](int t, const Pages& g) __attribute__((always_inline)) {      // byte offset in either cache of the wave's first row
@@ -1189,6 +1190,7 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
         return MV_ERR_INVALID_ARG;
     if ((d != 64 && d != 128) || hq / hkv > 8 || (page & (page - 1)) || page < kTreeBlock || max_nodes > kTreeMaxNodes || num_splits > kTreeMaxSplits)
         return MV_ERR_UNSUPPORTED;
+    if (((int64_t)bt_cols << __builtin_ctz((unsigned)page)) > (1 << 30)) return MV_ERR_UNSUPPORTED;      // (an index of a key, and what is added to it, has 32 bits)
     if (rows == 0 || tokens == 0 || max_nodes == 0) return MV_OK;
     if (!q || !k_cache || !v_cache || !ctx_lens || !row_start || !block_table || !out) return MV_ERR_INVALID_ARG;
     if (mask && (words < 1 || words > kTreeMaxWords || words * 64 < max_nodes)) return MV_ERR_INVALID_ARG;
@@ -1198,6 +1200,8 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
         return MV_ERR_INVALID_ARG;
     if (num_splits > 1 && (!workspace || !aligned16(workspace) || workspace_bytes < mv_tree_attn_workspace_bytes(tokens, hq, d, num_splits)))
         return MV_ERR_WORKSPACE;
+    const int64_t bytes = f32 ? 4 : 2;
+    if (rows_meet(q, ldq * bytes, hq * d * bytes, out, ldo * bytes, hq * d * bytes, tokens)) return MV_ERR_INVALID_ARG;
     TreeArgs a;
     a.q = q;
     a.k_cache = k_cache;

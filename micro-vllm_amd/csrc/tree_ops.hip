@@ -477,6 +477,10 @@ int mv_qkv_norm_rotary_slots(const void* qkv, int64_t ld, const float* q_norm, c
     if (!qkv || !positions || !slots || !q_out || !k_cache || !v_cache || (rot > 0 && !inv_freq) ||
         ld < (int64_t)(heads + 2 * kv_heads) * d || ldq < (int64_t)heads * d)
         return MV_ERR_INVALID_ARG;
+    const int64_t sb = src_f32 ? 4 : 2, db = dst_f32 ? 4 : 2;      // q over its own part of the rows, or nowhere in them
+    if (!(q_out == qkv && ld * sb == ldq * db && sb == db) &&
+        rows_meet(qkv, ld * sb, (int64_t)(heads + 2 * kv_heads) * d * sb, q_out, ldq * db, (int64_t)heads * d * db, tokens))
+        return MV_ERR_INVALID_ARG;
     SlotStoreArgs a{qkv, ld, q_norm, k_norm, eps, inv_freq, rot, adjacent, positions, slots, q_out, ldq, k_cache, v_cache, tokens, heads,
                     kv_heads, d, cache_slots};
     hipStream_t s = (hipStream_t)stream;

@@ -177,7 +177,12 @@ def test_norm_rotary_slots_in_place(ops, dtype, d, rot, adjacent):
 
 
 # ------------------------------------------------------------------------------------------------------------- attention
-def run_attn(ops, case, splits=0, mask="case", max_nodes=None, hq_stride=0):
+# Which kernel a launch takes goes by its rows and by the keys that its table has room for: behind this many columns more every launch takes the form
+# for much work (bf16: 16, 32 or (heads of 64) 64 stacked rows a workgroup, past 64 (heads of 128: 32) keys shared by the waves; fp32: 32 rows).
+MUCH = 26000
+
+
+def run_attn(ops, case, splits=0, mask="case", max_nodes=None, hq_stride=0, cols=0):
     T, hq, d = case.q.shape
     buf = torch.full((T, hq * d + hq_stride), 7.0, dtype=case.dtype, device=DEV)
     out = buf[:, :hq * d].unflatten(1, (hq, d))
@@ -188,8 +193,9 @@ def run_attn(ops, case, splits=0, mask="case", max_nodes=None, hq_stride=0):
     else:
         q = case.q.to(DEV)
     m = None if mask is None else case.mask().to(DEV)
-    ops.tree_attn(q, case.k.to(DEV), case.v.to(DEV), i32(case.ctx, DEV), i32(case.starts, DEV), i32(case.table, DEV), m,
-                  max_nodes or case.max_nodes, out=out, num_splits=splits)
+    table = torch.nn.functional.pad(i32(case.table, DEV), (0, cols), value=-1)
+    ops.tree_attn(q, case.k.to(DEV), case.v.to(DEV), i32(case.ctx, DEV), i32(case.starts, DEV), table, m, max_nodes or case.max_nodes, out=out,
+                  num_splits=splits)
     assert (out[case.T:] == 7.0).all(), "tokens behind the last row"
     assert hq_stride == 0 or (buf[:, hq * d:] == 7.0).all()
     return out
@@ -203,7 +209,8 @@ def test_attention_of_trees(ops, dtype, hq, hkv, d, page, ctx, counts):
     case = AttnCase(ctx, counts, hq, hkv, d, page, dtype, seed=hq * 1000 + d + page + sum(ctx), forest=True)
     want = case.reference()
     for splits in (0, 1, 3, 64):
-        case.check(run_attn(ops, case, splits), f"splits {splits}", want)
+        for cols in (0, MUCH):
+            case.check(run_attn(ops, case, splits, cols=cols), f"splits {splits} columns {cols}", want)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -211,17 +218,71 @@ def test_attention_of_the_largest_trees(ops, dtype):
     case = AttnCase([200, 3], [256, 250], 8, 1, 128 if dtype == BF16 else 64, 64, dtype, seed=9)
     want = case.reference()
     for splits in (0, 1, 2):
-        case.check(run_attn(ops, case, splits), f"splits {splits}", want)
+        for cols in (0, MUCH):
+            case.check(run_attn(ops, case, splits, cols=cols), f"splits {splits} columns {cols}", want)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("d", [64, 128])
-def test_attention_of_a_chain_is_the_causal_one(ops, dtype, d):
-    case = AttnCase([100, 0, 37], [30, 64, 1], 4, 2, d, 16, dtype, seed=2)
+@pytest.mark.parametrize("hq", [2, 4, 12])
+def test_attention_of_a_chain_is_the_causal_one(ops, dtype, d, hq):
+    case = AttnCase([100, 0, 37], [30, 64, 1], hq, 2, d, 16, dtype, seed=2)
     case.seen = [set(range(i + 1)) for n in case.counts for i in range(n)]
-    a, b = run_attn(ops, case, mask=None), run_attn(ops, case)
-    assert torch.equal(a, b)
-    case.check(a, "chain")
+    want = case.reference()
+    for cols in (0, MUCH):
+        a, b = run_attn(ops, case, mask=None, cols=cols), run_attn(ops, case, cols=cols)
+        assert torch.equal(a, b)
+        case.check(a, "chain", want)
+
+
+@pytest.mark.parametrize("hq,n,d", [(8, 8, 128), (8, 17, 128), (8, 17, 64), (8, 2, 64), (8, 4, 64), (8, 8, 64), (8, 4, 128)])
+@pytest.mark.parametrize("ctx", [700, 1500, 3136])
+def test_splits_that_keys_do_not_fill(ops, hq, n, d, ctx):
+    """Numbers of splits that leave the last of them short, or without any key, and masks with bits of nodes that a row does not have."""
+    case = AttnCase([ctx - n, 40], [n, 1], hq, 1, d, 64, BF16, seed=ctx + n)
+    want, seen = case.reference(), case.seen
+    case.seen = [s | set(range(n if t < n else 1, 64)) for t, s in enumerate(seen)]
+    for splits in (2, 3, 4, 7, 8, 30):
+        for cols in (0, MUCH):
+            case.check(run_attn(ops, case, splits, cols=cols), f"splits {splits} columns {cols}", want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_of_many_rows(ops, dtype):
+    """More rows than a wave has lanes, more than the joining launch has workgroups for one each; some without nodes."""
+    rng = np.random.default_rng(4)
+    ctx, counts = rng.integers(0, 40, 700).tolist(), rng.integers(0, 3, 700).tolist()
+    ctx[300], counts[300] = 2000, 5
+    case = AttnCase(ctx, counts, 2, 1, 64, 16, dtype, seed=4)
+    want = case.reference()
+    for splits in (0, 1, 4):
+        for cols in (0, MUCH):
+            case.check(run_attn(ops, case, splits, cols=cols), f"splits {splits} columns {cols}", want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_nodes_past_the_bound_are_left_alone(ops, dtype):
+    case = AttnCase([50, 20], [40, 6], 4, 1, 64, 16, dtype, seed=15)
+    want = [t.clone() for t in case.reference()]
+    for cols in (0, MUCH):
+        for splits in (1, 2):
+            out = run_attn(ops, case, splits, max_nodes=10, cols=cols)
+            assert (out[10:40] == 7.0).all()
+            keep = torch.ones(case.T, dtype=torch.bool)
+            keep[10:40] = False
+            o, mag, size, count = (t[keep] for t in want)
+            err = (out[:case.T].double().cpu()[keep] - o).abs()
+            assert (err <= ref.attn_bound(o, mag, size, count, 64, dtype)).all()
+    plan = ops.TreePlan.empty(2, case.T, 10, DEV)
+    for t in plan:
+        t.fill_(-5)
+    ops.tree_plan(i32(case.ctx, DEV), i32(case.starts, DEV), i32(case.table, DEV), i32(list(range(90)), DEV), 10, 16, 100, parents=case.parents.to(DEV),
+                  out=plan)
+    assert all((t[10:40] == -5).all() and (t[:10] != -5).all() and (t[40:] != -5).all() for t in (plan.slots, plan.positions, plan.rows))
+    assert (plan.mask[10:40] == -5).all() and plan.taken.tolist() == [0, 0]
+    tokens = torch.zeros(case.T, dtype=torch.int64, device=DEV)
+    got = ops.tree_accept(tokens, tokens, i32(case.starts, DEV), i32(case.ctx, DEV), 10)
+    assert got.counts.tolist() == [10, 6] and got.lens.tolist() == [60, 26]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -236,14 +297,16 @@ def test_masks_that_are_no_trees(ops, dtype, d):
     case.seen[5], case.seen[case.starts[1] + 3], case.seen[case.starts[2]] = set(), set(), set()
     want = case.reference()
     for splits in (0, 1, 5):
-        out = run_attn(ops, case, splits, hq_stride=16)
-        case.check(out, f"splits {splits}", want)
-        assert (out[5] == 0).all() and (out[case.starts[2]] == 0).all()
+        for cols in (0, MUCH):
+            out = run_attn(ops, case, splits, hq_stride=16, cols=cols)
+            case.check(out, f"splits {splits} columns {cols}", want)
+            assert (out[5] == 0).all() and (out[case.starts[2]] == 0).all()
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("d,hq,hkv", [(128, 4, 1), (64, 4, 4), (128, 16, 2)])
-def test_what_is_masked_may_be_infinite_or_nan(ops, dtype, d, hq, hkv):
+@pytest.mark.parametrize("d,hq,hkv", [(128, 4, 1), (64, 4, 4), (128, 16, 2), (64, 8, 1), (128, 1, 1), (64, 2, 1)])
+@pytest.mark.parametrize("cols", [0, MUCH])
+def test_what_is_masked_may_be_infinite_or_nan(ops, dtype, d, hq, hkv, cols):
     """Keys and values of nodes that are not seen, of places behind the last node and of pages that are nobody's hold NaN and infinities:
     nodes that see none of it get what they get without it; those that see an infinite value get it in that entry alone."""
     for n, ctx in ((20, 37), (64, 64), (33, 0)):
@@ -263,13 +326,13 @@ def test_what_is_masked_may_be_infinite_or_nan(ops, dtype, d, hq, hkv):
             p, s = where(i)
             case.k[p, s], case.v[p, s] = [float("inf"), float("nan"), -float("inf")][i % 3], [float("nan"), float("inf")][i % 2]
         for splits in (0, 1, 2):
-            out = run_attn(ops, case, splits)
+            out = run_attn(ops, case, splits, cols=cols)
             case.check(out, f"n {n} splits {splits}", clean)
         # one finite key with one infinite entry of its value: nodes that see it get the infinity there and nothing else changes
         p, s = where(2)
         case.v[p, s, :, 5] = float("inf")
         case.v[p, s, :, d - 1] = -float("inf")
-        out = run_attn(ops, case).double().cpu()[:n]
+        out = run_attn(ops, case, cols=cols).double().cpu()[:n]
         sees = torch.tensor([2 in z for z in case.seen])
         assert (out[sees][:, :, 5] == float("inf")).all() and (out[sees][:, :, d - 1] == -float("inf")).all()
         keep = torch.ones(d, dtype=torch.bool)
@@ -280,37 +343,68 @@ def test_what_is_masked_may_be_infinite_or_nan(ops, dtype, d, hq, hkv):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_places_without_a_page_do_not_count(ops, dtype):
-    case = AttnCase([100, 90, 40], [20, 40, 8], 4, 2, 64, 16, dtype, seed=6)
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (2, 2, 64), (8, 1, 64), (3, 3, 128), (4, 4, 128), (2, 1, 128), (8, 1, 128)])
+@pytest.mark.parametrize("cols", [0, MUCH])
+def test_places_without_a_page_do_not_count(ops, dtype, hq, hkv, d, cols):
+    case = AttnCase([100, 90, 40], [20, 40, 8], hq, hkv, d, 16, dtype, seed=6)
     case.table[0][2] = -1                                  # among the cached tokens
     case.table[1][(90 + 16) // 16] = case.pages + 5         # among the nodes
     case.table[2] = [-1] * len(case.table[2])               # a row without any page: zeros
     want = case.reference()
     for splits in (0, 1, 4):
-        out = run_attn(ops, case, splits)
+        out = run_attn(ops, case, splits, cols=cols)
         case.check(out, f"splits {splits}", want)
         assert (out[case.starts[2]:case.T] == 0).all()
-    narrow = AttnCase([100], [20], 4, 2, 64, 16, dtype, seed=6)
+    narrow = AttnCase([100], [20], hq, hkv, d, 16, dtype, seed=6)
     narrow.table = [narrow.table[0][:7]]                    # no column for the last nodes: their keys do not count
-    narrow.check(run_attn(ops, narrow), "narrow table")
+    narrow.check(run_attn(ops, narrow, cols=cols), "narrow table")
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_scores_of_any_size(ops, dtype):
     """Scores of hundreds on either side of zero, and one key that outweighs all others wherever it lies."""
-    for hq, hkv in ((4, 2), (8, 1)):
-        case = AttnCase([130], [24], hq, hkv, 64, 64, dtype, seed=11, scale_q=30.0)
-        case.check(run_attn(ops, case), "large scores")
+    for hq, hkv, d in ((4, 2, 64), (8, 1, 64), (2, 1, 128), (8, 1, 128)):
+        case = AttnCase([130], [24], hq, hkv, d, 64, dtype, seed=11, scale_q=30.0)
+        want = case.reference()
+        for cols in (0, MUCH):
+            case.check(run_attn(ops, case, cols=cols), f"large scores, columns {cols}", want)
         for at in (0, 15, 16, 63, 64, 129, 131):
-            case = AttnCase([130], [24], hq, hkv, 64, 64, dtype, seed=12)
+            case = AttnCase([130], [24], hq, hkv, d, 64, dtype, seed=12)
             p, s = case.table[0][at // 64], at % 64
             case.k[p, s] = case.q[5, ::hq // hkv].to(F32).to(dtype) * 4
+            want = case.reference()
             for splits in (1, 3):
-                case.check(run_attn(ops, case, splits), f"key {at}")
+                for cols in (0, MUCH):
+                    case.check(run_attn(ops, case, splits, cols=cols), f"key {at} columns {cols}", want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hq", [1, 2, 8])
+@pytest.mark.parametrize("d", [64, 128])
+def test_scores_of_minus_two_million(ops, dtype, hq, d):
+    """Every key that a row sees has a score of -2^21, -2^22 or -2^23 (products of powers of two, exact in any order): those of -2^21 share the weight."""
+    case = AttnCase([90], [24], hq, 1, d, 16, dtype, seed=16)
+    case.q.zero_()
+    case.q[:, :, 3] = 2.0 ** 10
+    case.k.zero_()
+    for j in range(114):
+        case.k[case.table[0][j // 16], j % 16, :, 3] = -(2.0 ** (12 + j % 3))
+    want = torch.zeros(24, hq, d, dtype=torch.float64)
+    for t in range(24):
+        best = [j for j in range(0, 114, 3) if j < 90 or j - 90 in case.seen[t]]
+        want[t] = torch.stack([case.v[case.table[0][j // 16], j % 16, 0].double() for j in best]).mean(0)
+    # equal weights: sums of up to 38 values and of as many weights, a division, a rounding of each; bf16: the weight's rounding and the output's
+    tol = (100 * 2.0 ** -24 + (2.02 * 2.0 ** -8 if dtype == BF16 else 0)) * case.v.abs().max().item()
+    for splits in (1, 3):
+        for cols in (0, MUCH):
+            table = torch.nn.functional.pad(i32(case.table, DEV), (0, cols), value=-1)
+            out = ops.tree_attn(case.q.to(DEV), case.k.to(DEV), case.v.to(DEV), i32(case.ctx, DEV), i32(case.starts, DEV), table, case.mask().to(DEV), 24,
+                                softmax_scale=0.5, num_splits=splits)
+            assert ((out[:24].double().cpu() - want).abs() <= tol).all()
 
 
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("hq,hkv", [(4, 2), (8, 1)])
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 2), (8, 1)])
 @pytest.mark.parametrize("step", [-1.0, 1.0])
 def test_scores_that_rise_or_fall_along_the_keys(ops, d, hq, hkv, step):
     """Scores that climb (fall) by one per key, over hundreds: no key of the first block says anything about the last ones', and nothing before
@@ -322,21 +416,27 @@ def test_scores_that_rise_or_fall_along_the_keys(ops, d, hq, hkv, step):
         for j in range(c + n):
             p, s = case.table[b][j // 64], j % 64
             case.k[p, s, :, 0] = step * j
+    want = case.reference()
     for splits in (0, 1, 2):
-        case.check(run_attn(ops, case, splits), f"splits {splits}")
+        for cols in (0, MUCH):
+            case.check(run_attn(ops, case, splits, cols=cols), f"splits {splits} columns {cols}", want)
 
 
-def test_values_near_the_end_of_the_range(ops):
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq", [1, 2, 8])
+@pytest.mark.parametrize("cols", [0, MUCH])
+def test_values_near_the_end_of_the_range(ops, d, hq, cols):
     """Values of 2^100 and scores 30 above those of the first keys: no sum may overflow on the way."""
-    case = AttnCase([400], [24], 8, 1, 64, 64, BF16, seed=14)
+    case = AttnCase([400], [24], hq, 1, d, 64, BF16, seed=14)
     case.v.mul_(2.0 ** 100)
     for j in (200, 390, 405):
         p, s = case.table[0][j // 64], j % 64
-        case.k[p, s] = case.q[7, ::8].to(F32).to(BF16) * 4
+        case.k[p, s] = case.q[7, ::hq].to(F32).to(BF16) * 4
+    want = case.reference()
     for splits in (0, 1, 2):
-        out = run_attn(ops, case, splits)
+        out = run_attn(ops, case, splits, cols=cols)
         assert torch.isfinite(out[:case.T].float()).all()
-        case.check(out, f"splits {splits}")
+        case.check(out, f"splits {splits}", want)
 
 
 def test_a_long_cache_past_32_bit_offsets(ops):

@@ -7,6 +7,7 @@ from oracle import ref_tree as ref
 from tree_util import AttnCase
 
 NULL, P = None, 1 << 20      # an address that is 16-byte aligned; nothing may follow it
+FAR = 1 << 30                # another
 
 
 @pytest.fixture(scope="module")
@@ -34,7 +35,7 @@ def test_plan_refuses(nv):
     assert plan(nv, rows=0, ctx=NULL, bt=NULL) == nv.MV_OK
 
 
-def store(nv, qkv=P, ld=1024, qn=P, kn=P, freq=P, rot=64, pos=P, slots=P, out=P, ldq=512, k=P, v=P, n=100, tokens=3, hq=8, hkv=4, d=64, src=0, dst=0):
+def store(nv, qkv=P, ld=1024, qn=P, kn=P, freq=P, rot=64, pos=P, slots=P, out=FAR, ldq=512, k=P, v=P, n=100, tokens=3, hq=8, hkv=4, d=64, src=0, dst=0):
     return nv.lib().mv_qkv_norm_rotary_slots(qkv, ld, qn, kn, 1e-6, freq, rot, 0, pos, slots, out, ldq, k, v, n, tokens, hq, hkv, d, src, dst, NULL)
 
 
@@ -44,10 +45,14 @@ def test_store_refuses(nv):
     for b in bad:
         assert store(nv, **b) == nv.MV_ERR_INVALID_ARG, b
     assert store(nv, dst=1) == nv.MV_ERR_UNSUPPORTED
+    # q over anything of the rows but its own part, or over that in another type or with another stride
+    for b in (dict(out=P + 512 * 2, ldq=1024), dict(out=P + 16, ldq=1024), dict(out=P, ldq=512), dict(out=P, ldq=1024, src=1), dict(out=P - 16, ldq=1024),
+              dict(out=P + 2 * 1024 * 2 + 1023 * 2, ldq=600), dict(out=P + 1000 * 2, ldq=1100, ld=1100), dict(tokens=1, out=P - 1022)):
+        assert store(nv, **b) == nv.MV_ERR_INVALID_ARG, b
     assert store(nv, tokens=0, qkv=NULL) == nv.MV_OK
 
 
-def attn(nv, q=P, ldq=512, k=P, v=P, ctx=P, starts=P, bt=P, stride=8, cols=8, mask=P, words=1, out=P, ldo=512, ws=NULL, ws_bytes=0, rows=2, tokens=9,
+def attn(nv, q=P, ldq=512, k=P, v=P, ctx=P, starts=P, bt=P, stride=8, cols=8, mask=P, words=1, out=FAR, ldo=512, ws=NULL, ws_bytes=0, rows=2, tokens=9,
          nodes=8, hq=8, hkv=4, d=64, page=16, pages=20, scale=0.1, splits=1, f32=0):
     return nv.lib().mv_tree_attn(q, ldq, k, v, ctx, starts, bt, stride, cols, mask, words, out, ldo, ws, ws_bytes, rows, tokens, nodes, hq, hkv, d,
                                  page, pages, scale, splits, f32, NULL)
@@ -60,8 +65,11 @@ def test_attention_refuses(nv):
            dict(scale=float("nan")), dict(scale=float("inf")), dict(words=0), dict(words=5), dict(nodes=65)]
     for b in bad:
         assert attn(nv, **b) == nv.MV_ERR_INVALID_ARG, b
-    for b in (dict(d=96, hq=4, ldq=384, ldo=384), dict(hq=36, ldq=4096, ldo=4096), dict(page=48), dict(page=8), dict(nodes=257, words=4), dict(splits=65)):
+    for b in (dict(d=96, hq=4, ldq=384, ldo=384), dict(hq=36, ldq=4096, ldo=4096), dict(page=48), dict(page=8), dict(nodes=257, words=4), dict(splits=65),
+              dict(cols=(1 << 26) + 1, stride=1 << 27)):      # (the last: keys past 2^30)
         assert attn(nv, **b) == nv.MV_ERR_UNSUPPORTED, b
+    for b in (dict(out=P), dict(out=P + 16), dict(out=P, ldo=1024), dict(out=P + 256, ldq=640, ldo=640), dict(tokens=1, out=P - 1008)):
+        assert attn(nv, **b) == nv.MV_ERR_INVALID_ARG, b          # out over q
     assert attn(nv, splits=2) == nv.MV_ERR_WORKSPACE
     need = nv.lib().mv_tree_attn_workspace_bytes(9, 8, 64, 2)
     assert need >= 2 * 9 * 8 * 66 * 4
