@@ -599,11 +599,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     unsigned char *const kring = ring, *const vring = ring + (KD + 1) * TB;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lq = lane & 31, hi = lane >> 5;
 
-    // parts of the same rows' keys eight workgroups apart, on one XCD: what one asks for the others find in its L2
-    const int units = a.rows * a.hkv, each = (units + 7) / 8 * 8 * a.row_blocks, split = blockIdx.x / each, within = blockIdx.x % each;
-    const int unit = within / (8 * a.row_blocks) * 8 + within % 8, rb = within / 8 % a.row_blocks;
-    if (unit >= units) return;
-    const int kvh = unit % a.hkv, b = unit / a.hkv;
+    // parts of the same keys' stacked rows eight workgroups apart, on one XCD: what one asks for the others find in its L2
+    const int units = a.rows * a.hkv, place = blockIdx.x / (8 * a.row_blocks) * 8 + blockIdx.x % 8, rb = blockIdx.x / 8 % a.row_blocks;
+    const int split = place / units, unit = place % units, kvh = unit % a.hkv, b = unit / a.hkv;
+    if (split >= a.nsplit) return;
     const int rounds = step_rounds(a);
     const TreeSpan s = tree_span(a, b);
     // a row's stacked rows in as few parts as 128 (64) allow, of even size
@@ -1125,13 +1124,16 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
 }
 
 // Which kernel a launch takes, with rows, workgroups and keys of its workgroups.
-// Where few workgroups have short rows, latency counts: a workgroup of 16 rows is the quickest through its keys, and as many of them as the chip has
-// units ask for the same keys again out of L2 (us, rows 1, 32 heads of 64 on 4, 7 nodes behind 45 keys: 16 rows a workgroup 5.1, 32 6.2, 64 8.1, the wide
-// form 6.9; 500 keys 6.9, 8.7, 11.6; 32 heads of 128 on 8, 64 nodes behind 300 keys 11.1, 12.3, -, 16.7).  Past `reach` (workgroups times keys) that
-// traffic is what they take: 4 rows of 4000 keys, 16 nodes, heads of 64 18.5, 15.5, 17.8, 17.1; heads of 128 45.6, 31.1, -, 24.3.  Then a workgroup
-// takes the rows it can: 64 of heads of 64 (32 rows of 4096 and 8 nodes 34.5, wide 36.9), 32 of heads of 128 (107; 64 in two groups of waves 183, wide 120),
-// and what is more goes to the wide form.  fp32, whose blocks are bound by their matrix instructions, 16 or 32 rows by the same rule (one row of 4000, 24
-// nodes, 8 heads of 64 on 2 12.9, 14.8; 16 rows, 16 nodes, 16 on 4 54, 49).
+// Where few workgroups have short rows, latency counts: a workgroup of 16 stacked rows is the quickest through its keys, and as many of them as the chip
+// has units ask for the same keys again out of L2.  Past `reach` (workgroups times keys) that traffic is what they take, and a workgroup takes more rows:
+// 32, then 64 (heads of 64), then the wide form.  In us, 16 rows a workgroup, 32, wide, each with the splits that it gets:
+//   32 heads of 64 on 4     1 row of 900, 64 nodes 9.5, 12.0, 20.3; 4 rows of 1200, 32 nodes 12.5, 14.7, 23.0; 1 row of 5000, 64 nodes 22.8, 20.2, 24.5;
+//                           4 rows of 5000, 16 nodes 31, 22, 21; 64 nodes 55, 43, 34
+//   32 heads of 128 on 8    1 row of 900, 16 nodes 13.9, 15.1, 17.3; 2500 18.6, 16.0, 17.8; 64 nodes 26.8, 26.5, 22.9; 4 rows of 1200, 32 nodes 30, 22, 25;
+//                           2500 57, 36, 26; 8 rows of 16000, 64 nodes 868, 595, 196
+// Where every other form has passed its reach: 64 rows a workgroup for heads of 64 (32 rows of 4096, 8 nodes 34.5, wide 36.9), else wide; 32 rows of heads of
+// 128 in the narrow form (107, wide 120).  fp32, whose blocks are bound by their matrix instructions, 16 or 32 rows by the same rule (one row of 4000,
+// 24 nodes, 8 heads of 64 on 2 12.9, 14.8; 16 rows, 16 nodes, 16 on 4 54, 49).
 struct TreeForm {
     int row_tiles, row_part, row_blocks, round_keys, wide, slots, least;
 };
@@ -1143,9 +1145,10 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     };
     TreeForm f;
     f.wide = 0;
+    const bool few = max_keys <= 1536;
     if (f32) f.row_tiles = stacked <= 16 || fits(1, num_cus(), 400000) ? 1 : 2;
-    else if (stacked <= 16 || fits(1, num_cus(), d == 64 ? 200000 : 50000)) f.row_tiles = 1;
-    else if (stacked <= 32 || fits(2, d == 64 ? num_cus() : num_cus() / 2, d == 64 ? 300000 : 64000)) f.row_tiles = 2;
+    else if (stacked <= 16 || fits(1, num_cus(), d == 64 ? few ? 400000 : 200000 : 50000)) f.row_tiles = 1;
+    else if (stacked <= 32 || fits(2, d == 64 ? num_cus() : num_cus() / 2, d == 64 ? few ? 400000 : 300000 : few ? 200000 : 90000)) f.row_tiles = 2;
     else f.row_tiles = 4, f.wide = d == 128 || stacked > 64;
     f.row_part = f.wide ? (stacked <= 64 ? 64 : 128) : 16 * f.row_tiles;
     f.row_blocks = (int)((stacked + f.row_part - 1) / f.row_part);
@@ -1171,11 +1174,15 @@ int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, in
     using namespace mv;
     if (rows <= 0 || max_nodes <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || max_keys <= 0) return 1;
     const TreeForm f = tree_form(rows, max_nodes, hkv, hq / hkv, d, f32, max_keys);
-    // the launch that joins the splits costs some 3 us, a round of a workgroup 0.5 (heads of 64) to 1.2 (of 128): short rows are not cut
-    if (max_keys <= (f32 ? 384 : d == 64 ? 1152 : 512)) return 1;
+    // the launch that joins the splits costs some 3 us, a round of a workgroup 0.5 (heads of 64) to 1.2 (of 128): short rows are not cut (heads of 64,
+    // one row of 1200, 64 nodes whole 10.7, cut 12.5, of 2500 17.3, 16.0; heads of 128 of 600 14.4, 15.8, of 1200, 16 nodes 18.3, 14.4)
+    if (max_keys <= (f32 ? 384 : d == 64 ? 1536 : 1024)) return 1;
     // (as many as the kernels may want: they cut a row in fewer where its keys or the step's rows do not ask for them)
     const int64_t units = (int64_t)rows * hkv * f.row_blocks, most = ((int64_t)max_keys + f.round_keys * f.least - 1) / (f.round_keys * f.least);
-    int64_t splits = units < f.slots ? (f.slots + units - 1) / units * (rows > 1 ? 2 : 1) : rows > 1 && max_keys >= 2048 ? 4 : 1;
+    // Rows enough for every slot are cut for the sake of long ones among short ones, where the longest that the table has room for would last: what is
+    // not cut is 7 to 15 % quicker where the rows are alike (64 rows of 2048, 8 nodes 64, 69; 512 rows, 2 nodes 432, 498).
+    int64_t splits = units < f.slots ? (f.slots + units - 1) / units * (rows > 1 ? 2 : 1) : max_keys >= 2048 && max_keys >= 1024 * units / f.slots ? 4 : 1;
+    if (rows == 1 && units >= f.slots) splits = 1;
     if (splits > most) splits = most;
     return (int)(splits < 1 ? 1 : splits > kTreeMaxSplits ? kTreeMaxSplits : splits);
 }
@@ -1235,7 +1242,7 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     a.slots = f.slots;
     a.least = f.least;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const int64_t grid = ((int64_t)rows * hkv + (f.wide ? 7 : 0)) / (f.wide ? 8 : 1) * (f.wide ? 8 : 1) * a.row_blocks * num_splits;
+    const int64_t places = (int64_t)rows * hkv * num_splits, grid = (f.wide ? (places + 7) / 8 * 8 : places) * a.row_blocks;
     if (grid > 0x7fffffff || rows > 65535) return MV_ERR_UNSUPPORTED;
     hipStream_t s = (hipStream_t)stream;
     const dim3 g1((unsigned)grid);
