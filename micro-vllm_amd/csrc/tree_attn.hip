@@ -1175,8 +1175,9 @@ int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, in
     if (rows <= 0 || max_nodes <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || max_keys <= 0) return 1;
     const TreeForm f = tree_form(rows, max_nodes, hkv, hq / hkv, d, f32, max_keys);
     // the launch that joins the splits costs some 3 us, a round of a workgroup 0.5 (heads of 64) to 1.2 (of 128): short rows are not cut (heads of 64,
-    // one row of 1200, 64 nodes whole 10.7, cut 12.5, of 2500 17.3, 16.0; heads of 128 of 600 14.4, 15.8, of 1200, 16 nodes 18.3, 14.4)
-    if (max_keys <= (f32 ? 384 : d == 64 ? 1536 : 1024)) return 1;
+    // one row of 1200, 64 nodes whole 10.7, cut 12.5, of 2500 17.3, 16.0; heads of 128 of 600 14.4, 15.8, of 1200, 16 nodes 18.3,
+    // 14.4; fp32, 8 heads of 64 of 300 8.3, 10.1, of 600 12.1, 10.6)
+    if (max_keys <= (f32 ? 512 : d == 64 ? 1536 : 1024)) return 1;
     // (as many as the kernels may want: they cut a row in fewer where its keys or the step's rows do not ask for them)
     const int64_t units = (int64_t)rows * hkv * f.row_blocks, most = ((int64_t)max_keys + f.round_keys * f.least - 1) / (f.round_keys * f.least);
     // Rows enough for every slot are cut for the sake of long ones among short ones, where the longest that the table has room for would last: what is
