@@ -22,6 +22,9 @@ MAX_NODES = 256      # nodes of a row with a tree or a mask
 
 
 _I32, _I64, _F32, _BF16 = torch.int32, torch.int64, torch.float32, torch.bfloat16
+# hipStream_t of a device's current stream, for a device that tensors lie on (nv.stream_ptr also asks which device and whether there is one: 0.3 us of
+# a small step's 8)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _vec(t: torch.Tensor, n: int, dev: int, dtype=_I32) -> int:
@@ -113,7 +116,7 @@ def tree_plan(ctx_lens: torch.Tensor, row_start: torch.Tensor, block_table: torc
     nv.check("mv_tree_plan", nv.lib().mv_tree_plan(
         _vec(ctx_lens, rows, dev), _vec(row_start, rows + 1, dev), None if parents is None else _vec(parents, tokens, dev), bt, bt_stride,
         cols, _vec(free_pages, free, dev), free, rows, tokens, max_nodes, page, num_pages, slots, positions, row_of, m, out.words, taken,
-        nv.stream_ptr()))
+        _stream(dev)))
     return out
 
 
@@ -157,7 +160,7 @@ def qkv_norm_rotary_slots(qkv: torch.Tensor, positions: torch.Tensor, slots: tor
         qkv.data_ptr(), ld if tokens > 1 else width, None if q_norm is None else _vec(q_norm, d, dev, _F32),
         None if k_norm is None else _vec(k_norm, d, dev, _F32), eps, None if rot == 0 else _vec(inv_freq, rot // 2, dev, torch.float64), rot,
         adjacent, _vec(positions, tokens, dev), _vec(slots, tokens, dev), out.data_ptr(), _heads(out, (tokens, heads, d), dst, dev, "out"),
-        k_cache.data_ptr(), v_cache.data_ptr(), pages * page, tokens, heads, kv_heads, d, src is _F32, dst is _F32, nv.stream_ptr()))
+        k_cache.data_ptr(), v_cache.data_ptr(), pages * page, tokens, heads, kv_heads, d, src is _F32, dst is _F32, _stream(dev)))
     return out
 
 
@@ -198,7 +201,7 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx
         q_ptr, _heads(q, shape, dtype, dev, "q"), k_cache.data_ptr(), v_cache.data_ptr(), _vec(ctx_lens, rows, dev),
         _vec(row_start, rows + 1, dev), bt, bt_stride, cols, m, words, out_ptr, _heads(out, shape, dtype, dev, "out"), ws or None, need, rows,
         tokens, max_nodes, heads, kv_heads, d, page, pages, d ** -0.5 if softmax_scale is None else softmax_scale, num_splits, f32,
-        nv.stream_ptr()))
+        _stream(dev)))
     return out
 
 
@@ -281,5 +284,5 @@ def tree_accept(tokens: torch.Tensor, picks: torch.Tensor, row_start: torch.Tens
         move = (*_table(block_table, rows, dev), caches.k, caches.v, caches.layers, caches.row_bytes, caches.page, caches.pages)
     nv.check("mv_tree_accept", nv.lib().mv_tree_accept(
         _vec(tokens, n_tokens, dev, _I64), _vec(picks, n_tokens, dev, _I64), None if parents is None else _vec(parents, n_tokens, dev),
-        _vec(row_start, rows + 1, dev), ctx, *move, rows, n_tokens, max_nodes, out.max_path, path, ids, counts, lens, nv.stream_ptr()))
+        _vec(row_start, rows + 1, dev), ctx, *move, rows, n_tokens, max_nodes, out.max_path, path, ids, counts, lens, _stream(dev)))
     return out
