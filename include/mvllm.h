@@ -971,7 +971,7 @@ int mv_tree_plan(const int32_t* ctx_lens, const int32_t* row_start, const int32_
  * itself (q_norm / k_norm fp32 [d]; NULL: none), then the rotation of its first `rot` dimensions by positions[t] * inv_freq[i] (fp64
  * [rot / 2]; adjacent pairs, or i with i + rot / 2); q to q_out [tokens, ldq], k and v to the caches' slot slots[t] (outside
  * [0, cache_slots): not stored), bf16 or (dst_f32, from fp32 rows only) fp32.  fp32 throughout, rounded once.  q_out may be
- * q's part of qkv where the types agree. */
+ * q's part of qkv where the types agree, and may share no other memory with it. */
 int mv_qkv_norm_rotary_slots(const void* qkv, int64_t ld, const float* q_norm, const float* k_norm, float eps, const double* inv_freq,
                              int rot, int adjacent, const int32_t* positions, const int32_t* slots, void* q_out, int64_t ldq,
                              void* k_cache, void* v_cache, int64_t cache_slots, int tokens, int heads, int kv_heads, int d, int src_f32,
@@ -979,8 +979,10 @@ int mv_qkv_norm_rotary_slots(const void* qkv, int64_t ld, const float* q_norm, c
 
 /* out[t, h] = sum_j softmax_j(q[t, h] . k_j * scale) v_j over the row's cached tokens and the nodes of mask[t] (NULL: the nodes up to t),
  * whose keys and values are in the cache [num_pages, page, hkv, d].  q [tokens, ldq], out [tokens, ldo], caches bf16 or (f32) fp32, all 16-byte
- * aligned; d 64 or 128, hq / hkv <= 8, page a power of two >= 16.  A node that sees nothing: zeros.  Places whose page is not in
- * [0, num_pages) and keys behind column bt_cols do not count.  scale > 0.  num_splits (1 .. 64) pieces of the keys side by side;
+ * aligned; d 64 or 128, hq / hkv <= 8, page a power of two >= 16, page * bt_cols <= 2^30.  A node that sees nothing: zeros.  Places whose
+ * page is not in [0, num_pages) and keys behind column bt_cols do not count; q . k * scale below 2^30 in size (fp32 scores, and the
+ * difference to the row's largest is formed from their rounded products).  scale > 0.  out may not share memory with q.  num_splits
+ * (1 .. 64) pieces of the keys side by side;
  * workspace: of mv_tree_attn_workspace_bytes, 16-byte aligned, needs no clearing, of one running call at a time. */
 size_t mv_tree_attn_workspace_bytes(int tokens, int hq, int d, int num_splits);
 /* How many pieces a step should be given (max_keys: the longest row there may be). */

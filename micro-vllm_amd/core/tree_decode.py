@@ -145,7 +145,7 @@ def qkv_norm_rotary_slots(qkv: torch.Tensor, positions: torch.Tensor, slots: tor
     2 * inv_freq.numel() dimensions are turned by positions[t] * inv_freq (float64; None: no rotation; `adjacent` pairs (2i, 2i + 1), else i
     with i + half), all of it in fp32 and rounded once.  q goes to out [tokens, heads, d], k and v to k_cache / v_cache
     [pages, page, kv_heads, d] at slots[t] (negative or past the last page: not stored; no two tokens may name one slot).  qkv bf16 with bf16
-    caches, float32 with either; out has the caches' type and may be q's own part of qkv where the types agree."""
+    caches, float32 with either; out has the caches' type and may be q's own part of qkv where the types agree, no other part of it."""
     dev = _current(qkv)
     pages, page, kv_heads, d = _cache(k_cache, v_cache, dev)
     (tokens, width), src, dst = qkv.shape, qkv.dtype, k_cache.dtype
@@ -171,8 +171,9 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx
     be a tree's; None: a chain), whose keys and values are in the cache already.  q [tokens, heads, d] bf16 or float32 as the caches
     [pages, page, kv_heads, d]; d 64 or 128, up to eight heads to a kv head, pages of a power of two of 16 tokens or more; max_nodes (at most
     256) bounds the nodes of a row.  A node that sees nothing gets zeros; places without a page (-1) and keys behind the table's last
-    column do not count; tokens behind the last row, and nodes past max_nodes, keep what `out` held.  Scores and softmax in fp32; bf16:
-    weights rounded to bf16 in front of the product with the values.  num_splits 0: picked; `workspace`: float32, at least
+    column do not count; tokens behind the last row, and nodes past max_nodes, keep what `out` held.  Scores (below 2^30 in size) and
+    softmax in fp32; bf16: weights rounded to bf16 in front of the product with the values.  `out` may not share memory with q; the table
+    has room for 2^30 keys at most.  num_splits 0: picked; `workspace`: float32, at least
     tree_attn_workspace(...) bytes, of this call alone while it runs (default: allocated)."""
     dev = _current(q)
     pages, page, kv_heads, d = _cache(k_cache, v_cache, dev)

@@ -455,6 +455,32 @@ def test_a_long_cache_past_32_bit_offsets(ops):
     small.check(out, "far pages")
 
 
+def test_store_and_accept_past_32_bit_offsets(ops):
+    """Slots whose first value lies past 2^32 bytes from the pool's: stored there, and moved there."""
+    hkv, d, page, hq = 8, 128, 64, 8
+    pages = (1 << 32) // (page * hkv * d * 2) + 4
+    k = torch.zeros(pages, page, hkv, d, dtype=BF16, device=DEV)
+    v = torch.zeros(pages, page, hkv, d, dtype=BF16, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(6)
+    qkv = torch.randn(6, (hq + 2 * hkv) * d, generator=g, device=DEV).to(BF16)
+    table = i32([[pages - 1, pages - 2]], DEV)
+    starts, ctx = i32([0, 6], DEV), i32([61], DEV)
+    plan = ops.tree_plan(ctx, starts, table, i32([pages - 2], DEV), 6, page, pages, parents=i32([-1, 0, 0, 2, 3, 4], DEV))
+    assert plan.slots.tolist() == [(pages - 1) * page + 61 + i for i in range(3)] + [(pages - 2) * page + i for i in range(3)]
+    ops.qkv_norm_rotary_slots(qkv, plan.positions, plan.slots, k, v, hq)
+    kv = qkv[:, hq * d:].view(6, 2, hkv, d)
+    where = [(pages - 1, 61 + i) for i in range(3)] + [(pages - 2, i) for i in range(3)]
+    assert all(torch.equal(k[p, s], kv[i, 0]) and torch.equal(v[p, s], kv[i, 1]) for i, (p, s) in enumerate(where))
+    tokens = torch.arange(6, device=DEV)
+    picks = torch.tensor([2, 9, 3, 4, 5, 9], device=DEV)      # 0, 2, 3, 4, 5
+    got = ops.tree_accept(tokens, picks, starts, ctx, 6, parents=i32([-1, 0, 0, 2, 3, 4], DEV), caches=ops.TreeCaches([k], [v]), block_table=table)
+    assert got.path.tolist() == [[0, 2, 3, 4, 5, -1]]
+    for j, node in enumerate([0, 2, 3, 4, 5]):
+        p, s = where[j]
+        assert torch.equal(k[p, s], kv[node, 0]) and torch.equal(v[p, s], kv[node, 1])
+    assert int((k != 0).any(-1).any(-1).sum()) == 6            # and nowhere else
+
+
 # ---------------------------------------------------------------------------------------------------------------- accept
 def accept_case(ctx, counts, page, layers, hkv, d, dtype, seed, vocab=5, forest=False):
     rng = np.random.default_rng(seed)
