@@ -34,6 +34,7 @@ struct TreeArgs {
     int bt_cols, rows, tokens, max_nodes, hq, hkv, g, page, page_shift, num_pages, nsplit, row_blocks;
     int round_keys;              // keys that a split's workgroup takes in one round
     int row_part, slots, least;  // stacked rows of a workgroup, workgroups that run at once, rounds below which nothing is cut
+    int per_unit;                // slots of a compute unit
     float scale_log2;
 };
 
@@ -62,28 +63,43 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int b) {
 }
 // How many of the launch's splits a row of `total` keys takes.  A piece of work is a round (round_keys keys of up to row_part stacked rows of one
 // key/value head); rows are cut so that no split has more than its share of the step's rounds over `slots` workgroups: where rows differ in
-// length the long ones take more splits, and where there are rounds enough for every slot none is cut.  In two halves, the rounds that a lane
-// counts (its loads go out with a kernel's first) and their sum; all lanes of a wave call them together.
-__device__ __forceinline__ int step_rounds(const TreeArgs& a) {
-    int work = 0;
+// length the long ones take more splits, and where there are rounds enough for every slot none is cut.  Nor is any where the longest row is no more than
+// a compute unit's share of all (two workgroups run on one: 32 rows of 4096 to 8192 keys, 64 nodes of 8B heads, cut to their shares 277 us, whole 245).  In
+// two halves, what a lane counts (its loads go out with a kernel's first) and their sums; all lanes of a wave call them together.
+struct TreeWork {
+    int rounds, longest;
+};
+__device__ __forceinline__ TreeWork step_work(const TreeArgs& a) {
+    TreeWork w = {0, 0};
     if (a.nsplit > 1)
         for (int i = threadIdx.x & 63; i < a.rows; i += 64) {
             const int from = min(max(a.row_start[i], 0), a.tokens);
             const int n = min(min(max(a.row_start[i + 1], from), a.tokens) - from, a.max_nodes);
-            const int keys = (int)min((int64_t)max(a.ctx[i], 0) + n, (int64_t)a.bt_cols << a.page_shift);
-            work += ((n * a.g + a.row_part - 1) / a.row_part) * ((keys + a.round_keys - 1) / a.round_keys);
+            const int keys = (int)min((int64_t)max(a.ctx[i], 0) + n, (int64_t)a.bt_cols << a.page_shift), rounds = (keys + a.round_keys - 1) / a.round_keys;
+            w.rounds += (n * a.g + a.row_part - 1) / a.row_part * rounds;
+            w.longest = max(w.longest, n > 0 ? rounds : 0);
         }
-    return work;
+    return w;
 }
-__device__ __forceinline__ int row_splits(const TreeArgs& a, int total, int work) {
+template <int SHR> __device__ __forceinline__ void add_lanes(TreeWork& w) {      // from SHR lanes below, within rows of 16
+    w.rounds += __builtin_amdgcn_update_dpp(0, w.rounds, 0x110 + SHR, 0xf, 0xf, true);
+    w.longest = max(w.longest, __builtin_amdgcn_update_dpp(0, w.longest, 0x110 + SHR, 0xf, 0xf, true));
+}
+__device__ __forceinline__ int row_splits(const TreeArgs& a, int total, TreeWork w) {
     if (a.nsplit == 1) return 1;
-    work += __builtin_amdgcn_update_dpp(0, work, 0x111, 0xf, 0xf, true);      // row_shr 1, 2, 4, 8: a row's sum in its lane 15
-    work += __builtin_amdgcn_update_dpp(0, work, 0x112, 0xf, 0xf, true);
-    work += __builtin_amdgcn_update_dpp(0, work, 0x114, 0xf, 0xf, true);
-    work += __builtin_amdgcn_update_dpp(0, work, 0x118, 0xf, 0xf, true);
-    const int64_t sum = (int64_t)__builtin_amdgcn_readlane(work, 15) + __builtin_amdgcn_readlane(work, 31) + __builtin_amdgcn_readlane(work, 47) +
-                        __builtin_amdgcn_readlane(work, 63);
+    add_lanes<1>(w);
+    add_lanes<2>(w);
+    add_lanes<4>(w);
+    add_lanes<8>(w);
+    int64_t sum = 0;
+    int longest = 0;
+#pragma unroll
+    for (int l = 15; l < 64; l += 16) {
+        sum += __builtin_amdgcn_readlane(w.rounds, l);
+        longest = max(longest, __builtin_amdgcn_readlane(w.longest, l));
+    }
     const int share = max((int)((sum * a.hkv + a.slots - 1) / a.slots), a.least), rounds = (total + a.round_keys - 1) / a.round_keys;
+    if (longest <= share * a.per_unit) return 1;
     return max(1, min(a.nsplit, (rounds + share - 1) / share));
 }
 // Which of the 32 keys from kb on a node sees (bit i: key kb + i): cached tokens all, nodes by its mask, whose first word is given
@@ -211,12 +227,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_f32_kernel(TreeArgs a) {
     Entry* bt = (Entry*)(uintptr_t)(a.block_table + (int64_t)b * a.bt_stride);
     auto page_of = [&](int blk) { return bt[min((blk * kTreeBlock) >> a.page_shift, a.bt_cols - 1)]; };
     int blk = split * W + wid, pg = page_of(blk);
-    const int rounds = step_rounds(a);
+    const TreeWork work = step_work(a);
     const TreeSpan s = tree_span(a, b);
     const int stacked = s.n * a.g, row0 = rb * RT * 16;
     const int blocks = (s.total + kTreeBlock - 1) / kTreeBlock;
     if (row0 >= stacked || (split > 0 && split * a.round_keys >= s.total)) return;
-    const int splits = row_splits(a, s.total, rounds);
+    const int splits = row_splits(a, s.total, work);
     if (split >= splits) return;
 
     const unsigned row_bytes = (unsigned)a.hkv * D * 4, k_at = r * row_bytes + 16 * q, v_at = 4 * q * row_bytes + 16 * r;
@@ -412,11 +428,11 @@ __global__ __launch_bounds__(256, 2) void tree_attn_narrow_kernel(TreeArgs a) {
     int blk = split * W + wid, pg[2];
     bool odd = false;
     pages_of(blk, pg);
-    const int rounds = step_rounds(a);
+    const TreeWork work = step_work(a);
     const TreeSpan s = tree_span(a, b);
     const int stacked = s.n * a.g, row0 = rb * ROWS, blocks = (s.total + 31) / 32;
     if (row0 >= stacked || (split > 0 && split * a.round_keys >= s.total)) return;
-    const int splits = row_splits(a, s.total, rounds);
+    const int splits = row_splits(a, s.total, work);
     if (split >= splits) return;
 
     // (a request = a base that is the same for the wave, in scalar registers, and a lane's offset of 32 bits that never changes)
@@ -643,12 +659,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     const TreePlace w = tree_place(a);
     const int split = w.split, rb = w.rb, kvh = w.kvh, b = w.b;
     if (split >= a.nsplit) return;
-    const int rounds = step_rounds(a);
+    const TreeWork work = step_work(a);
     const TreeSpan s = tree_span(a, b);
     // a row's stacked rows in as few parts as 128 (64) allow, of even size
     const int stacked = s.n * a.g, parts = (stacked + 128 / KW - 1) / (128 / KW);
     if (rb >= parts || (split > 0 && split * 64 * a.least >= s.total)) return;
-    const int splits = row_splits(a, s.total, rounds);
+    const int splits = row_splits(a, s.total, work);
     if (split >= splits) return;
     const int part_rows = ((stacked + parts - 1) / parts + 31) & ~31, row0 = rb * part_rows;
     if (row0 >= stacked) return;
@@ -1097,9 +1113,9 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
     __shared__ float topL[GROUPS], denL[GROUPS];
     __shared__ f32x4_t oL[256];
     const int b = blockIdx.y, group = threadIdx.x / LPR, c = threadIdx.x % LPR * 4;
-    const int rounds = step_rounds(a);
+    const TreeWork work = step_work(a);
     const TreeSpan s = tree_span(a, b);
-    const int filled = row_splits(a, s.total, rounds);
+    const int filled = row_splits(a, s.total, work);
     if (filled <= 1) return;
     int shift = 0;
     while ((MOST << shift) < filled && (1 << shift) < GROUPS) ++shift;
@@ -1175,7 +1191,7 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
 // 128 in the narrow form (107, wide 120).  fp32, whose blocks are bound by their matrix instructions, 16 or 32 rows by the same rule (4 rows of 2500, 16 heads
 // of 64 on 4, 16 nodes 18.4, 21.7; 64 nodes of heads of 128 75, 66).
 struct TreeForm {
-    int row_tiles, row_part, row_blocks, round_keys, wide, slots, least;
+    int row_tiles, row_part, row_blocks, round_keys, wide, per_unit, slots, least;
 };
 static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f32, int64_t max_keys) {
     const int64_t stacked = (int64_t)max_nodes * g, heads = (int64_t)rows * hkv;
@@ -1196,7 +1212,8 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     // Work for one workgroup a unit, or for two where there are two without any cut (wide, us with one and two: 32 uneven rows of up to 8191, 64 nodes
     // of 8B heads 211, 205; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4)
     const bool two = f.wide ? heads * f.row_blocks >= 2 * num_cus() : f32 && (d == 64 || f.row_tiles == 1);
-    f.slots = num_cus() * (two ? 2 : 1);
+    f.per_unit = two ? 2 : 1;
+    f.slots = num_cus() * f.per_unit;
     f.least = f.wide ? 6 : 1;
     return f;
 }
@@ -1284,6 +1301,7 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     a.row_part = f.row_part;
     a.slots = f.slots;
     a.least = f.least;
+    a.per_unit = f.per_unit;
     a.scale_log2 = scale * 1.4426950408889634f;
     const int64_t places = (int64_t)rows * hkv * num_splits, together = places >= 8 ? 8 : 1, high = (places + together - 1) / together;
     if (high > 65535 || rows > 65535) return MV_ERR_UNSUPPORTED;
