@@ -40,7 +40,7 @@ struct TreeArgs {
 
 // Which keys and stacked rows a workgroup has: the grid is (8, row_blocks, places / 8), a place a row's split for one key/value head.  Workgroups go to the
 // eight XCDs in turn, so the row_blocks workgroups that want the same keys are on one of them, and what one asks for the others find in its L2 (4 rows of
-// 900 keys, 16 nodes of 8B heads, 32 stacked rows a workgroup: 20.2 -> 17.8 us; where there are fewer places than XCDs x is 1).  Splits slowest: where
+// 1200 keys, 64 nodes of 8B heads, 32 stacked rows a workgroup: 32 -> 21 us; where there are fewer places than XCDs x is 1).  Splits slowest: where
 // no row is cut the first workgroups have the work.
 struct TreePlace {
     int split, rb, kvh, b;
@@ -1105,7 +1105,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
 }
 
 // Splits added in order; rows that one split holds are written already.  A (node, head) is 2^shift groups of D / 4 lanes, each of which adds every
-// 2^shift-th split with all its requests out at once (64 splits in one group: 32 dependent trips, 17 us where this takes 3).
+// 2^shift-th split with all its requests out at once (64 splits in one group: 32 dependent trips, 17 us where this takes 4).
 template <bool F32, int D>
 __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
     typedef TreeT<F32> X;
@@ -1209,8 +1209,8 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     f.row_part = f.wide ? (stacked <= 64 ? 64 : 128) : 16 * f.row_tiles;
     f.row_blocks = (int)((stacked + f.row_part - 1) / f.row_part);
     f.round_keys = f.wide || f32 ? 64 : 128;
-    // Work for one workgroup a unit, or for two where there are two without any cut (wide, us with one and two: 32 uneven rows of up to 8191, 64 nodes
-    // of 8B heads 211, 205; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4)
+    // Work for one workgroup a unit, or for two where there are two without any cut (wide, us with one and two: 32 uneven rows of 256 to 8191, 64
+    // nodes of 8B heads 203, 199; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4)
     const bool two = f.wide ? heads * f.row_blocks >= 2 * num_cus() : f32 && (d == 64 || f.row_tiles == 1);
     f.per_unit = two ? 2 : 1;
     f.slots = num_cus() * f.per_unit;

@@ -176,6 +176,26 @@ def test_norm_rotary_slots_in_place(ops, dtype, d, rot, adjacent):
     assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("off,extra,out_off", [(1, 0, 0), (8, 1, 0), (0, 0, 3), (4, 4, 0)])
+def test_norm_rotary_slots_of_rows_that_are_not_aligned(ops, dtype, off, extra, out_off):
+    """Rows, strides and outputs off the 16-byte grid: the values of rows on it, up to a sum's order."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    hq, hkv, d, T = 5, 2, 128, 21
+    width = (hq + 2 * hkv) * d
+    buf = torch.randn(T, width + off + extra, generator=g, device=DEV).to(dtype)
+    pos, slots = torch.arange(T, dtype=torch.int32, device=DEV) * 7, torch.arange(T, dtype=torch.int32, device=DEV)
+    w, freqs = torch.rand(d, generator=g, device=DEV) + 0.5, rotary_freqs(d // 2).to(DEV)
+    caches = [torch.zeros(2, 16, hkv, d, dtype=dtype, device=DEV) for _ in range(2)]
+    out = torch.zeros(T, hq * d + 8, dtype=dtype, device=DEV)[:, out_off:out_off + hq * d].unflatten(1, (hq, d))
+    ops.qkv_norm_rotary_slots(buf[:, off:off + width], pos, slots, *caches, hq, w, w, 1e-6, freqs, out=out)
+    q, k, v, mq, mk = ref.norm_rotary(buf[:, off:off + width].cpu(), hq, hkv, d, pos.cpu(), w.cpu(), w.cpu(), 1e-6, freqs.cpu(), False)
+    half, rel = torch.finfo(dtype).eps / 2, (d / 2 + 32) * 2.0 ** -24 + 140 * 2.0 ** -50       # (as in test_norm_rotary_slots)
+    assert ((out.double().cpu() - q).abs() <= half * q.abs() + 1.01 * rel * mq).all()
+    got = [c.view(-1, hkv, d)[:T].double().cpu() for c in caches]
+    assert ((got[0] - k).abs() <= half * k.abs() + 1.01 * rel * mk).all() and torch.equal(got[1], v.to(dtype).double())
+
+
 # ------------------------------------------------------------------------------------------------------------- attention
 # Which kernel a launch takes goes by its rows and by the keys that its table has room for: behind this many columns more every launch takes the form
 # for much work (bf16: 16, 32 or (heads of 64) 64 stacked rows a workgroup, past 64 (heads of 128: 32) keys shared by the waves; fp32: 32 rows).
@@ -258,6 +278,48 @@ def test_attention_of_many_rows(ops, dtype):
     for splits in (0, 1, 4):
         for cols in (0, MUCH):
             case.check(run_attn(ops, case, splits, cols=cols), f"splits {splits} columns {cols}", want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hq,d", [(1, 64), (2, 128), (8, 64), (8, 128)])
+@pytest.mark.parametrize("cols", [0, MUCH])
+def test_a_query_that_is_not_finite_is_its_own(ops, dtype, hq, d, cols):
+    """NaN in one head of one node: NaN there, every other head and node as without it; a mask of more words than the nodes need."""
+    case = AttnCase([200], [30], hq, 1, d, 16, dtype, seed=17)
+    case.words = 4
+    want = case.reference()
+    case.q[11, hq - 1, 7] = float("nan")
+    keep = torch.ones(30, hq, dtype=torch.bool)
+    keep[11, hq - 1] = False
+    for splits in (1, 3):
+        out = run_attn(ops, case, splits, cols=cols)[:30].double().cpu()
+        o, mag, size, count = want
+        assert out[11, hq - 1].isnan().all() and ((out - o).abs() <= ref.attn_bound(o, mag, size, count, d, dtype))[keep].all()
+
+
+def test_threads_with_streams_of_their_own(ops):
+    """Four threads, a stream each, rows cut into splits: everyone's workspace is their own."""
+    import threading
+    cases = [AttnCase([900 + 40 * i, 30], [20, 7 + i], 8, 2, 64, 64, BF16, seed=30 + i) for i in range(4)]
+    alone = [run_attn(ops, c, 6) for c in cases]
+    torch.cuda.synchronize()
+    got, wrong = [None] * 4, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = run_attn(ops, cases[i], 6)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:      # (an assertion of a thread is the test's)
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and all(torch.equal(a, b) for a, b in zip(alone, got))
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
