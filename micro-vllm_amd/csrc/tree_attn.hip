@@ -1210,8 +1210,10 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     f.row_blocks = (int)((stacked + f.row_part - 1) / f.row_part);
     f.round_keys = f.wide || f32 ? 64 : 128;
     // Work for one workgroup a unit, or for two where there are two without any cut (wide, us with one and two: 32 uneven rows of 256 to 8191, 64
-    // nodes of 8B heads 203, 199; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4)
-    const bool two = f.wide ? heads * f.row_blocks >= 2 * num_cus() : f32 && (d == 64 || f.row_tiles == 1);
+    // nodes of 8B heads 203, 199; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4;
+    // fp32 of much work, 4 rows of 6000, 64 nodes, 16 heads of 64 on 4 84, 76, of less one row of 3000, 16 nodes 12.9, 14.4, heads of 128 16.5, 19.5)
+    const bool two = f.wide ? heads * f.row_blocks >= 2 * num_cus()
+                            : f32 && (d == 64 || f.row_tiles == 1) && heads * f.row_blocks * max_keys >= 200000;
     f.per_unit = two ? 2 : 1;
     f.slots = num_cus() * f.per_unit;
     f.least = f.wide ? 6 : 1;
