@@ -12,6 +12,7 @@ on one device, which has to be the current one; every call goes to the current s
 `workspace`), and can be captured.  Rows must not share the pages that a step's nodes lie in.
 """
 import ctypes
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -164,6 +165,12 @@ def qkv_norm_rotary_slots(qkv: torch.Tensor, positions: torch.Tensor, slots: tor
     return out
 
 
+@lru_cache(maxsize=1024)
+def _pick_splits(dev: int, rows: int, max_nodes: int, heads: int, kv_heads: int, d: int, max_keys: int, f32: bool) -> int:
+    """mv_tree_attn_pick_splits, a function of the sizes and of the current device (the argument `dev`)."""
+    return nv.lib().mv_tree_attn_pick_splits(rows, max_nodes, heads, kv_heads, d, max_keys, f32)
+
+
 def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx_lens: torch.Tensor, row_start: torch.Tensor,
               block_table: torch.Tensor, mask: Optional[torch.Tensor], max_nodes: int, softmax_scale: Optional[float] = None,
               out: Optional[torch.Tensor] = None, num_splits: int = 0, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -190,7 +197,7 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx
     bt, bt_stride, cols = _table(block_table, rows, dev)
     L, f32 = nv.lib(), dtype is _F32
     if num_splits <= 0:
-        num_splits = L.mv_tree_attn_pick_splits(rows, max_nodes, heads, kv_heads, d, cols * page, f32)
+        num_splits = _pick_splits(dev, rows, max_nodes, heads, kv_heads, d, cols * page, f32)
     ws = need = 0
     if num_splits > 1:
         need = L.mv_tree_attn_workspace_bytes(tokens, heads, d, num_splits)
