@@ -624,13 +624,16 @@ __global__ __launch_bounds__(256, 2) void tree_attn_narrow_kernel(TreeArgs a) {
 //   * v_mfma_f32_32x32x16_bf16: S^T = K . Q^T leaves a lane (row l & 31, half h = l >> 5) 16 scores of a 32-key block, keys (i & 3) + 8 (i >> 2) +
 //     4 h; registers 8 s .. 8 s + 7, rounded to bf16, are operand B of step s of O^T += V^T . P^T as they stand, and the transposing reads of
 //     V deliver those keys.
-//   * pipeline over 32-key blocks: while the matrix unit forms S of block u + 1 the vector unit turns S of u into weights, the matrix unit then adds
-//     V^T P of u; LDS reads run a few matrix instructions ahead.  Pieces are dealt out slot by slot between scheduling fences.
+//   * pipeline over 32-key blocks: the matrix unit forms S of block u + 1 and adds V^T P of u, the vector unit turns scores into weights, half of a
+//     block's in the step behind their product and half in the next, LDS reads run a few matrix instructions ahead, requests go out one a slot.  All of
+//     it is dealt out slot by slot (a matrix instruction each) between scheduling fences.  A tile takes 0.8 us where 0.43 are matrix instructions (1.05 with
+//     a block's weights all in one step, all requests in front and a scalar page number a tile).
 //   * no running maximum: weights are 2^(s - m) with m the maximum of the row's first block.  Their size does not touch their precision (bf16 and
 //     the fp32 sums are relative), only their range, so a row whose denominator or sums leave the range that is safe - scores 44 nats above those of
 //     its first block - makes the workgroup do its keys again with a running maximum.  (The maximum of every block, its exchange between lanes and
-//     the test for a rescale were a fifth of the vector unit's work: 32 rows of 4096 and 64 nodes 188 -> 165 us.)
-//   * a tile in which every key counts for every row (all but the one or two with nodes in them) takes no mask.
+//     the test for a rescale were a fifth of the vector unit's work: 32 rows of 4096 and 64 nodes 188 -> 165 us, now 151.)
+//   * a tile in which every key counts for every row (all but the one or two with nodes in them) takes no mask; the others, and the second pass, go through
+//     a plainer step.
 // Waves without rows (short trees) only stage.  KW 2, for up to 64 rows: two waves take the two 32-key blocks of a tile for the same 32 rows and join
 // their states at the end.
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
@@ -681,34 +684,34 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
 #pragma unroll
         for (int k = 0; k < KS; ++k) qf[k] = __builtin_bit_cast(bf16x8_t, ld16(qp + k * 16));
     }
-    // ---- pages: the four runs of 16 keys of a tile lie in a page each; a wave stages one of them
-    typedef const int32_t __attribute__((address_space(4))) Entry;      // (nothing here writes the table: scalar loads)
-    Entry* bt = (Entry*)(uintptr_t)(a.block_table + (int64_t)b * a.bt_stride);
-    struct Pages {
-        int own;               // of the wave's run
-        uint64_t there;        // keys of the tile that lie in a page
-    };
-    const bool small = a.page_shift < 6;      // pages of less than a tile
-    auto page_ids = [&](int t) __attribute__((always_inline)) {
-        const int kb = min(t, t1 - 1) * KT;
-        Pages r;
-        r.own = bt[min((kb + 16 * wid) >> a.page_shift, a.bt_cols - 1)];
-        r.there = (unsigned)r.own < (unsigned)a.num_pages ? ~0ull : 0;
-        if (small) {
-            r.there = 0;
+    // ---- pages: the four runs of 16 keys of a tile lie in a page each; a wave stages one of them.  The numbers of 64 tiles are asked for at once: lane l has
+    // the page of the wave's run of tile tb + l, and which of that tile's four runs have one (a scalar load a tile, waited for with every LDS read on
+    // its way, was a tenth of the loop)
+    const int32_t* table = a.block_table + (int64_t)b * a.bt_stride;
+    int tb, ids, oks, open_end;      // open_end: tiles in front of this one take no mask, as far as their pages are known
+    auto fill = [&](int t) __attribute__((always_inline)) {
+        tb = t;
+        const int kb = min(t + lane, t1 - 1) * KT;
+        ids = table[min((kb + 16 * wid) >> a.page_shift, a.bt_cols - 1)];
+        oks = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if ((unsigned)bt[min((kb + 16 * i) >> a.page_shift, a.bt_cols - 1)] < (unsigned)a.num_pages) r.there |= 0xffffull << (16 * i);
-        }
-        return r;
+        for (int i = 0; i < 4; ++i) oks |= (int)((unsigned)table[min((kb + 16 * i) >> a.page_shift, a.bt_cols - 1)] < (unsigned)a.num_pages) << i;
+        asm volatile("" : "+v"(ids));      // (both have landed: nothing waits for them in the loop)
+        const uint64_t holes = __builtin_amdgcn_ballot_w64(oks != 15);
+        if (holes) open_end = min(open_end, t + __builtin_ctzll(holes));
     };
-    auto counted = [&](int t, const Pages& g) __attribute__((always_inline)) {      // keys of a tile that count (the last splits may have no tile)
-        const int left = s.total - t * KT;
-        return left < KT ? g.there & ((1ull << max(left, 0)) - 1) : g.there;
+    auto counted = [&](int t) __attribute__((always_inline)) -> uint64_t {      // keys of a tile that count (the last splits may have no tile)
+        const int left = s.total - t * KT, ok = __builtin_amdgcn_readlane(oks, min(t, t1 - 1) - tb);
+        uint64_t there = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) there |= ok >> i & 1 ? 0xffffull << (16 * i) : 0;
+        return left < KT ? there & ((1ull << max(left, 0)) - 1) : there;
     };
+    auto open_tile = [&](int t, uint64_t bits) __attribute__((always_inline)) { return bits == ~0ull && (t + 1) * KT <= s.ctx; };
     const unsigned row_bytes = (unsigned)a.hkv * RB;
-    auto base_of = [&](int t, const Pages& g) __attribute__((always_inline)) {      // byte offset in either cache of the wave's first row
-        const int64_t row = ((int64_t)((unsigned)g.own < (unsigned)a.num_pages ? g.own : 0) << a.page_shift) + ((min(t, t1 - 1) * KT + 16 * wid) & (a.page - 1));
+    auto base_of = [&](int t) __attribute__((always_inline)) {      // byte offset in either cache of the wave's first row
+        const int at = min(t, t1 - 1), page = __builtin_amdgcn_readlane(ids, at - tb);
+        const int64_t row = ((int64_t)((unsigned)page < (unsigned)a.num_pages ? page : 0) << a.page_shift) + ((at * KT + 16 * wid) & (a.page - 1));
         return row * row_bytes + kvh * RB;
     };
     // The LDS image of a tile is its rows back to back; 16-byte piece c of row r stands at c ^ k_turn(r) (keys: operand reads of 16 rows) or
@@ -729,13 +732,11 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                      : : "v"(from), "s"((const unsigned char*)cache + base), "s"(dst) : "memory");
     };
-    auto copy_k = [&](int64_t base, int slot) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i) copy(a.k_cache, base, k_from[i], kring + slot * TB + wid * 16 * RB + i * 1024);
+    auto copy_k = [&](int64_t base, int slot, int i) __attribute__((always_inline)) {
+        copy(a.k_cache, base, k_from[i], kring + slot * TB + wid * 16 * RB + i * 1024);
     };
-    auto copy_v = [&](int64_t base, int slot) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i) copy(a.v_cache, base, v_from[i], vring + slot * TB + wid * 16 * RB + i * 1024);
+    auto copy_v = [&](int64_t base, int slot, int i) __attribute__((always_inline)) {
+        copy(a.v_cache, base, v_from[i], vring + slot * TB + wid * 16 * RB + i * 1024);
     };
     // values of keys that do not count become zero, and what is not finite of the others is left for the end: in the pieces that this wave asked
     // for, once they are there
@@ -751,7 +752,6 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
             *at = v;
         }
     };
-    auto open_tile = [&](int t, uint64_t bits) __attribute__((always_inline)) { return bits == ~0ull && (t + 1) * KT <= s.ctx; };
     // which of a tile's keys the lane's row sees
     auto visible = [&](int t, uint64_t bits) __attribute__((always_inline)) -> uint64_t {
         const int first = t * KT - s.ctx;
@@ -788,8 +788,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     bool saw = false;                  // any key
     uint32_t pw[8];
     float fa[8][2], eb[8][2];
-    auto softmax_slot = [&](const f32x16_t& sc, int at) __attribute__((always_inline)) {      // three stages of a pair of scores, a slot apart
-        constexpr int kEnter128[8] = {1, 2, 3, 4, 5, 6, 7, 8}, kEnter64[8] = {1, 1, 1, 1, 2, 2, 3, 3};
+    // The eight pairs of a lane's scores of a block take three stages, a slot apart: product with the scale, exponential, sum and packing.  A block's slots are
+    // numbered from the step that adds its values; the first pairs go through during the step before (negative numbers), behind that step's scores, so
+    // that the vector unit has about as much to do in every slot.  Pairs 0 to 3 are due in slot KS, 4 to 7 in KS + DB.
+    constexpr int NS = KS + NP;
+    auto softmax_slot = [&](const f32x16_t& sc, int at) __attribute__((always_inline)) {
+        constexpr int kEnter128[8] = {-5, -3, 0, 2, 4, 6, 8, 9}, kEnter64[8] = {-3, -2, -1, 0, 0, 1, 2, 3};
 #pragma unroll
         for (int pr = 0; pr < 8; ++pr)
             if (at == (D == 128 ? kEnter128[pr] : kEnter64[pr]) + 2) {
@@ -809,6 +813,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
                 fa[pr][0] = __builtin_fmaf(sc[2 * pr], a.scale_log2, -mrun);
                 fa[pr][1] = __builtin_fmaf(sc[2 * pr + 1], a.scale_log2, -mrun);
             }
+    };
+    auto softmax_ahead = [&](const f32x16_t& sc) __attribute__((always_inline)) {      // what belongs into the step before a block's, at once
+#pragma unroll
+        for (int at = -NS; at < 0; ++at) softmax_slot(sc, at);
     };
     auto p_frag = [&](int st) __attribute__((always_inline)) {
         return __builtin_bit_cast(bf16x8_t, make_uint4(pw[4 * st], pw[4 * st + 1], pw[4 * st + 2], pw[4 * st + 3]));
@@ -845,13 +853,13 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
         }
     };
     // Block u (scores sc, masked): weights, O += V^T P; scores of block u + 1 (keys at kblock) into sn.  kpre: its first reads, made
-    // during the step before, refilled from kblock_after.
+    // during the step before, refilled from kblock_after.  `dealt`: the first weights of block u + 1 in the slots too; else behind them, raised maximum
+    // first where it runs.  hook(i): what else goes into slot i.
     bf16x8_t kpre[PF];
     auto block_step = [&](const f32x16_t& sc, f32x16_t& sn, const unsigned char* kblock, const unsigned char* vblock,
-                          const unsigned char* kblock_after, uint32_t vis_next, auto has_next, auto has_after,
-                          auto mask_next) __attribute__((always_inline)) {
-        constexpr bool kNext = decltype(has_next)::value, kAfter = decltype(has_after)::value;
-        if (exact) raise(sc);
+                          const unsigned char* kblock_after, uint32_t vis_next, auto hook, auto has_next, auto has_after, auto mask_next,
+                          auto dealt) __attribute__((always_inline)) {
+        constexpr bool kNext = decltype(has_next)::value, kAfter = decltype(has_after)::value, kDealt = decltype(dealt)::value;
         bf16x8_t kf[KS], vf[NP];
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
@@ -864,6 +872,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
             }
             if (i + PFV >= KS) vf[i + PFV - KS] = v_frag(vblock, i + PFV - KS);
             softmax_slot(sc, i);
+            hook(i);
         }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
@@ -874,71 +883,79 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
             }
             oacc[j % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j], p_frag(j / DB), oacc[j % DB], 0, 0, 0);
             softmax_slot(sc, KS + j);
+            if constexpr (kNext && kDealt) softmax_slot(sn, j - NP);
             if constexpr (kNext && decltype(mask_next)::value) {
                 if (j >= DB) {
 #pragma unroll
                     for (int mi = (j - DB) * 4 / DB; mi < (j - DB + 1) * 4 / DB; ++mi) mask_piece(sn, mi, vis_next);
                 }
             }
+            hook(KS + j);
         }
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kNext && !kDealt) {
+            if (exact) raise(sn);
+            softmax_ahead(sn);
+        }
     };
     const std::true_type yes{};
     const std::false_type no{};
 
     // ---- prologue: keys of KD and values of VD tiles asked for
-    // bits[i]: keys that count in tile t + i.  open_end: tiles in front of this one take no mask, as far as their pages are known
-    uint64_t bits[KD];
-    int64_t v_base[KD - VD];           // of tiles t + VD .., whose keys have been asked for
-    int open_end, kslot, vslot;        // slots: of tile t
-    Pages ahead;
+    int64_t k_base, v_base[KD - VD];   // of tile t + KD; of tiles t + VD .., whose keys have been asked for
+    int kslot, vslot;                  // slots: of tile t
+    auto after = [](int slot, int step, int n) __attribute__((always_inline)) { return slot + step < n ? slot + step : slot + step - n; };
+    auto tidy = [&](int t, int slot) __attribute__((always_inline)) {
+        const uint64_t bits = counted(t);
+        if (!open_tile(t, bits)) clean(slot, bits);
+    };
     auto begin = [&]() __attribute__((always_inline)) {
         open_end = min(t1, s.ctx / KT);
         kslot = vslot = 0;
-        Pages g[KD];
-#pragma unroll
-        for (int i = 0; i < KD; ++i) g[i] = page_ids(t0 + i);
+        fill(t0);
 #pragma unroll
         for (int i = 0; i < KD; ++i) {
-            const int64_t base = base_of(t0 + i, g[i]);
-            copy_k(base, i);
-            if (i < VD) copy_v(base, i);
-            else v_base[i - VD] = base;
-            bits[i] = counted(t0 + i, g[i]);
-        }
+            const int64_t base = base_of(t0 + i);
 #pragma unroll
-        for (int i = KD - 1; i >= 0; --i)
-            if (bits[i] != ~0ull) open_end = min(open_end, t0 + i);
-        ahead = page_ids(t0 + KD);
+            for (int n = 0; n < NI; ++n) copy_k(base, i, n);
+            if (i < VD) {
+#pragma unroll
+                for (int n = 0; n < NI; ++n) copy_v(base, i, n);
+            } else {
+                v_base[i - VD] = base;
+            }
+        }
         // (the query rows' loads are waited for with the first tiles)
         wait_landed<(KD - 2) * NI + (VD - 1) * NI>();
-        if (!open_tile(t0, bits[0])) clean(0, bits[0]);
+        if (t0 >= open_end) tidy(t0, 0);
         __syncthreads();
     };
-    auto after = [](int slot, int step, int n) __attribute__((always_inline)) { return slot + step < n ? slot + step : slot + step - n; };
-    // K(t + KD) and V(t + VD) into the slots that K(t - 1) and V(t - 1) left, page numbers of the tile behind
-    auto request = [&](int t) __attribute__((always_inline)) {
-        const int64_t base = base_of(t + KD, ahead);
-        copy_k(base, after(kslot, KD, KD + 1));
-        copy_v(v_base[0], after(vslot, VD, VD + 1));
+    // V(t + VD) and K(t + KD) into the slots that V(t - 1) and K(t - 1) left, in 2 NI pieces (values first, they are due first: 16 rows of 8191 keys, 64 nodes
+    // of 8B heads 189 -> 185 us); in front of them the pages of the tiles to come
+    auto look_ahead = [&](int t) __attribute__((always_inline)) {
+        if (t + KD - tb > 63) fill(t);
+    };
+    auto request = [&](int t, int i) __attribute__((always_inline)) {
+        if (i < NI) copy_v(v_base[0], after(vslot, VD, VD + 1), i);
+        if (i == NI - 1) {
+            k_base = base_of(t + KD);
 #pragma unroll
-        for (int i = 0; i + 1 < KD - VD; ++i) v_base[i] = v_base[i + 1];
-        v_base[KD - VD - 1] = base;
-        const uint64_t last = counted(t + KD, ahead);
-        if (last != ~0ull) open_end = min(open_end, t + KD);
-        ahead = page_ids(t + KD + 1);
-        return last;
+            for (int n = 0; n + 1 < KD - VD; ++n) v_base[n] = v_base[n + 1];
+            v_base[KD - VD - 1] = k_base;
+        }
+        if (i >= NI && i < 2 * NI) copy_k(k_base, after(kslot, KD, KD + 1), i - NI);
     };
     // the end of a tile: K(t + 2) and V(t + 1) have landed (what was asked for since the tile before may be on its way), values cleaned if need be
-    auto turn = [&](int t, uint64_t last, bool masks) __attribute__((always_inline)) {
-        wait_landed<(KD - 2) * NI + (VD - 1) * NI>();
+    auto turn = [&](int t, auto masks) __attribute__((always_inline)) {
         vslot = after(vslot, 1, VD + 1);
         kslot = after(kslot, 1, KD + 1);
-        if (masks && !open_tile(t + 1, bits[1])) clean(vslot, bits[1]);
-#pragma unroll
-        for (int i = 0; i + 1 < KD; ++i) bits[i] = bits[i + 1];
-        bits[KD - 1] = last;
-        __syncthreads();
+        if constexpr (decltype(masks)::value) {
+            wait_landed<(KD - 2) * NI + (VD - 1) * NI>();
+            if (t + 1 >= open_end) tidy(t + 1, vslot);
+            __syncthreads();
+        } else {       // (a __syncthreads would wait for the next block's keys too, which nobody overwrites)
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((KD - 2) * NI + (VD - 1) * NI) : "memory");
+        }
     };
     // behind the last tile: whether any wave left a value out (1), and whether any row left the safe range (2).  The word is the ring's first, which
     // nothing reads or writes any more
@@ -958,8 +975,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
         for (int pass = 0; pass < 2; ++pass) {
             begin();
             for (int t = t0; t + 1 < t1; ++t) {
-                const uint64_t last = request(t);
-                turn(t, last, true);
+                look_ahead(t);
+#pragma unroll
+                for (int i = 0; i < 2 * NI; ++i) request(t, i);
+                turn(t, yes);
             }
             if (!(report(false) & 2)) break;
         }
@@ -969,27 +988,31 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
     auto mine = [&](uint64_t keys) __attribute__((always_inline)) -> uint64_t { return KW == 1 ? keys : keys >> (32 * kh) & 0xffffffffull; };
 
     f32x16_t s0, s1;
+    auto nothing = [](int) {};
     auto tile_step = [&](int t, auto masks) __attribute__((always_inline)) {
         constexpr bool kMask = decltype(masks)::value;
+        std::integral_constant<bool, !kMask> dealt;
+        look_ahead(t);
         const unsigned char *kcur = kring + kslot * TB, *knext = kring + after(kslot, 1, KD + 1) * TB, *vcur = vring + vslot * TB;
-        const uint64_t last = request(t);
         uint32_t vis1 = 0, vis2 = 0;
         if constexpr (kMask) {
-            const uint64_t here = mine(visible(t, bits[0])), there = mine(visible(t + 1, bits[1]));
+            const uint64_t here = mine(visible(t, counted(t))), there = mine(visible(t + 1, counted(t + 1)));
             saw |= (here | there) != 0;
             vis1 = (uint32_t)(here >> 32) >> (4 * hi);
             vis2 = (uint32_t)there >> (4 * hi);
         }
+        auto asks = [&](int i) __attribute__((always_inline)) { request(t, i); };
+        static_assert(NS >= 2 * NI, "a request a slot");
         if constexpr (KW == 1) {
-            block_step(s0, s1, kcur + 32 * RB, vcur, knext, vis1, yes, yes, masks);
-            block_step(s1, s0, knext, vcur + 32 * RB, knext + 32 * RB, vis2, yes, yes, masks);
+            block_step(s0, s1, kcur + 32 * RB, vcur, knext, vis1, asks, yes, yes, masks, dealt);
+            block_step(s1, s0, knext, vcur + 32 * RB, knext + 32 * RB, vis2, nothing, yes, yes, masks, dealt);
         } else {
 #pragma unroll
             for (int k = 0; k < PF; ++k) kpre[k] = k_frag(knext + kh * 32 * RB, k);
-            block_step(s0, s1, knext + kh * 32 * RB, vcur + kh * 32 * RB, nullptr, vis2, yes, no, masks);
+            block_step(s0, s1, knext + kh * 32 * RB, vcur + kh * 32 * RB, nullptr, vis2, asks, yes, no, masks, dealt);
             s0 = s1;
         }
-        turn(t, last, kMask);
+        turn(t, masks);
     };
     int flags;
     while (true) {
@@ -1004,28 +1027,32 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeArgs a) {
         for (int i = 0; i < 16; ++i) s0[i] = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(kring + kh * 32 * RB, k), qf[k], s0, 0, 0, 0);
-        const uint64_t first = mine(visible(t0, bits[0]));
+        const uint64_t first = mine(visible(t0, counted(t0)));
         saw = first != 0;
 #pragma unroll
         for (int mi = 0; mi < 4; ++mi) mask_piece(s0, mi, (uint32_t)first >> (4 * hi));
-        if (!exact) {
+        if (exact) {
+            raise(s0);
+        } else {
             mrun = block_max(s0);
             if (!(fabsf(mrun) <= 3.4028235e38f)) mrun = 0.f;      // nothing seen yet
         }
+        softmax_ahead(s0);
         if constexpr (KW == 1) {
 #pragma unroll
             for (int k = 0; k < PF; ++k) kpre[k] = k_frag(kring + 32 * RB, k);
         }
         int t = t0;
-        for (; t + 1 < open_end; ++t) tile_step(t, no);
+        if (!exact)
+            for (; t + 1 < open_end; ++t) tile_step(t, no);
         for (; t + 1 < t1; ++t) tile_step(t, yes);
         if constexpr (KW == 2) {
-            block_step(s0, s1, nullptr, vring + vslot * TB + kh * 32 * RB, nullptr, 0, no, no, no);
+            block_step(s0, s1, nullptr, vring + vslot * TB + kh * 32 * RB, nullptr, 0, nothing, no, no, no, no);
         } else {   // the last tile: nothing follows its second block
-            const uint32_t vis1 = (uint32_t)(visible(t, bits[0]) >> 32) >> (4 * hi);
+            const uint32_t vis1 = (uint32_t)(visible(t, counted(t)) >> 32) >> (4 * hi);
             const unsigned char *kcur = kring + kslot * TB, *vcur = vring + vslot * TB;
-            block_step(s0, s1, kcur + 32 * RB, vcur, nullptr, vis1, yes, no, yes);
-            block_step(s1, s0, kcur, vcur + 32 * RB, nullptr, 0, no, no, no);
+            block_step(s0, s1, kcur + 32 * RB, vcur, nullptr, vis1, nothing, yes, no, yes, no);
+            block_step(s1, s0, kcur, vcur + 32 * RB, nullptr, 0, nothing, no, no, no, no);
         }
         bool bad = false;
         if (!exact) {
