@@ -1210,10 +1210,10 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
 // Where few workgroups have short rows, latency counts: a workgroup of 16 stacked rows is the quickest through its keys, and as many of them as the chip
 // has units ask for the same keys again out of L2.  Past `reach` (workgroups times keys) that traffic is what they take, and a workgroup takes more rows:
 // 32, then 64 (heads of 64), then the wide form.  In us, 16 rows a workgroup, 32, wide, each with the splits that it gets:
-//   32 heads of 64 on 4     1 row of 600, 64 nodes 8.2, 10.7, 16.4; 4 rows of 1200, 32 nodes 11.1, 14.1, 22.9; 64 nodes 17.1, 14.8, 23.0; of 5000, 16 nodes
-//                           21.5, 19.9, 21.5; 64 nodes 54, 43, 34; 32 rows of 1200, 8 nodes 17.1, 15.5, 20.1
-//   32 heads of 128 on 8    1 row of 600, 64 nodes 12.8, 16.0, 22.1; 1200 17.0, 18.5, 22.5; 2500 23.4, 22.0, 22.8; 4 rows of 1200, 32 nodes 17.8, 20.7,
-//                           25.8; 64 nodes 24, 21, 29; 2500 47, 38, 32; 16 rows of 1200, 16 nodes 25.9, 21.9, 27.5
+//   32 heads of 64 on 4     1 row of 600, 64 nodes 8.2, 10.7, 16.4; 4 rows of 1200, 32 nodes 11.1, 14.2, 20.3; 64 nodes 17.1, 14.7, 20.7; of 5000, 16 nodes
+//                           21.5, 20.0, 19.9; 64 nodes 54, 44, 32; 32 rows of 1200, 8 nodes 17.1, 15.5, 20.1
+//   32 heads of 128 on 8    1 row of 600, 64 nodes 12.8, 16.0, 22.1; 1200 17.0, 18.4, 21.3; 2500 23.4, 22.0, 21.8; 4 rows of 1200, 32 nodes 17.8, 20.6,
+//                           24.7; 64 nodes 24, 21, 28; 2500 47, 38, 30; 16 rows of 1200, 16 nodes 25.9, 21.9, 26.7
 // Where every other form has passed its reach: 64 rows a workgroup for heads of 64 (32 rows of 4096, 8 nodes 34.5, wide 36.9), else wide; 32 rows of heads of
 // 128 in the narrow form (107, wide 120).  fp32, whose blocks are bound by their matrix instructions, 16 or 32 rows by the same rule (4 rows of 2500, 16 heads
 // of 64 on 4, 16 nodes 18.4, 21.7; 64 nodes of heads of 128 75, 66).
@@ -1231,7 +1231,7 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     const bool few = max_keys <= 1536;
     if (f32) f.row_tiles = stacked <= 16 || fits(1, num_cus(), 400000) ? 1 : 2;
     else if (stacked <= 16 || fits(1, num_cus(), few ? 400000 : d == 64 ? 200000 : 250000)) f.row_tiles = 1;
-    else if (stacked <= 32 || fits(2, num_cus(), few ? 400000 : 350000)) f.row_tiles = 2;
+    else if (stacked <= 32 || fits(2, num_cus(), few ? 400000 : 250000)) f.row_tiles = 2;
     else f.row_tiles = 4, f.wide = d == 128 || stacked > 64;
     f.row_part = f.wide ? (stacked <= 64 ? 64 : 128) : 16 * f.row_tiles;
     f.row_blocks = (int)((stacked + f.row_part - 1) / f.row_part);
