@@ -64,7 +64,7 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int b) {
 // How many of the launch's splits a row of `total` keys takes.  A piece of work is a round (round_keys keys of up to row_part stacked rows of one
 // key/value head); rows are cut so that no split has more than its share of the step's rounds over `slots` workgroups: where rows differ in
 // length the long ones take more splits, and where there are rounds enough for every slot none is cut.  Nor is any where the longest row is no more than
-// a compute unit's share of all (two workgroups run on one: 32 rows of 4096 to 8192 keys, 64 nodes of 8B heads, cut to their shares 277 us, whole 245).  In
+// a compute unit's share of all (two workgroups run on one: 32 rows of 4096 to 8192 keys, 64 nodes of 8B heads, cut to their shares 265 us, whole 246).  In
 // two halves, what a lane counts (its loads go out with a kernel's first) and their sums; all lanes of a wave call them together.
 struct TreeWork {
     int rounds, longest;
@@ -1267,7 +1267,7 @@ int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, in
     // (as many as the kernels may want: they cut a row in fewer where its keys or the step's rows do not ask for them)
     const int64_t units = (int64_t)rows * hkv * f.row_blocks, most = ((int64_t)max_keys + f.round_keys * f.least - 1) / (f.round_keys * f.least);
     // Rows enough for every slot are cut for the sake of long ones among short ones, where the longest that the table has room for would last: what is
-    // not cut is 7 to 15 % quicker where the rows are alike (64 rows of 2048, 8 nodes 64, 69; 512 rows, 2 nodes 432, 498).  fp32: one workgroup a unit is
+    // not cut is 7 to 15 % quicker where the rows are alike (64 rows of 2048, 8 nodes 64, 69; 512 rows, 2 nodes 432, 475).  fp32: one workgroup a unit is
     // enough (4 rows of 900, 64 nodes, 16 heads of 128 on 4 whole 31, cut 38).
     int64_t splits = units < (f32 ? num_cus() : f.slots) ? (f.slots + units - 1) / units * (rows > 1 ? 2 : 1) : max_keys >= 2048 && max_keys >= 1024 * units / f.slots ? 4 : 1;
     if (rows == 1 && units >= f.slots) splits = 1;
@@ -1354,8 +1354,9 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
         const int groups = 1024 / d;
         int shift = 0;
         while ((4 << shift) < num_splits && (1 << shift) < groups) ++shift;      // (as the kernel at most)
-        // (rows that are not cut leave at once, but a workgroup that leaves has asked for lengths too: no more of them than twice what the chip holds)
-        const int64_t most = ((int64_t)max_nodes * hq + (groups >> shift) - 1) / (groups >> shift), fair = (16 * num_cus() + rows - 1) / rows;
+        // (rows that are not cut leave at once, but a workgroup that leaves has asked for lengths too: no more of them than the chip holds: 8 rows of 8191
+        // keys, 48 nodes, 8 heads of 128 on 1 33.8 us, with twice as many 35.5)
+        const int64_t most = ((int64_t)max_nodes * hq + (groups >> shift) - 1) / (groups >> shift), fair = (8 * num_cus() + rows - 1) / rows;
         const dim3 g2((unsigned)(most < fair ? most : fair), (unsigned)rows);
         if (f32 && d == 64) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 64>), g2, dim3(256), 0, s, a);
         else if (f32) hipLaunchKernelGGL((tree_attn_merge_kernel<true, 128>), g2, dim3(256), 0, s, a);
