@@ -47,7 +47,9 @@ struct TreePlace {
 };
 __device__ __forceinline__ TreePlace tree_place(const TreeArgs& a) {
     const unsigned place = blockIdx.z * gridDim.x + blockIdx.x, row = place / (unsigned)a.hkv, split = row / (unsigned)a.rows;
-    return {(int)split, (int)blockIdx.y, (int)(place - row * a.hkv), (int)(row - split * a.rows)};
+    unsigned b = row - split * a.rows;
+    if (split > 0) b = (b + split) % (unsigned)a.rows;      // a row's splits on different XCDs (8 uneven rows, 48 nodes of one key/value head 37 -> 31 us)
+    return {(int)split, (int)blockIdx.y, (int)(place - row * a.hkv), (int)b};
 }
 
 struct TreeSpan {
