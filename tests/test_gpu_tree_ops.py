@@ -267,6 +267,22 @@ def test_splits_that_keys_do_not_fill(ops, hq, n, d, ctx):
             case.check(run_attn(ops, case, splits, cols=cols), f"splits {splits} columns {cols}", want)
 
 
+@pytest.mark.parametrize("hq,n,d", [(8, 17, 64), (8, 17, 128), (8, 8, 128), (2, 3, 128), (8, 8, 64)])
+@pytest.mark.parametrize("page", [16, 32, 64, 256])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_thousands_of_keys_in_one_piece(ops, hq, n, d, page, dtype):
+    """More keys than the page numbers that a wave holds at a time (64 tiles of 64), with holes in the table on either side, and non-finite values there."""
+    case = AttnCase([8500, 4100], [n, 2], hq, 1, d, page, dtype, seed=page + n)
+    for key in (4090, 4200, 8300):
+        case.table[0][key // page] = -1
+    used = {p for row in case.table for p in row}
+    for p in set(range(case.pages)) - used:
+        case.v[p], case.k[p] = float("nan"), float("inf")
+    want = case.reference()
+    for splits in (1, 2, 0):
+        case.check(run_attn(ops, case, splits, cols=MUCH), f"splits {splits}", want)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_attention_of_many_rows(ops, dtype):
     """More rows than a wave has lanes, more than the joining launch has workgroups for one each; some without nodes."""
