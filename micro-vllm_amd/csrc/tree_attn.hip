@@ -392,7 +392,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_f32_kernel(TreeArgs a) {
 }
 
 // ------------------------------------------------------------------ bf16, up to 64 stacked rows (heads of 128: 32)
-// Every wave has keys of its own (32 at a time) and all the rows: nothing is shared until the end, no barrier in the loop.
+// Each of W waves has keys of its own (32 at a time) and all the rows: nothing is shared until the end, no barrier in the loop.
 //   S^T = K . Q^T   v_mfma_f32_16x16x32_bf16, operand A = key rows as they lie in memory (lane (r, q): row r, dimensions 32 k + 8 q ..);
 //   O^T = V^T . P^T operand B = P as S^T left it, rounded to bf16 (keys 4 q + j and 16 + 4 q + j), operand A through the wave's own piece of
 //                   LDS with the transposing read, which delivers those keys.
@@ -404,18 +404,18 @@ __global__ __launch_bounds__(256, 2) void tree_attn_f32_kernel(TreeArgs a) {
 // slower for it, 900 keys 9.1 -> 10.0; with 32 rows registers spill.)
 template <int D, int RT>
 constexpr bool kNarrowTurn = D == 128 && RT == 1;
-template <int D, int RT>
+template <int D, int RT, int W>
 constexpr size_t kNarrowLds = [] {
-    constexpr size_t stage = 4 * 32 * (D * 2 + 32 + (kNarrowTurn<D, RT> ? D * 2 : 0)), merge = 4 * RT * 16 * (D + 4) * sizeof(float);
+    constexpr size_t stage = W * 32 * (D * 2 + 32 + (kNarrowTurn<D, RT> ? D * 2 : 0)), merge = W * RT * 16 * (D + 4) * sizeof(float);
     return stage > merge ? stage : merge;
 }();
 
-template <int D, int RT>
-__global__ __launch_bounds__(256, 2) void tree_attn_narrow_kernel(TreeArgs a) {
-    constexpr int W = 4, KS = D / 32, DT = D / 16, RB = D * 2, VROW = RB + 32, VPR = D / 8, NV = 32 * VPR / 64, OROW = D + 4, ROWS = RT * 16;
+template <int D, int RT, int W>
+__global__ __launch_bounds__(W * 64, 2) void tree_attn_narrow_kernel(TreeArgs a) {
+    constexpr int KS = D / 32, DT = D / 16, RB = D * 2, VROW = RB + 32, VPR = D / 8, NV = 32 * VPR / 64, OROW = D + 4, ROWS = RT * 16;
     constexpr bool TURN = kNarrowTurn<D, RT>;
     static_assert(NV == 2 * KS, "a block's keys are as many pieces either way");
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kNarrowLds<D, RT>];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kNarrowLds<D, RT, W>];
     __shared__ float mL[W][ROWS], lL[W][ROWS];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
     const TreePlace w = tree_place(a);
@@ -600,7 +600,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_narrow_kernel(TreeArgs a) {
     const bool any_odd = __syncthreads_or(odd);
     const bool whole = splits == 1;
 #pragma unroll 1
-    for (int it = threadIdx.x; it < ROWS * (D / 4); it += 256) {
+    for (int it = threadIdx.x; it < ROWS * (D / 4); it += W * 64) {
         const int rr = it / (D / 4), c = it % (D / 4) * 4, sr = row0 + rr;
         if (sr >= stacked) break;
         float top = mL[0][rr];
@@ -1214,13 +1214,13 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
 // 32, then 64 (heads of 64), then the wide form.  In us, 16 rows a workgroup, 32, wide, each with the splits that it gets:
 //   32 heads of 64 on 4     1 row of 600, 64 nodes 8.2, 10.7, 16.4; 4 rows of 1200, 32 nodes 11.1, 14.2, 20.3; 64 nodes 17.1, 14.7, 20.7; of 5000, 16 nodes
 //                           21.5, 20.0, 19.9; 64 nodes 54, 44, 32; 32 rows of 1200, 8 nodes 17.1, 15.5, 20.1
-//   32 heads of 128 on 8    1 row of 600, 64 nodes 12.8, 16.0, 22.1; 1200 17.0, 18.4, 21.3; 2500 23.4, 22.0, 21.8; 4 rows of 1200, 32 nodes 17.8, 20.6,
-//                           24.7; 64 nodes 24, 21, 28; 2500 47, 38, 30; 16 rows of 1200, 16 nodes 25.9, 21.9, 26.7
+//   32 heads of 128 on 8    1 row of 600, 64 nodes 11.3, 15.3, 19.2; 1200 15.0, 18.4, 21.4; 2500 20.9, 21.9, 21.8; 2 rows of 1900 20.5, 24.2, 23.0; 4 rows of
+//                           1200, 32 nodes 15.7, 20.6, 24.7; 64 nodes 29, 21, 27; 2500 57, 38, 30; 16 rows of 1200, 16 nodes 31.7, 21.9, 26.5
 // Where every other form has passed its reach: 64 rows a workgroup for heads of 64 (32 rows of 4096, 8 nodes 34.5, wide 36.9), else wide; 32 rows of heads of
 // 128 in the narrow form (107, wide 120).  fp32, whose blocks are bound by their matrix instructions, 16 or 32 rows by the same rule (4 rows of 2500, 16 heads
 // of 64 on 4, 16 nodes 18.4, 21.7; 64 nodes of heads of 128 75, 66).
 struct TreeForm {
-    int row_tiles, row_part, row_blocks, round_keys, wide, per_unit, slots, least;
+    int row_tiles, row_part, row_blocks, round_keys, wide, waves, per_unit, slots, least;
 };
 static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f32, int64_t max_keys) {
     const int64_t stacked = (int64_t)max_nodes * g, heads = (int64_t)rows * hkv;
@@ -1230,14 +1230,17 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     };
     TreeForm f;
     f.wide = 0;
-    const bool few = max_keys <= 1536;
+    const bool few = max_keys <= (d == 64 ? 1536 : 2304);
     if (f32) f.row_tiles = stacked <= 16 || fits(1, num_cus(), 400000) ? 1 : 2;
-    else if (stacked <= 16 || fits(1, num_cus(), few ? 400000 : d == 64 ? 200000 : 250000)) f.row_tiles = 1;
-    else if (stacked <= 32 || fits(2, num_cus(), few ? 400000 : 250000)) f.row_tiles = 2;
+    else if (stacked <= 16 || fits(1, num_cus(), d == 64 ? few ? 400000 : 200000 : few ? 600000 : 250000)) f.row_tiles = 1;
+    else if (stacked <= 32 || fits(2, num_cus(), max_keys <= 1536 ? 400000 : 250000)) f.row_tiles = 2;
     else f.row_tiles = 4, f.wide = d == 128 || stacked > 64;
     f.row_part = f.wide ? (stacked <= 64 ? 64 : 128) : 16 * f.row_tiles;
     f.row_blocks = (int)((stacked + f.row_part - 1) / f.row_part);
-    f.round_keys = f.wide || f32 ? 64 : 128;
+    // (16 rows of heads of 128: what a compute unit has on its way is what it gets through; eight waves have twice as much.  8 heads of 128 on 1, 16 nodes, four
+    // and eight: 45 keys 6.4, 6.7; 300 8.9, 8.3; 2500 in one piece 26.5, 21.5; one row of 4096 of 32 on 8 17.2, 15.9.  Heads of 64 gain nothing)
+    f.waves = !f32 && !f.wide && d == 128 && f.row_tiles == 1 && max_keys > 256 ? 8 : 4;
+    f.round_keys = f.wide || f32 ? 64 : 32 * f.waves;
     // Work for one workgroup a unit, or for two where there are two without any cut (wide, us with one and two: 32 uneven rows of 256 to 8191, 64
     // nodes of 8B heads 203, 199; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4;
     // fp32 of much work, 4 rows of 6000, 64 nodes, 16 heads of 64 on 4 84, 76, of less one row of 3000, 16 nodes 12.9, 14.4, heads of 128 16.5, 19.5)
@@ -1266,6 +1269,9 @@ int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, in
     // one row of 1200, 64 nodes whole 10.7, cut 12.5, of 2500 17.3, 16.0; heads of 128 of 600 14.4, 15.8, of 1200, 16 nodes 18.3,
     // 14.4; fp32, 8 heads of 64 of 300 8.3, 10.1, of 600 12.1, 10.6)
     if (max_keys <= (f32 ? 512 : d == 64 ? 1536 : 1024)) return 1;
+    // (nor rows that workgroups of eight waves are through with soon, of which there is one for every other unit: 4 rows of 1200, 16 nodes of 8B heads 14.6,
+    // 17.3; 2 rows of 1900, 64 nodes 20.5, 27.0)
+    if (f.waves == 8 && 2 * (int64_t)rows * hkv * f.row_blocks >= num_cus() && max_keys <= 2304) return 1;
     // (as many as the kernels may want: they cut a row in fewer where its keys or the step's rows do not ask for them)
     const int64_t units = (int64_t)rows * hkv * f.row_blocks, most = ((int64_t)max_keys + f.round_keys * f.least - 1) / (f.round_keys * f.least);
     // Rows enough for every slot are cut for the sake of long ones among short ones, where the longest that the table has room for would last: what is
@@ -1338,7 +1344,7 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     if (high > 65535 || rows > 65535) return MV_ERR_UNSUPPORTED;
     hipStream_t s = (hipStream_t)stream;
     const dim3 g1((unsigned)together, (unsigned)a.row_blocks, (unsigned)high);
-#define MV_TREE(K_) hipLaunchKernelGGL((K_), g1, dim3(256), 0, s, a)
+#define MV_TREE(K_) hipLaunchKernelGGL((K_), g1, dim3((unsigned)f.waves * 64), 0, s, a)
     if (f32 && d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_f32_kernel<64, 1>));
     else if (f32 && d == 64) MV_TREE((tree_attn_f32_kernel<64, 2>));
     else if (f32 && f.row_tiles == 1) MV_TREE((tree_attn_f32_kernel<128, 1>));
@@ -1346,11 +1352,12 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     else if (f.wide && d == 64) MV_TREE((tree_attn_wide_kernel<64, 1>));      // (64 rows of such heads: the narrow form)
     else if (f.wide && f.row_part == 64) MV_TREE((tree_attn_wide_kernel<128, 2>));
     else if (f.wide) MV_TREE((tree_attn_wide_kernel<128, 1>));
-    else if (d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<64, 1>));
-    else if (d == 64 && f.row_tiles == 2) MV_TREE((tree_attn_narrow_kernel<64, 2>));
-    else if (d == 64) MV_TREE((tree_attn_narrow_kernel<64, 4>));
-    else if (f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<128, 1>));
-    else MV_TREE((tree_attn_narrow_kernel<128, 2>));
+    else if (d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<64, 1, 4>));
+    else if (d == 64 && f.row_tiles == 2) MV_TREE((tree_attn_narrow_kernel<64, 2, 4>));
+    else if (d == 64) MV_TREE((tree_attn_narrow_kernel<64, 4, 4>));
+    else if (f.row_tiles == 1 && f.waves == 8) MV_TREE((tree_attn_narrow_kernel<128, 1, 8>));
+    else if (f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<128, 1, 4>));
+    else MV_TREE((tree_attn_narrow_kernel<128, 2, 4>));
 #undef MV_TREE
     if (num_splits > 1) {
         const int groups = 1024 / d;
