@@ -1220,7 +1220,7 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
 // 128 in the narrow form (107, wide 120).  fp32, whose blocks are bound by their matrix instructions, 16 or 32 rows by the same rule (4 rows of 2500, 16 heads
 // of 64 on 4, 16 nodes 18.4, 21.7; 64 nodes of heads of 128 75, 66).
 struct TreeForm {
-    int row_tiles, row_part, row_blocks, round_keys, wide, waves, per_unit, slots, least;
+    int row_tiles, row_part, row_blocks, round_keys, wide, waves, whole, per_unit, slots, least;
 };
 static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f32, int64_t max_keys) {
     const int64_t stacked = (int64_t)max_nodes * g, heads = (int64_t)rows * hkv;
@@ -1239,7 +1239,10 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     f.row_blocks = (int)((stacked + f.row_part - 1) / f.row_part);
     // (16 rows of heads of 128: what a compute unit has on its way is what it gets through; eight waves have twice as much.  8 heads of 128 on 1, 16 nodes, four
     // and eight: 45 keys 6.4, 6.7; 300 8.9, 8.3; 2500 in one piece 26.5, 21.5; one row of 4096 of 32 on 8 17.2, 15.9.  Heads of 64 gain nothing)
-    f.waves = !f32 && !f.wide && d == 128 && f.row_tiles == 1 && max_keys > 256 ? 8 : 4;
+    // So have 32 rows of heads of 64 that are not cut (below): 4 rows of 1200, 64 nodes 15.0, 13.8; cut they are slower for it, 16 nodes of 2500 15.5, 16.8.
+    const bool half = 2 * heads * f.row_blocks >= num_cus();      // a workgroup for every other unit
+    f.waves = !f32 && !f.wide && ((d == 128 && f.row_tiles == 1 && max_keys > 256) || (d == 64 && f.row_tiles == 2 && half && max_keys <= 6144)) ? 8 : 4;
+    f.whole = f.waves == 8 && half && max_keys <= (d == 64 ? 6144 : 2304);
     f.round_keys = f.wide || f32 ? 64 : 32 * f.waves;
     // Work for one workgroup a unit, or for two where there are two without any cut (wide, us with one and two: 32 uneven rows of 256 to 8191, 64
     // nodes of 8B heads 203, 199; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4;
@@ -1270,14 +1273,14 @@ int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, in
     // 14.4; fp32, 8 heads of 64 of 300 8.3, 10.1, of 600 12.1, 10.6)
     if (max_keys <= (f32 ? 512 : d == 64 ? 1536 : 1024)) return 1;
     // (nor rows that workgroups of eight waves are through with soon, of which there is one for every other unit: 4 rows of 1200, 16 nodes of 8B heads 14.6,
-    // 17.3; 2 rows of 1900, 64 nodes 20.5, 27.0)
-    if (f.waves == 8 && 2 * (int64_t)rows * hkv * f.row_blocks >= num_cus() && max_keys <= 2304) return 1;
+    // 17.3; 2 rows of 1900, 64 nodes 20.5, 27.0; 32 rows of 5000, 4 nodes, 32 heads of 64 on 4 32, 36)
+    if (f.whole) return 1;
     // (as many as the kernels may want: they cut a row in fewer where its keys or the step's rows do not ask for them)
     const int64_t units = (int64_t)rows * hkv * f.row_blocks, most = ((int64_t)max_keys + f.round_keys * f.least - 1) / (f.round_keys * f.least);
     // Rows enough for every slot are cut for the sake of long ones among short ones, where the longest that the table has room for would last: what is
     // not cut is 7 to 15 % quicker where the rows are alike (64 rows of 2048, 8 nodes 64, 69; 512 rows, 2 nodes 432, 475).  fp32: one workgroup a unit is
     // enough (4 rows of 900, 64 nodes, 16 heads of 128 on 4 whole 31, cut 38).
-    int64_t splits = units < (f32 ? num_cus() : f.slots) ? (f.slots + units - 1) / units * (rows > 1 ? 2 : 1) : max_keys >= 2048 && max_keys >= 1024 * units / f.slots ? 4 : 1;
+    int64_t splits = units < (f32 ? num_cus() : f.slots) ? (f.slots + units - 1) / units * (rows > 1 ? 2 : 1) : max_keys >= 4096 && max_keys >= 1024 * units / f.slots ? 4 : 1;
     if (rows == 1 && units >= f.slots) splits = 1;
     if (splits > most) splits = most;
     if (splits > 1 && (int64_t)rows * hkv * splits > 8 * 65535) splits = 1;      // (the grid's third dimension)
@@ -1353,6 +1356,7 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     else if (f.wide && f.row_part == 64) MV_TREE((tree_attn_wide_kernel<128, 2>));
     else if (f.wide) MV_TREE((tree_attn_wide_kernel<128, 1>));
     else if (d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<64, 1, 4>));
+    else if (d == 64 && f.row_tiles == 2 && f.waves == 8) MV_TREE((tree_attn_narrow_kernel<64, 2, 8>));
     else if (d == 64 && f.row_tiles == 2) MV_TREE((tree_attn_narrow_kernel<64, 2, 4>));
     else if (d == 64) MV_TREE((tree_attn_narrow_kernel<64, 4, 4>));
     else if (f.row_tiles == 1 && f.waves == 8) MV_TREE((tree_attn_narrow_kernel<128, 1, 8>));

@@ -297,6 +297,26 @@ def test_attention_of_many_rows(ops, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d,page", [(64, 16), (64, 64), (128, 64)])
+def test_rows_of_up_to_32_heads_and_nodes_in_a_full_launch(ops, dtype, d, page):
+    """Workgroups for half the chip and more with short rows (bf16, heads of 64: eight waves on 32 stacked rows); holes in the table, a node whose key and value are not
+    finite."""
+    rng = np.random.default_rng(page + d)
+    ctx, counts = rng.integers(0, 700, 70).tolist(), rng.integers(0, 9, 70).tolist()
+    counts[0], counts[5] = 8, 8
+    case = AttnCase(ctx, counts, 8, 2, d, page, dtype, seed=page + d, forest=True)
+    for b in (3, 9, 40):
+        case.table[b][0] = -1
+    t = case.starts[5]
+    case.seen = [s - {2} if t <= i < t + 8 else s for i, s in enumerate(case.seen)]
+    p, s = case.table[5][(ctx[5] + 2) // page], (ctx[5] + 2) % page
+    case.k[p, s], case.v[p, s] = float("nan"), float("inf")
+    want = case.reference()
+    for splits in (0, 1, 2, 5):
+        case.check(run_attn(ops, case, splits), f"splits {splits}", want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("hq,d", [(1, 64), (2, 128), (8, 64), (8, 128)])
 @pytest.mark.parametrize("cols", [0, MUCH])
 def test_a_query_that_is_not_finite_is_its_own(ops, dtype, hq, d, cols):
