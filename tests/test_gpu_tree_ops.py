@@ -316,6 +316,25 @@ def test_rows_of_up_to_32_heads_and_nodes_in_a_full_launch(ops, dtype, d, page):
         case.check(run_attn(ops, case, splits), f"splits {splits}", want)
 
 
+@pytest.mark.parametrize("page", [16, 64])
+def test_64_heads_and_nodes_in_one_workgroup_a_unit(ops, page):
+    """26 rows on eight key/value heads of 128: workgroups of 64 stacked rows for most of the chip and no more than it has; rows that rise, a hole, a value
+    that is not finite."""
+    rng = np.random.default_rng(page)
+    ctx, counts = rng.integers(0, 300, 26).tolist(), rng.integers(0, 17, 26).tolist()
+    counts[0], ctx[7], counts[7] = 16, 900, 12
+    case = AttnCase(ctx, counts, 32, 8, 128, page, BF16, seed=page, forest=True)
+    case.table[3][0] = -1
+    t = case.starts[7]
+    case.seen = [s - {2} if t <= i < t + 12 else s for i, s in enumerate(case.seen)]
+    p, s = case.table[7][902 // page], 902 % page
+    case.k[p, s], case.v[p, s] = float("nan"), float("inf")
+    case.q[t + 5] *= 40                                    # scores of hundreds: the second pass
+    want = case.reference()
+    for splits in (0, 1, 2):
+        case.check(run_attn(ops, case, splits), f"splits {splits}", want)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("hq,d", [(1, 64), (2, 128), (8, 64), (8, 128)])
 @pytest.mark.parametrize("cols", [0, MUCH])
