@@ -95,7 +95,8 @@ def tree_plan(ctx_lens: torch.Tensor, row_start: torch.Tensor, block_table: torc
 
     ctx_lens [rows] and row_start [rows + 1] int32; max_nodes bounds the nodes of a row (256 where there are parents or a mask, any
     number of them, as of a prompt's portion, otherwise; nodes past it are left alone).  block_table [rows, columns] int32 in place: columns
-    of the cached tokens are kept, the ones that the nodes open get pages of free_pages in row order, free_pages[0] first.  A row whose
+    of the cached tokens are kept, the ones that the nodes open get pages of free_pages in row order, free_pages[0] first, whatever they
+    held (pages of an earlier step's nodes that were not accepted are the caller's to give back first).  A row whose
     pages are not there any more, and every row behind it that needs some, or one that has no columns for them, gets none (taken -1, slots
     -1, its columns untouched).  parents int32 [tokens], None: a chain.  `tokens` (default: those of parents or out) is the number of
     tokens that the outputs hold; `mask` (default: with parents or out, what they have) says whether a mask is wanted."""
