@@ -523,6 +523,7 @@ int mv_tree_accept(const int64_t* tokens, const int64_t* picks, const int32_t* p
     if (max_nodes > kTreeNodes || max_path > kTreeNodes) return MV_ERR_UNSUPPORTED;
     if (rows == 0) return MV_OK;
     if (!row_start || !ctx_lens || !path || !ids || !counts || (n_tokens > 0 && (!tokens || !picks))) return MV_ERR_INVALID_ARG;
+    if (lens == ctx_lens || ids == tokens || ids == picks) return MV_ERR_INVALID_ARG;      // (other workgroups still read them)
     AcceptArgs a{tokens, picks, parents, row_start, ctx_lens, block_table, bt_stride, bt_cols, rows, n_tokens, max_nodes, max_path, 0,
                  page, num_pages, 0, ids, path, counts, lens, {}};
     if (layers > 0) {

@@ -80,7 +80,7 @@ def test_attention_refuses(nv):
 
 
 def accept(nv, tokens=P, picks=P, parents=P, starts=P, ctx=P, bt=P, stride=8, cols=8, k=(P,), v=(P,), layers=1, row_bytes=256, page=16, pages=20, rows=2,
-           n=9, nodes=8, max_path=8, path=P, ids=P, counts=P, lens=P):
+           n=9, nodes=8, max_path=8, path=FAR, ids=FAR, counts=FAR, lens=FAR):
     import ctypes
     arr = lambda t: None if t is None else (ctypes.c_void_p * len(t))(*t)      # noqa: E731
     return nv.lib().mv_tree_accept(tokens, picks, parents, starts, ctx, bt, stride, cols, arr(k), arr(v), layers, row_bytes, page, pages, rows, n,
@@ -90,7 +90,7 @@ def accept(nv, tokens=P, picks=P, parents=P, starts=P, ctx=P, bt=P, stride=8, co
 def test_accept_refuses(nv):
     bad = [dict(tokens=NULL), dict(picks=NULL), dict(starts=NULL), dict(ctx=NULL), dict(path=NULL), dict(ids=NULL), dict(counts=NULL), dict(bt=NULL),
            dict(k=None), dict(v=None), dict(k=(NULL,)), dict(v=(P + 8,)), dict(rows=-1), dict(n=-1), dict(nodes=-1), dict(max_path=0), dict(layers=-1),
-           dict(page=0), dict(pages=0), dict(row_bytes=0), dict(stride=7)]
+           dict(page=0), dict(pages=0), dict(row_bytes=0), dict(stride=7), dict(lens=P), dict(ids=P)]
     for b in bad:
         assert accept(nv, **b) == nv.MV_ERR_INVALID_ARG, b
     for b in (dict(nodes=257), dict(max_path=257), dict(row_bytes=24)):
