@@ -982,8 +982,8 @@ int mv_qkv_norm_rotary_slots(const void* qkv, int64_t ld, const float* q_norm, c
  * aligned; d 64 or 128, hq / hkv <= 8, page a power of two >= 16, page * bt_cols <= 2^30.  A node that sees nothing: zeros.  Places whose
  * page is not in [0, num_pages) and keys behind column bt_cols do not count; q . k * scale below 2^30 in size (fp32 scores, and the
  * difference to the row's largest is formed from their rounded products).  scale > 0.  out may not share memory with q.  num_splits
- * (1 .. 64) pieces of the keys side by side;
- * workspace: of mv_tree_attn_workspace_bytes, 16-byte aligned, needs no clearing, of one running call at a time. */
+ * (1 .. 64) pieces of the keys side by side; rows < 2^16, rows * hkv * num_splits < 2^19.  workspace: of
+ * mv_tree_attn_workspace_bytes, 16-byte aligned, needs no clearing, of one running call at a time. */
 size_t mv_tree_attn_workspace_bytes(int tokens, int hq, int d, int num_splits);
 /* How many pieces a step should be given (max_keys: the longest row there may be). */
 int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, int max_keys, int f32);

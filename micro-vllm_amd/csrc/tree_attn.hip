@@ -1220,7 +1220,7 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
 // 128 in the narrow form (107, wide 120).  fp32, whose blocks are bound by their matrix instructions, 16 or 32 rows by the same rule (4 rows of 2500, 16 heads
 // of 64 on 4, 16 nodes 18.4, 21.7; 64 nodes of heads of 128 75, 66).
 struct TreeForm {
-    int row_tiles, row_part, row_blocks, round_keys, wide, waves, ahead, whole, per_unit, slots, least;
+    int row_tiles, row_part, row_blocks, round_keys, wide, waves, deep, whole, per_unit, slots, least;
 };
 static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f32, int64_t max_keys) {
     const int64_t stacked = (int64_t)max_nodes * g, heads = (int64_t)rows * hkv;
@@ -1243,13 +1243,11 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     const bool half = 2 * heads * f.row_blocks >= num_cus();      // a workgroup for every other unit
     f.waves = !f32 && !f.wide && ((d == 128 && f.row_tiles == 1 && max_keys > 256) || (d == 64 && f.row_tiles == 2 && half && max_keys <= 6144)) ? 8 : 4;
     f.whole = f.waves == 8 && half && max_keys <= (d == 64 ? 6144 : 2304);
-    // 64 rows of heads of 128 go through a tile in less time than memory answers in: where there is one workgroup a unit or nearly, keys three tiles ahead instead of
-    // two (112 KB of LDS) and rows whole: 32 rows of 4000, 16 nodes of 8B heads 119 -> 103 us, uneven ones 71 -> 65; 24 rows
-    // 97 -> 85, uneven 49 -> 51; 18 uneven ones would be 39 -> 46.  (Of 128 rows the compiler then moves
-    // accumulators between its two files of registers, 17 % slower.)
-    f.ahead = d == 64 ? 4 : 2;
-    if (f.wide && f.row_part == 64 && 4 * heads * f.row_blocks >= 3 * num_cus() && heads * f.row_blocks <= num_cus() && max_keys <= 6144)
-        f.ahead = 3, f.whole = 1;
+    // 64 rows of heads of 128 go through a tile in less time than memory answers in: where there is one workgroup a unit or nearly, keys three tiles ahead
+    // instead of two (112 KB of LDS) and rows whole: 32 rows of 4000, 16 nodes of 8B heads 119 -> 103 us, uneven ones 71 -> 65; 24 rows 97 -> 85, uneven
+    // 49 -> 51; 18 uneven ones would be 39 -> 46.  (With 128 rows the compiler then moves accumulators between its two files of registers, 17 % slower.)
+    f.deep = f.wide && f.row_part == 64 && 4 * heads * f.row_blocks >= 3 * num_cus() && heads * f.row_blocks <= num_cus() && max_keys <= 6144;
+    f.whole |= f.deep;
     f.round_keys = f.wide || f32 ? 64 : 32 * f.waves;
     // Work for one workgroup a unit, or for two where there are two without any cut (wide, us with one and two: 32 uneven rows of 256 to 8191, 64
     // nodes of 8B heads 203, 199; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4;
@@ -1287,7 +1285,8 @@ int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, in
     // Rows enough for every slot are cut for the sake of long ones among short ones, where the longest that the table has room for would last: what is
     // not cut is 7 to 15 % quicker where the rows are alike (64 rows of 2048, 8 nodes 64, 69; 512 rows, 2 nodes 432, 475).  fp32: one workgroup a unit is
     // enough (4 rows of 900, 64 nodes, 16 heads of 128 on 4 whole 31, cut 38).
-    int64_t splits = units < (f32 ? num_cus() : f.slots) ? (f.slots + units - 1) / units * (rows > 1 ? 2 : 1) : max_keys >= 4096 && max_keys >= 1024 * units / f.slots ? 4 : 1;
+    int64_t splits = units < (f32 ? num_cus() : f.slots) ? (f.slots + units - 1) / units * (rows > 1 ? 2 : 1)
+                     : max_keys >= 4096 && max_keys >= 1024 * units / f.slots ? 4 : 1;
     if (rows == 1 && units >= f.slots) splits = 1;
     if (splits > most) splits = most;
     if (splits > 1 && (int64_t)rows * hkv * splits > 8 * 65535) splits = 1;      // (the grid's third dimension)
@@ -1360,7 +1359,7 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
     else if (f32 && f.row_tiles == 1) MV_TREE((tree_attn_f32_kernel<128, 1>));
     else if (f32) MV_TREE((tree_attn_f32_kernel<128, 2>));
     else if (f.wide && d == 64) MV_TREE((tree_attn_wide_kernel<64, 1, 4>));      // (64 rows of such heads: the narrow form)
-    else if (f.wide && f.row_part == 64 && f.ahead == 3) MV_TREE((tree_attn_wide_kernel<128, 2, 3>));
+    else if (f.wide && f.row_part == 64 && f.deep) MV_TREE((tree_attn_wide_kernel<128, 2, 3>));
     else if (f.wide && f.row_part == 64) MV_TREE((tree_attn_wide_kernel<128, 2, 2>));
     else if (f.wide) MV_TREE((tree_attn_wide_kernel<128, 1, 2>));
     else if (d == 64 && f.row_tiles == 1) MV_TREE((tree_attn_narrow_kernel<64, 1, 4>));

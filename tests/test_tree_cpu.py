@@ -66,7 +66,7 @@ def test_attention_refuses(nv):
     for b in bad:
         assert attn(nv, **b) == nv.MV_ERR_INVALID_ARG, b
     for b in (dict(d=96, hq=4, ldq=384, ldo=384), dict(hq=36, ldq=4096, ldo=4096), dict(page=48), dict(page=8), dict(nodes=257, words=4), dict(splits=65),
-              dict(cols=(1 << 26) + 1, stride=1 << 27)):      # (the last: keys past 2^30)
+              dict(cols=(1 << 26) + 1, stride=1 << 27), dict(rows=1 << 16), dict(rows=60000, hq=36, hkv=36, ldq=4096, ldo=4096)):      # keys past 2^30, rows
         assert attn(nv, **b) == nv.MV_ERR_UNSUPPORTED, b
     for b in (dict(out=P), dict(out=P + 16), dict(out=P, ldo=1024), dict(out=P + 256, ldq=640, ldo=640), dict(tokens=1, out=P - 1008)):
         assert attn(nv, **b) == nv.MV_ERR_INVALID_ARG, b          # out over q
