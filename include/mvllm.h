@@ -952,7 +952,7 @@ int mv_layernorm_gather(const float* x, int64_t ldx, const int32_t* idx, const f
  * reference, whose decode step is one token a row.
  *
  * Row b (a sequence) has ctx_lens[b] cached tokens and brings nodes row_start[b] .. row_start[b + 1] - 1 of the step's
- * tokens (at most max_nodes; the rest is left alone).  Node i continues the earlier node parents[.] of its row (anything
+ * tokens (row_start ascends; at most max_nodes: those past it are no nodes).  Node i continues the earlier node parents[.] of its row (anything
  * else: none; parents == NULL: the node in front of it).  It lies in the cache at index ctx_lens[b] + i of the sequence, at position
  * ctx_lens[b] + its depth.  A mask has `words` 64-bit words per token: bit i % 64 of word i / 64 is node i of the row.  Trees and
  * masks go up to 256 nodes a row.  No two rows may share a page that nodes lie in.
@@ -962,7 +962,9 @@ int mv_layernorm_gather(const float* x, int64_t ldx, const int32_t* idx, const f
  * that the nodes open behind those of the cached tokens get free_pages [n_free] in row order.  taken [rows] = pages a row took; -1: the
  * free ones did not last up to this row, or it has no columns for them - it takes none and its slots are -1.  slots [tokens] = page *
  * page size + place (-1 also where the page is not in [0, num_pages)), positions, row_of [tokens]; mask [tokens, words] (NULL:
- * none) = the node and its ancestors.  Without parents and mask rows may be of any length.  page * num_pages < 2^31. */
+ * none) = the node and its ancestors.  Without parents and mask rows may be of any length.  page * num_pages < 2^31.  Of tokens that no row has (in
+ * front of row_start[0], behind row_start[rows], past max_nodes of a row) nothing is written, but that a slot of theirs that is not negative becomes
+ * -1, whatever an earlier step left there: a store of all `tokens` stores the nodes.  rows == 0 writes nothing. */
 int mv_tree_plan(const int32_t* ctx_lens, const int32_t* row_start, const int32_t* parents, int32_t* block_table, int64_t bt_stride,
                  int bt_cols, const int32_t* free_pages, int n_free, int rows, int tokens, int max_nodes, int page, int num_pages,
                  int32_t* slots, int32_t* positions, int32_t* row_of, uint64_t* mask, int words, int32_t* taken, mv_stream_t stream);

@@ -60,7 +60,7 @@ def _mask(m: torch.Tensor, tokens: int, max_nodes: int, dev: int):
 
 
 class TreePlan:
-    """What tree_plan leaves.  Per token: slots (page * page size + place in it, -1: none), positions, rows, mask [tokens, words] int64
+    """What tree_plan leaves.  Per token: slots (page * page size + place in it, negative: none), positions, rows, mask [tokens, words] int64
     (bit i of word i // 64: node i of the row is the token itself or an ancestor; None where no mask was asked for); per row: taken, the
     pages taken off the free list, -1 for a row that did not get its pages.  The buffers are checked once, here."""
     __slots__ = ("_t", "_p", "tokens", "n_rows", "words", "device")
@@ -94,12 +94,14 @@ def tree_plan(ctx_lens: torch.Tensor, row_start: torch.Tensor, block_table: torc
     """The tables of a step from its rows' lengths, on the device: pages for the nodes, slots, positions, rows and ancestor masks.
 
     ctx_lens [rows] and row_start [rows + 1] int32; max_nodes bounds the nodes of a row (256 where there are parents or a mask, any
-    number of them, as of a prompt's portion, otherwise; nodes past it are left alone).  block_table [rows, columns] int32 in place: columns
+    number of them, as of a prompt's portion, otherwise; tokens past it are no nodes).  block_table [rows, columns] int32 in place: columns
     of the cached tokens are kept, the ones that the nodes open get pages of free_pages in row order, free_pages[0] first, whatever they
     held (pages of an earlier step's nodes that were not accepted are the caller's to give back first).  A row whose
     pages are not there any more, and every row behind it that needs some, or one that has no columns for them, gets none (taken -1, slots
     -1, its columns untouched).  parents int32 [tokens], None: a chain.  `tokens` (default: those of parents or out) is the number of
-    tokens that the outputs hold; `mask` (default: with parents or out, what they have) says whether a mask is wanted."""
+    tokens that the outputs hold, which may be more than the rows have: the others' slots are negative afterwards (-1 in place of what an earlier
+    step left), so that a store of all of them stores the nodes, and the rest of their values is left alone.  `mask` (default: with
+    parents or out, what they have) says whether a mask is wanted."""
     rows, dev = ctx_lens.shape[0], _current(ctx_lens)
     if out is None:
         if tokens is None:
@@ -110,6 +112,8 @@ def tree_plan(ctx_lens: torch.Tensor, row_start: torch.Tensor, block_table: torc
         assert (tokens is None or tokens == out.tokens) and out.n_rows == rows and out.device == dev, "out is of another step's sizes"
         assert mask is None or mask == (out.mask is not None)
         tokens = out.tokens
+    if rows == 0 and tokens:
+        out.slots.fill_(-1)      # (the entry point has nothing to launch)
     slots, positions, row_of, m, taken = out._p
     assert m is None or out.words * 64 >= max_nodes, f"{out.words} mask words for {max_nodes} nodes"
     assert max_nodes <= MAX_NODES or (m is None and parents is None), f"trees and masks go up to {MAX_NODES} nodes a row"

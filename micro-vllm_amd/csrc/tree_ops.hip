@@ -14,12 +14,12 @@ constexpr int kTreeNodes = 256;                // nodes of a row with a tree or 
 constexpr int kTreeWords = kTreeNodes / 64;
 
 struct TreeRow {
-    int start, n;
+    int start, n, end;       // end: of all its nodes, n: of those within the bound
 };
 // nodes of row b, kept inside the step's tokens and the caller's bound whatever row_start holds
 __device__ __forceinline__ TreeRow tree_row(const int32_t* row_start, int b, int tokens, int max_nodes) {
     const int s = min(max(row_start[b], 0), tokens), e = min(max(row_start[b + 1], s), tokens);
-    return {s, min(e - s, max_nodes)};
+    return {s, min(e - s, max_nodes), e};
 }
 
 // ------------------------------------------------------------------ plan
@@ -52,6 +52,8 @@ __device__ __forceinline__ PageNeed page_need(const PlanArgs& a, int b) {
 // rows before its own itself: two dependent trips to the caches for any number of rows, where a scan in a launch of its own is a
 // launch.  Ancestors by doubling: a node's bits and its ancestor 2^k steps up; after k + 1 rounds it holds 2^(k + 1) of them, and the
 // rounds end when every pointer has left the tree.
+// The store behind the plan goes by slots alone, so tokens that no row has (in front of the first, behind the last, past a row's bound) may not keep
+// the place that an earlier step's node had: their slot becomes -1, unless it is negative already.
 __global__ __launch_bounds__(256) void tree_plan_kernel(PlanArgs a) {
     __shared__ int64_t red[4];
     __shared__ uint64_t bitsL[kTreeWords][kTreeNodes];
@@ -79,7 +81,16 @@ __global__ __launch_bounds__(256) void tree_plan_kernel(PlanArgs a) {
             for (int64_t j = own.held + tid; j < own.total; j += nt) table[j] = a.free_pages[before + j - own.held];
     }
 
-    const int i = blockIdx.y * nt + tid;
+    const auto none = [&](int64_t t, int64_t end, int64_t step) {
+        for (; t < end; t += step)
+            if (a.slots[t] >= 0) a.slots[t] = -1;
+    };
+    const int i = blockIdx.y * nt + tid, wide = gridDim.y * nt;
+    const int64_t nth = (int64_t)b * wide + i, all = (int64_t)gridDim.x * wide;
+    none(nth, min(max(a.row_start[0], 0), a.tokens), all);
+    none((int64_t)row.start + row.n + i, row.end, wide);
+    none((int64_t)max(a.row_start[a.rows], 0) + nth, a.tokens, all);
+
     int depth = i;
     if (a.mask || a.parents) {       // one chunk holds the row
         int up = -1;

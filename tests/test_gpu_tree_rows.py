@@ -1,0 +1,125 @@
+"""Tokens of a drafted-token step that no row has, and rows that got no pages (core/tree_decode.py): what the plan says of them, and that the
+store, the attention and the acceptance behind it leave everything of other rows as it was."""
+import numpy as np
+import pytest
+import torch
+
+from tree_util import i32, random_parents, starts_of, tables
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import micro_vllm_amd  # noqa: F401
+    from micro_vllm_amd.core import tree_decode
+    return tree_decode
+
+
+def stale_plan(ops, rows, tokens, max_nodes, mask, slots):
+    """A plan's buffers as an earlier step left them: `slots` are places that belong to someone else by now."""
+    out = ops.TreePlan.empty(rows, tokens, max_nodes, DEV, mask=mask)
+    for t in out:
+        if t is not None:
+            t.fill_(3)
+    out.slots.copy_(slots)
+    return out
+
+
+@pytest.mark.parametrize("tree", [True, False])
+@pytest.mark.parametrize("lead,counts,tail,max_nodes", [
+    (0, [3], 1, None), (0, [1], 900, None), (0, [5, 0, 8], 9, None), (4, [5, 7], 0, None), (70, [64, 1], 700, None), (0, [40, 6], 3, 10),
+    (0, [0, 0], 50, 4), (3, [200, 256], 5, 65), (0, [1] * 300, 1000, None)])
+def test_tokens_that_no_row_has_name_no_place(ops, tree, lead, counts, tail, max_nodes):
+    """Tokens in front of the first row, behind the last and past the bound of a row: their slots name no place whatever the buffer held, so
+    the store writes the live tokens' keys and values and nothing else.  Their other values are left alone."""
+    page, hkv, d, hq = 16, 2, 64, 4
+    rng = np.random.default_rng(lead + sum(counts) + tail)
+    bound = max(counts + [1]) if max_nodes is None else max_nodes
+    live_counts = [min(n, bound) for n in counts]
+    ctx = rng.integers(0, 50, len(counts)).tolist()
+    table, pages = tables(ctx, live_counts, page, rng)
+    starts = [lead + s for s in starts_of(counts)]
+    T, first = starts[-1] + tail, pages
+    pages += -(-T // page)                                        # a place of its own for every token of the earlier step
+    stale = first * page + torch.arange(T, dtype=torch.int32)
+    parents = torch.zeros(T, dtype=torch.int32)
+    for b, n in enumerate(counts):
+        parents[starts[b]:starts[b] + n] = random_parents([n], rng)
+    out = stale_plan(ops, len(counts), T, bound, tree, stale)
+    free = [p for b, c in enumerate(ctx) for p in table[b][-(-c // page):-(-(c + live_counts[b]) // page)]]
+    ops.tree_plan(i32(ctx, DEV), i32(starts, DEV), i32(table, DEV), i32(free, DEV), bound, page, pages, parents=parents.to(DEV) if tree else None, out=out)
+    live = {starts[b] + i: table[b][(c + i) // page] * page + (c + i) % page for b, c in enumerate(ctx) for i in range(live_counts[b])}
+    got = out.slots.tolist()
+    assert all(got[t] == s for t, s in live.items())
+    assert all(got[t] < 0 for t in range(T) if t not in live)
+    dead = torch.tensor([t not in live for t in range(T)])
+    assert all((t[dead.to(DEV)] == 3).all() for t in (out.positions, out.rows, out.mask) if t is not None)
+
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn(T, (hq + 2 * hkv) * d, generator=g).to(BF16)
+    k, v = (torch.randn(pages, page, hkv, d, generator=g).to(BF16) for _ in range(2))
+    dk, dv = k.to(DEV), v.to(DEV)
+    ops.qkv_norm_rotary_slots(qkv.to(DEV), out.positions, out.slots, dk, dv, hq)
+    kv = qkv[:, hq * d:].view(T, 2, hkv, d)
+    for t, s in live.items():
+        k[s // page, s % page], v[s // page, s % page] = kv[t, 0], kv[t, 1]
+    assert torch.equal(dk.cpu(), k) and torch.equal(dv.cpu(), v)
+
+
+def test_a_step_without_rows_names_no_place(ops):
+    out = stale_plan(ops, 0, 6, 8, True, torch.arange(6, dtype=torch.int32))
+    none = i32([], DEV)
+    ops.tree_plan(none, i32([0], DEV), torch.zeros(0, 4, dtype=torch.int32, device=DEV), none, 8, 16, 10, parents=torch.zeros(6, dtype=torch.int32, device=DEV),
+                  out=out)
+    assert (out.slots < 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_recorded_step_of_fewer_nodes_each_time(ops, dtype):
+    """A step recorded for 40 tokens, replayed with fewer of them while the cached tokens grow over the places of the step before: each replay
+    leaves the cache as its own nodes' keys and values make it."""
+    rows, hq, hkv, d, page, T, bound, cols = 3, 4, 2, 64, 16, 40, 20, 8
+    pages = rows * cols
+    g = torch.Generator(device=DEV).manual_seed(2)
+    rng = np.random.default_rng(2)
+    table = [list(range(cols * b, cols * (b + 1))) for b in range(rows)]      # column j of row b is page 8 b + j, held or taken
+    ctx, starts, bt, free = i32([0] * rows, DEV), i32([0] * (rows + 1), DEV), i32(table, DEV), i32([-1] * 6, DEV)
+    parents = torch.zeros(T, dtype=torch.int32, device=DEV)
+    qkv = torch.zeros(T, (hq + 2 * hkv) * d, dtype=dtype, device=DEV)
+    k, v = (torch.zeros(pages, page, hkv, d, dtype=dtype, device=DEV) for _ in range(2))
+    plan, q, o = ops.TreePlan.empty(rows, T, bound, DEV), torch.empty(T, hq, d, dtype=dtype, device=DEV), torch.zeros(T, hq, d, dtype=dtype, device=DEV)
+    plan.slots.fill_(-1)
+
+    def go():
+        ops.tree_plan(ctx, starts, bt, free, bound, page, pages, parents=parents, out=plan)
+        ops.qkv_norm_rotary_slots(qkv, plan.positions, plan.slots, k, v, hq, out=q)
+        ops.tree_attn(q, k, v, ctx, starts, bt, plan.mask, bound, out=o)
+
+    go()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        go()
+    lens = [15, 0, 30]
+    for counts in ([17, 20, 3], [9, 1, 11], [1, 0, 1], [0, 0, 0], [2, 16, 0]):
+        at = starts_of(counts)
+        take = [table[b][j] for b in range(rows) for j in range(-(-lens[b] // page), -(-(lens[b] + counts[b]) // page))]
+        ctx.copy_(i32(lens, DEV))
+        starts.copy_(i32(at, DEV))
+        free.copy_(i32(take + [-1] * (6 - len(take)), DEV))
+        parents[:at[-1]] = random_parents(counts, rng).to(DEV)
+        qkv.normal_(generator=g)
+        want_k, want_v, kv = k.clone(), v.clone(), qkv[:, hq * d:].view(T, 2, hkv, d)
+        for b, (c, n) in enumerate(zip(lens, counts)):
+            for i in range(n):
+                p, s = table[b][(c + i) // page], (c + i) % page
+                want_k[p, s], want_v[p, s] = kv[at[b] + i, 0], kv[at[b] + i, 1]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(s < 0 for s in plan.slots[at[-1]:].tolist()) and plan.taken.sum().item() == len(take)
+        assert torch.equal(k, want_k) and torch.equal(v, want_v), counts
+        lens = [c + (n + 1) // 2 for c, n in zip(lens, counts)]
