@@ -960,7 +960,7 @@ int mv_layernorm_gather(const float* x, int64_t ldx, const int32_t* idx, const f
 
 /* Pages, slots, positions, rows and ancestor masks of a step.  block_table [rows, bt_cols] (row stride bt_stride) in place: the columns
  * that the nodes open behind those of the cached tokens get free_pages [n_free] in row order.  taken [rows] = pages a row took; -1: the
- * free ones did not last up to this row, or it has no columns for them - it takes none and its slots are -1.  slots [tokens] = page *
+ * free ones did not last up to this row, or it has no columns for them - it takes none, its slots and the columns that its nodes would open are -1.  slots [tokens] = page *
  * page size + place (-1 also where the page is not in [0, num_pages)), positions, row_of [tokens]; mask [tokens, words] (NULL:
  * none) = the node and its ancestors.  Without parents and mask rows may be of any length.  page * num_pages < 2^31.  Of tokens that no row has (in
  * front of row_start[0], behind row_start[rows], past max_nodes of a row) nothing is written, but that a slot of theirs that is not negative becomes

@@ -98,7 +98,7 @@ def tree_plan(ctx_lens: torch.Tensor, row_start: torch.Tensor, block_table: torc
     of the cached tokens are kept, the ones that the nodes open get pages of free_pages in row order, free_pages[0] first, whatever they
     held (pages of an earlier step's nodes that were not accepted are the caller's to give back first).  A row whose
     pages are not there any more, and every row behind it that needs some, or one that has no columns for them, gets none (taken -1, slots
-    -1, its columns untouched).  parents int32 [tokens], None: a chain.  `tokens` (default: those of parents or out) is the number of
+    -1, and -1 in the columns that its nodes would open, which may hold pages that are another row's by now).  parents int32 [tokens], None: a chain.  `tokens` (default: those of parents or out) is the number of
     tokens that the outputs hold, which may be more than the rows have: the others' slots are negative afterwards (-1 in place of what an earlier
     step left), so that a store of all of them stores the nodes, and the rest of their values is left alone.  `mask` (default: with
     parents or out, what they have) says whether a mask is wanted."""

@@ -77,8 +77,9 @@ __global__ __launch_bounds__(256) void tree_plan_kernel(PlanArgs a) {
     int32_t* table = a.block_table + (int64_t)b * a.bt_stride;
     if (blockIdx.y == 0) {
         if (tid == 0) a.taken[b] = refused ? -1 : (int)own.need();
-        if (!refused)
-            for (int64_t j = own.held + tid; j < own.total; j += nt) table[j] = a.free_pages[before + j - own.held];
+        // (a refused row's columns may name pages that were given back since, and that another row takes here)
+        const int64_t end = min(own.total, (int64_t)a.bt_cols);
+        for (int64_t j = own.held + tid; j < end; j += nt) table[j] = refused ? -1 : a.free_pages[before + j - own.held];
     }
 
     const auto none = [&](int64_t t, int64_t end, int64_t step) {

@@ -35,6 +35,9 @@ def plan(ctx, starts, table, free, page, num_pages, parents=None):
         if ok:
             table[b][held:total] = free[used:used + need]
             used += need
+        else:
+            end = min(total, len(table[b]))
+            table[b][held:end] = [-1] * max(0, end - held)
         taken.append(need if ok else -1)
         for i in range(n):
             up = ancestors(parents, starts[b], i)

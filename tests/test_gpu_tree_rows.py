@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import ref_tree as ref
 from tree_util import i32, random_parents, starts_of, tables
 
 pytestmark = pytest.mark.gpu
@@ -123,3 +124,56 @@ def test_a_recorded_step_of_fewer_nodes_each_time(ops, dtype):
         assert all(s < 0 for s in plan.slots[at[-1]:].tolist()) and plan.taken.sum().item() == len(take)
         assert torch.equal(k, want_k) and torch.equal(v, want_v), counts
         lens = [c + (n + 1) // 2 for c, n in zip(lens, counts)]
+
+
+# ------------------------------------------------------------------------------------------------------- rows without pages
+@pytest.mark.parametrize("page", [1, 16, 64])
+@pytest.mark.parametrize("tree", [True, False])
+def test_a_refused_row_names_no_pages_behind_its_cached_tokens(ops, page, tree):
+    """Columns that hold what earlier steps left: a row that gets pages has those, one that does not (none left, or no columns) has -1 where its nodes
+    would lie, up to the table's end; columns behind the nodes and those of cached tokens stay."""
+    ctx, counts, cols = [page, 3 * page, 2 * page, page, 6 * page], [2 * page, 2 * page, 0, 9 * page, page], 8
+    old = [[100 * b + j for j in range(cols)] for b in range(5)]
+    free = [301, 102, 7]
+    for n_free in range(4):
+        bt = i32(old, DEV)
+        starts = starts_of(counts)
+        parents = random_parents(counts, np.random.default_rng(page)) if tree and max(counts) <= 256 else None
+        plan = ops.tree_plan(i32(ctx, DEV), i32(starts, DEV), bt, i32(free[:n_free], DEV), max(counts), page, 1000,
+                             parents=None if parents is None else parents.to(DEV), tokens=starts[-1])
+        slots, positions, _, _, taken, _ = ref.plan(ctx, starts, old, free[:n_free], page, 1000, parents)
+        want = [list(r) for r in old]
+        want[0][1:3] = free[:2] if n_free >= 2 else [-1, -1]
+        want[1][3:5] = [-1, -1]
+        want[3][1:8] = [-1] * 7                                    # wants ten columns
+        want[4][6] = -1
+        assert bt.tolist() == want and plan.taken.tolist() == taken == [2 if n_free >= 2 else -1, -1, 0, -1, -1]
+        assert plan.slots.tolist() == slots and plan.positions.tolist() == positions
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_refused_row_reads_and_moves_nothing_of_other_rows(ops, dtype):
+    """Row 1 is refused, and the pages its old columns name are row 0's nodes' now: its attention sees its cached tokens alone, and the acceptance leaves row
+    0's nodes where row 0 has them."""
+    page, hq, hkv, d, layers = 16, 4, 2, 64, 3
+    g = torch.Generator().manual_seed(1)
+    ctx, starts = [16, 32], [0, 20, 44]
+    old = [[4, 0, 1, -1], [5, 6, 2, 3]]
+    bt = i32(old, DEV)
+    parents = torch.tensor([i - 1 for i in range(20)] + [-1, 0] + [i - 2 for i in range(2, 24)], dtype=torch.int32)
+    plan = ops.tree_plan(i32(ctx, DEV), i32(starts, DEV), bt, i32([2, 3, 1], DEV), 24, page, 7, parents=parents.to(DEV))
+    assert plan.taken.tolist() == [2, -1] and bt.tolist() == [[4, 2, 3, -1], [5, 6, -1, -1]]
+    k, v = (torch.randn(layers, 7, page, hkv, d, generator=g).to(dtype).to(DEV) for _ in range(2))
+    qkv = torch.randn(44, (hq + 2 * hkv) * d, generator=g).to(dtype).to(DEV)
+    q = ops.qkv_norm_rotary_slots(qkv, plan.positions, plan.slots, k[0], v[0], hq)
+    out = ops.tree_attn(q, k[0], v[0], i32(ctx, DEV), i32(starts, DEV), bt, plan.mask, 24)
+    seen = [set(range(i + 1)) for i in range(20)] + [set() for _ in range(24)]
+    o, mag, size, count = ref.attn(q.cpu(), k[0].cpu(), v[0].cpu(), ctx, starts, bt.tolist(), seen, d ** -0.5)
+    assert ((out.double().cpu() - o).abs() <= ref.attn_bound(o, mag, size, count, d, dtype)).all()
+    tokens = torch.arange(44, device=DEV)
+    picks = torch.full((44,), -1, device=DEV)
+    picks[20:44:2] = torch.arange(22, 46, 2, device=DEV)               # row 1: 0, 2, 4, ..: every node after the first would move
+    picks[0] = 1
+    before_k, before_v = k.clone(), v.clone()
+    ops.tree_accept(tokens, picks, i32(starts, DEV), i32(ctx, DEV), 24, parents=parents.to(DEV), caches=ops.TreeCaches(k, v), block_table=bt)
+    assert torch.equal(k, before_k) and torch.equal(v, before_v)
