@@ -998,11 +998,18 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
  * nodes: path [rows, max_path] (-1 behind its end), ids [rows, max_path] = the picks along it (-1), counts [rows], lens [rows] = ctx_lens +
  * counts (NULL: not wanted; not ctx_lens itself).  layers > 0: then keys and values (row_bytes a token, a multiple of 16, in each of the
  * layers' caches; the addresses are host arrays) at index ctx_lens + path[j] of the sequence go to index ctx_lens + j; places without a page:
- * not.  One launch per 64 layers. */
+ * not.  One launch per 64 layers.  Every row must have got its pages. */
 int mv_tree_accept(const int64_t* tokens, const int64_t* picks, const int32_t* parents, const int32_t* row_start, const int32_t* ctx_lens,
                    const int32_t* block_table, int64_t bt_stride, int bt_cols, void* const* k_caches, void* const* v_caches, int layers,
                    int64_t row_bytes, int page, int num_pages, int rows, int n_tokens, int max_nodes, int max_path, int32_t* path,
                    int64_t* ids, int32_t* counts, int32_t* lens, mv_stream_t stream);
+/* The same for rows that a plan may have refused: taken [rows] as mv_tree_plan leaves it (NULL: every row has its pages).  A row with a negative
+ * entry has no nodes in the cache: an empty path, lens = ctx_lens, nothing moved. */
+int mv_tree_accept_planned(const int64_t* tokens, const int64_t* picks, const int32_t* parents, const int32_t* row_start,
+                           const int32_t* ctx_lens, const int32_t* taken, const int32_t* block_table, int64_t bt_stride, int bt_cols,
+                           void* const* k_caches, void* const* v_caches, int layers, int64_t row_bytes, int page, int num_pages, int rows,
+                           int n_tokens, int max_nodes, int max_path, int32_t* path, int64_t* ids, int32_t* counts, int32_t* lens,
+                           mv_stream_t stream);
 
 #ifdef __cplusplus
 }

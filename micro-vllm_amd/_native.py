@@ -196,6 +196,7 @@ PROTOTYPES = {
     "mv_tree_attn_pick_splits": (_I, [_I, _I, _I, _I, _I, _I, _I]),
     "mv_tree_attn": (_I, [_P, _L, _P, _P, _P, _P, _P, _L, _I, _P, _I, _P, _L, _P, _Z, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P]),
     "mv_tree_accept": (_I, [_P, _P, _P, _P, _P, _P, _L, _I, _P, _P, _I, _L, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P]),
+    "mv_tree_accept_planned": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _I, _P, _P, _I, _L, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P]),
     "mv_graph_begin_capture": (_I, [_P]),
     "mv_graph_end_capture": (_I, [_P, ctypes.POINTER(c_void_p)]),
     "mv_graph_launch": (_I, [_P, _P]),

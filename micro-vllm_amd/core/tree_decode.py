@@ -276,12 +276,13 @@ class TreePath:
 
 def tree_accept(tokens: torch.Tensor, picks: torch.Tensor, row_start: torch.Tensor, ctx_lens: torch.Tensor, max_nodes: int,
                 parents: Optional[torch.Tensor] = None, max_path: Optional[int] = None, caches: Optional[TreeCaches] = None,
-                block_table: Optional[torch.Tensor] = None, out: Optional[TreePath] = None) -> TreePath:
+                block_table: Optional[torch.Tensor] = None, out: Optional[TreePath] = None, taken: Optional[torch.Tensor] = None) -> TreePath:
     """The part of every row's tree that the target model agrees with: from node 0 on to the lowest later node whose parent is the
     current one and whose token (int64 [tokens]) is the target's pick behind it (int64 [tokens]), until there is none or the path has
     max_path nodes (default: out's, else max_nodes).  With `caches` the keys and values of the path's j-th node are moved to index
     ctx_lens[b] + j of the sequence in every layer (places without a page: not moved), which is where a sequence of lens[b] tokens has
-    them; all of it one launch for up to 64 layers.  A row without nodes has an empty path."""
+    them; all of it one launch for up to 64 layers.  A row without nodes has an empty path, and so has one that did not get its pages
+    (`taken`, the plan's, is negative): its nodes are stored nowhere, its length stays.  Without `taken` every row counts as stored."""
     n_tokens, rows, dev = tokens.shape[0], ctx_lens.shape[0], _current(tokens)
     assert max_nodes <= MAX_NODES, f"trees go up to {MAX_NODES} nodes a row"
     if out is None:
@@ -295,7 +296,7 @@ def tree_accept(tokens: torch.Tensor, picks: torch.Tensor, row_start: torch.Tens
     else:
         assert block_table is not None and caches.device == dev, "moving keys and values takes the block table, on the caches' device"
         move = (*_table(block_table, rows, dev), caches.k, caches.v, caches.layers, caches.row_bytes, caches.page, caches.pages)
-    nv.check("mv_tree_accept", nv.lib().mv_tree_accept(
+    nv.check("mv_tree_accept_planned", nv.lib().mv_tree_accept_planned(
         _vec(tokens, n_tokens, dev, _I64), _vec(picks, n_tokens, dev, _I64), None if parents is None else _vec(parents, n_tokens, dev),
-        _vec(row_start, rows + 1, dev), ctx, *move, rows, n_tokens, max_nodes, out.max_path, path, ids, counts, lens, _stream(dev)))
+        _vec(row_start, rows + 1, dev), ctx, None if taken is None else _vec(taken, rows, dev), *move, rows, n_tokens, max_nodes, out.max_path, path, ids, counts, lens, _stream(dev)))
     return out

@@ -356,7 +356,7 @@ __global__ __launch_bounds__(256) void slot_store_kernel(SlotStoreArgs a, int he
 constexpr int kAcceptLayers = 64;      // layers of one launch: their addresses travel in its arguments
 struct AcceptArgs {
     const int64_t *tokens, *picks;
-    const int32_t *parents, *row_start, *ctx, *block_table;
+    const int32_t *parents, *row_start, *ctx, *taken, *block_table;
     int64_t bt_stride;
     int bt_cols, rows, n_tokens, max_nodes, max_path, layers, page, num_pages;
     int row_vecs;                      // 16-byte pieces of one token's keys in a layer
@@ -374,7 +374,8 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(AcceptArgs a) {
     __shared__ int64_t srcL[kTreeNodes], dstL[kTreeNodes];
     __shared__ int countL;
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-    const TreeRow row = tree_row(a.row_start, b, a.n_tokens, a.max_nodes);
+    TreeRow row = tree_row(a.row_start, b, a.n_tokens, a.max_nodes);
+    if (a.taken && a.taken[b] < 0) row.n = 0;      // its nodes were stored nowhere
     const int64_t ctx = max(a.ctx[b], 0);
     if (tid < row.n) pickL[tid] = a.picks[row.start + tid];
     __syncthreads();
@@ -526,17 +527,18 @@ int mv_qkv_norm_rotary_slots(const void* qkv, int64_t ld, const float* q_norm, c
     return check_launch();
 }
 
-int mv_tree_accept(const int64_t* tokens, const int64_t* picks, const int32_t* parents, const int32_t* row_start, const int32_t* ctx_lens,
-                   const int32_t* block_table, int64_t bt_stride, int bt_cols, void* const* k_caches, void* const* v_caches, int layers,
-                   int64_t row_bytes, int page, int num_pages, int rows, int n_tokens, int max_nodes, int max_path, int32_t* path,
-                   int64_t* ids, int32_t* counts, int32_t* lens, mv_stream_t stream) {
+int mv_tree_accept_planned(const int64_t* tokens, const int64_t* picks, const int32_t* parents, const int32_t* row_start,
+                           const int32_t* ctx_lens, const int32_t* taken, const int32_t* block_table, int64_t bt_stride, int bt_cols,
+                           void* const* k_caches, void* const* v_caches, int layers, int64_t row_bytes, int page, int num_pages, int rows,
+                           int n_tokens, int max_nodes, int max_path, int32_t* path, int64_t* ids, int32_t* counts, int32_t* lens,
+                           mv_stream_t stream) {
     using namespace mv;
     if (rows < 0 || n_tokens < 0 || max_nodes < 0 || max_path <= 0 || layers < 0) return MV_ERR_INVALID_ARG;
     if (max_nodes > kTreeNodes || max_path > kTreeNodes) return MV_ERR_UNSUPPORTED;
     if (rows == 0) return MV_OK;
     if (!row_start || !ctx_lens || !path || !ids || !counts || (n_tokens > 0 && (!tokens || !picks))) return MV_ERR_INVALID_ARG;
     if (lens == ctx_lens || ids == tokens || ids == picks) return MV_ERR_INVALID_ARG;      // (other workgroups still read them)
-    AcceptArgs a{tokens, picks, parents, row_start, ctx_lens, block_table, bt_stride, bt_cols, rows, n_tokens, max_nodes, max_path, 0,
+    AcceptArgs a{tokens, picks, parents, row_start, ctx_lens, taken, block_table, bt_stride, bt_cols, rows, n_tokens, max_nodes, max_path, 0,
                  page, num_pages, 0, ids, path, counts, lens, {}};
     if (layers > 0) {
         if (!block_table || !k_caches || !v_caches || bt_cols < 0 || bt_stride < bt_cols || page <= 0 || num_pages <= 0 || row_bytes <= 0)
@@ -560,6 +562,14 @@ int mv_tree_accept(const int64_t* tokens, const int64_t* picks, const int32_t* p
         a.counts = nullptr;
     }
     return MV_OK;
+}
+
+int mv_tree_accept(const int64_t* tokens, const int64_t* picks, const int32_t* parents, const int32_t* row_start, const int32_t* ctx_lens,
+                   const int32_t* block_table, int64_t bt_stride, int bt_cols, void* const* k_caches, void* const* v_caches, int layers,
+                   int64_t row_bytes, int page, int num_pages, int rows, int n_tokens, int max_nodes, int max_path, int32_t* path,
+                   int64_t* ids, int32_t* counts, int32_t* lens, mv_stream_t stream) {
+    return mv_tree_accept_planned(tokens, picks, parents, row_start, ctx_lens, nullptr, block_table, bt_stride, bt_cols, k_caches, v_caches,
+                                  layers, row_bytes, page, num_pages, rows, n_tokens, max_nodes, max_path, path, ids, counts, lens, stream);
 }
 
 }  // extern "C"

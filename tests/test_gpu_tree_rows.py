@@ -177,3 +177,76 @@ def test_a_refused_row_reads_and_moves_nothing_of_other_rows(ops, dtype):
     before_k, before_v = k.clone(), v.clone()
     ops.tree_accept(tokens, picks, i32(starts, DEV), i32(ctx, DEV), 24, parents=parents.to(DEV), caches=ops.TreeCaches(k, v), block_table=bt)
     assert torch.equal(k, before_k) and torch.equal(v, before_v)
+
+
+@pytest.mark.parametrize("layers", [0, 2, 70])
+def test_acceptance_of_rows_that_got_no_pages(ops, layers):
+    """A refused row has an empty path, its old length and nothing moved, in its own half-filled page neither; the rows beside it as without it."""
+    ctx, counts, page, hkv, d = [20, 5, 30, 0], [12, 9, 40, 3], 16, 1, 16
+    rng = np.random.default_rng(layers)
+    starts = starts_of(counts)
+    table, pages = tables(ctx, counts, page, rng)
+    parents = torch.tensor([max(-1, i - 2) for n in counts for i in range(n)], dtype=torch.int32)
+    tokens = torch.arange(starts[-1])
+    picks = torch.cat([tokens[2:], torch.zeros(2, dtype=torch.int64)])             # node i's child is i + 2
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.randn(max(1, layers), pages, page, hkv, d, generator=g).to(BF16) for _ in range(2))
+    for taken in ([1, 0, 3, 1], [-1, 0, 3, 1], [1, -1, -1, 1], [-1, -1, -1, -1]):
+        dk, dv = k.to(DEV), v.to(DEV)
+        got = ops.tree_accept(tokens.to(DEV), picks.to(DEV), i32(starts, DEV), i32(ctx, DEV), 40, parents=parents.to(DEV),
+                              caches=ops.TreeCaches(dk, dv) if layers else None, block_table=i32(table, DEV), taken=i32(taken, DEV))
+        path, ids, n, lens = ref.accept(tokens.tolist(), picks.tolist(), starts, ctx, 40, parents)
+        for b, t in enumerate(taken):
+            if t < 0:
+                path[b], ids[b], n[b], lens[b] = [-1] * 40, [-1] * 40, 0, ctx[b]
+        assert n[3] == (2 if taken[3] >= 0 else 0)
+        assert got.path.tolist() == path and got.ids.tolist() == ids and got.counts.tolist() == n and got.lens.tolist() == lens
+        assert torch.equal(dk.cpu(), ref.move(k, ctx, table, path, n) if layers else k)
+        assert torch.equal(dv.cpu(), ref.move(v, ctx, table, path, n) if layers else v)
+
+
+def test_a_recorded_step_whose_row_is_refused_and_comes_again(ops):
+    """Plan, store, attention and acceptance recorded once.  Replayed with no columns for the second row's nodes it keeps its length and the cache its content;
+    replayed with some it goes on, and all of it is what the eager calls give."""
+    page, hq, hkv, d, T, pages = 16, 4, 2, 64, 30, 12
+    g = torch.Generator(device=DEV).manual_seed(4)
+    starts, bt, free = i32([0, 12, 30], DEV), i32([[0, 3, 2], [1, 2, 3]], DEV), i32([-1, -1, -1, -1], DEV)
+    ctx, parents = i32([10, 16], DEV), i32([max(-1, i - 2) for n in (12, 18) for i in range(n)], DEV)
+    k, v = (torch.randn(1, pages, page, hkv, d, generator=g, device=DEV).to(BF16) for _ in range(2))
+    tokens, qkv = torch.arange(T, device=DEV), torch.randn(T, (hq + 2 * hkv) * d, generator=g, device=DEV).to(BF16)
+    picks = torch.cat([tokens[2:], tokens[:2] - 9])
+    plan, got, caches = ops.TreePlan.empty(2, T, 18, DEV), ops.TreePath.empty(2, 18, DEV), ops.TreeCaches(k, v)
+    q, o = torch.empty(T, hq, d, dtype=BF16, device=DEV), torch.empty(T, hq, d, dtype=BF16, device=DEV)
+
+    def go():
+        ops.tree_plan(ctx, starts, bt, free, 18, page, pages, parents=parents, out=plan)
+        ops.qkv_norm_rotary_slots(qkv, plan.positions, plan.slots, k[0], v[0], hq, out=q)
+        ops.tree_attn(q, k[0], v[0], ctx, starts, bt, plan.mask, 18, out=o)
+        ops.tree_accept(tokens, picks, starts, ctx, 18, parents=parents, caches=caches, block_table=bt, out=got, taken=plan.taken)
+
+    state = (bt, k, v)
+    begin = [t.clone() for t in state]
+    go()
+    for t, b in zip(state, begin):
+        t.copy_(b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        go()
+    for turn, cols in enumerate(([[0, 3, 2], [1, 2, 3]], [[0, 7, 2], [1, 8, 9]])):
+        results = []
+        for run in (graph.replay, go):
+            for t, b in zip(state, begin):
+                t.copy_(b)
+            bt.copy_(i32(cols, DEV))
+            free.copy_(i32([7, 8, 9, 10], DEV))
+            ctx.copy_(i32([10, 16 if turn else 16 + 32], DEV))          # (a row without columns for its nodes, then the same row with them)
+            torch.cuda.synchronize()
+            run()
+            torch.cuda.synchronize()
+            results.append([t.clone() for t in (*plan, *got, bt, k, v)])
+        assert all(torch.equal(a, b) for a, b in zip(*results)), turn
+        assert plan.taken.tolist() == ([1, 2] if turn else [1, -1])
+        assert got.counts.tolist() == ([6, 9] if turn else [6, 0]) and got.lens.tolist() == ([16, 25] if turn else [16, 48])
+        if turn == 0:
+            assert torch.equal(k[0, 1:7], begin[1][0, 1:7]) and torch.equal(k[0, 8:], begin[1][0, 8:])      # pages 0 and 7 are row 0's

@@ -144,3 +144,18 @@ def test_oracle_plan_by_hand():
     slots, pos, rows, seen, taken, table = ref.plan([5, 3], [0, 4, 7], [[2, -1], [7, -1]], [9, 4], 4, 20, parents)
     assert taken == [-1, 1] and slots[:4] == [-1] * 4 and slots[4:] == [7 * 4 + 3, 9 * 4, 9 * 4 + 1] and table == [[2, -1], [7, 9]]
     assert pos[:4] == [5, 6, 6, 7] and seen[3] == {0, 1, 3} and rows == [0] * 4 + [1] * 3
+
+
+def test_acceptance_of_planned_rows_refuses(nv):
+    """The form with what the plan took: the same checks, and shims that want the plan's tensor as it is."""
+    import ctypes
+    one = (ctypes.c_void_p * 1)(P)
+
+    def planned(tokens=P, taken=P, rows=2, nodes=8, row_bytes=256, counts=FAR, layers=1):
+        return nv.lib().mv_tree_accept_planned(tokens, P, P, P, P, taken, P, 8, 8, one, one, layers, row_bytes, 16, 20, rows, 9, nodes, 8, FAR, FAR + 4096,
+                                               counts, FAR + 12288, NULL)
+
+    for b in (dict(tokens=NULL), dict(counts=NULL), dict(rows=-1), dict(nodes=-1), dict(layers=-1), dict(row_bytes=0)):
+        assert planned(**b) == nv.MV_ERR_INVALID_ARG, b
+    assert planned(nodes=257) == nv.MV_ERR_UNSUPPORTED and planned(row_bytes=24) == nv.MV_ERR_UNSUPPORTED
+    assert planned(rows=0, tokens=NULL, taken=NULL) == nv.MV_OK
