@@ -282,7 +282,8 @@ def tree_accept(tokens: torch.Tensor, picks: torch.Tensor, row_start: torch.Tens
     max_path nodes (default: out's, else max_nodes).  With `caches` the keys and values of the path's j-th node are moved to index
     ctx_lens[b] + j of the sequence in every layer (places without a page: not moved), which is where a sequence of lens[b] tokens has
     them; all of it one launch for up to 64 layers.  A row without nodes has an empty path, and so has one that did not get its pages
-    (`taken`, the plan's, is negative): its nodes are stored nowhere, its length stays.  Without `taken` every row counts as stored."""
+    (`taken`, the plan's, is negative): its nodes are stored nowhere, its length stays.  Without `taken` every row counts as stored.  No output may share
+    memory with another or with an input."""
     n_tokens, rows, dev = tokens.shape[0], ctx_lens.shape[0], _current(tokens)
     assert max_nodes <= MAX_NODES, f"trees go up to {MAX_NODES} nodes a row"
     if out is None:
@@ -290,7 +291,6 @@ def tree_accept(tokens: torch.Tensor, picks: torch.Tensor, row_start: torch.Tens
     assert out.n_rows == rows and out.device == dev and (max_path is None or max_path == out.max_path), "out is of another step's sizes"
     path, ids, counts, lens = out._p
     ctx = _vec(ctx_lens, rows, dev)
-    assert lens != ctx or rows == 0, "the new lengths may not overwrite the old ones"
     if caches is None:
         move = (None, 0, 0, None, None, 0, 0, 0, 0)
     else:

@@ -118,6 +118,28 @@ inline bool rows_meet(const void* a, int64_t lda, int64_t wa, const void* b, int
     const int64_t in = (at % lda + lda) % lda;
     return in < wa || in + wb > lda;
 }
+// Whether `rows` rows of w bytes, ld apart from a on, share memory with the n bytes from p on (ld >= w; in between the rows they may lie).
+inline bool rows_meet_span(const void* a, int64_t ld, int64_t w, int64_t rows, const void* p, int64_t n) {
+    if (!a || !p || rows <= 0 || w <= 0 || n <= 0) return false;
+    const int64_t at = (int64_t)(reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(a)), row = at < w ? 0 : (at - w) / ld + 1;
+    return row < rows && row * ld < at + n;      // the first row that ends behind p
+}
+struct MemSpan {
+    const void* p;      // NULL: none
+    int64_t n;
+};
+inline bool spans_meet(const MemSpan& a, const MemSpan& b) { return rows_meet_span(a.p, a.n, a.n, 1, b.p, b.n); }
+// Whether any of `outs` shares memory with another of them or with any of `ins`
+template <int NO, int NI>
+inline bool outputs_meet(const MemSpan (&outs)[NO], const MemSpan (&ins)[NI]) {
+    for (int o = 0; o < NO; ++o) {
+        for (int i = 0; i < o; ++i)
+            if (spans_meet(outs[o], outs[i])) return true;
+        for (int i = 0; i < NI; ++i)
+            if (spans_meet(outs[o], ins[i])) return true;
+    }
+    return false;
+}
 int num_cus();  // compute units of the current device (cached)
 // Opt a kernel in to `lds` bytes of dynamic LDS (needed past 64 KiB) on the current device.
 // `done` is the caller's per-kernel record of what each device was last configured for.

@@ -537,7 +537,6 @@ int mv_tree_accept_planned(const int64_t* tokens, const int64_t* picks, const in
     if (max_nodes > kTreeNodes || max_path > kTreeNodes) return MV_ERR_UNSUPPORTED;
     if (rows == 0) return MV_OK;
     if (!row_start || !ctx_lens || !path || !ids || !counts || (n_tokens > 0 && (!tokens || !picks))) return MV_ERR_INVALID_ARG;
-    if (lens == ctx_lens || ids == tokens || ids == picks) return MV_ERR_INVALID_ARG;      // (other workgroups still read them)
     AcceptArgs a{tokens, picks, parents, row_start, ctx_lens, taken, block_table, bt_stride, bt_cols, rows, n_tokens, max_nodes, max_path, 0,
                  page, num_pages, 0, ids, path, counts, lens, {}};
     if (layers > 0) {
@@ -548,6 +547,13 @@ int mv_tree_accept_planned(const int64_t* tokens, const int64_t* picks, const in
             if (!k_caches[i] || !v_caches[i] || !aligned16(k_caches[i]) || !aligned16(v_caches[i])) return MV_ERR_INVALID_ARG;
         a.row_vecs = (int)(row_bytes / 16);
     }
+    // (workgroups and launches behind the first still read what the call takes while the outputs are written)
+    const int64_t r4 = (int64_t)rows * 4, n4 = (int64_t)n_tokens * 4;
+    const MemSpan outs[] = {{path, r4 * max_path}, {ids, 2 * r4 * max_path}, {counts, r4}, {lens, r4}};
+    const MemSpan ins[] = {{tokens, 2 * n4}, {picks, 2 * n4}, {parents, n4}, {row_start, r4 + 4}, {ctx_lens, r4}, {taken, r4}};
+    if (outputs_meet(outs, ins)) return MV_ERR_INVALID_ARG;
+    for (const MemSpan& o : outs)
+        if (layers > 0 && rows_meet_span(block_table, bt_stride * 4, (int64_t)bt_cols * 4, rows, o.p, o.n)) return MV_ERR_INVALID_ARG;
     for (int first = 0; first == 0 || first < layers; first += kAcceptLayers) {
         a.layers = layers - first < kAcceptLayers ? layers - first : kAcceptLayers;
         for (int i = 0; i < a.layers; ++i) {

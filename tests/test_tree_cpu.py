@@ -159,3 +159,41 @@ def test_acceptance_of_planned_rows_refuses(nv):
         assert planned(**b) == nv.MV_ERR_INVALID_ARG, b
     assert planned(nodes=257) == nv.MV_ERR_UNSUPPORTED and planned(row_bytes=24) == nv.MV_ERR_UNSUPPORTED
     assert planned(rows=0, tokens=NULL, taken=NULL) == nv.MV_OK
+
+
+def test_acceptance_refuses_outputs_over_what_it_reads_or_writes(nv):
+    """Every output on every input and every other output, whole, by its last or its first value; next to them it is no refusal: the entry gets as far as
+    the device, of which there is none here that takes these addresses."""
+    import ctypes
+    rows, n, path_len, cols, stride, K = 3, 9, 8, 5, 7, 1 << 12
+    sizes = {"tokens": 8 * n, "picks": 8 * n, "parents": 4 * n, "starts": 4 * rows + 4, "ctx": 4 * rows, "taken": 4 * rows,
+             "bt": 4 * ((rows - 1) * stride + cols), "path": 4 * rows * path_len, "ids": 8 * rows * path_len, "counts": 4 * rows, "lens": 4 * rows}
+    apart = {name: P + K * i for i, name in enumerate(sizes)}
+    outs = ("path", "ids", "counts", "lens")
+
+    def call(entry=None, **at):
+        a = {**apart, **at}
+        caches = (ctypes.c_void_p * 1)(FAR)
+        head = [a["tokens"], a["picks"], a["parents"], a["starts"], a["ctx"]]
+        tail = [a["bt"], stride, cols, caches, caches, 1, 256, 16, 20, rows, n, 8, path_len, a["path"], a["ids"], a["counts"], a["lens"], NULL]
+        L = nv.lib()
+        return L.mv_tree_accept(*head, *tail) if entry == "plain" else L.mv_tree_accept_planned(*head, a["taken"], *tail)
+
+    for o in outs:
+        for other in sizes:
+            if other == o:
+                continue
+            for at in (apart[other], apart[other] + sizes[other] - 4, apart[other] - sizes[o] + 4):
+                assert call(**{o: at}) == nv.MV_ERR_INVALID_ARG, (o, other)
+                if other != "taken":
+                    assert call("plain", **{o: at}) == nv.MV_ERR_INVALID_ARG, (o, other)
+    if torch.cuda.is_available():
+        return
+    assert call() not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK)
+    for o in outs:
+        for other in sizes:
+            if other != o:
+                for at in (apart[other] + sizes[other], apart[other] - sizes[o]):
+                    assert call(**{o: at}) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK), (o, other)
+    assert call(counts=apart["bt"] + 4 * cols, lens=apart["bt"] + 4 * (stride + cols)) == nv.MV_ERR_INVALID_ARG       # 3 values between rows 2 apart
+    assert call(lens=apart["bt"] + 4 * (stride * (rows - 1) + cols)) != nv.MV_ERR_INVALID_ARG
