@@ -964,7 +964,8 @@ int mv_layernorm_gather(const float* x, int64_t ldx, const int32_t* idx, const f
  * page size + place (-1 also where the page is not in [0, num_pages)), positions, row_of [tokens]; mask [tokens, words] (NULL:
  * none) = the node and its ancestors.  Without parents and mask rows may be of any length.  page * num_pages < 2^31.  Of tokens that no row has (in
  * front of row_start[0], behind row_start[rows], past max_nodes of a row) nothing is written, but that a slot of theirs that is not negative becomes
- * -1, whatever an earlier step left there: a store of all `tokens` stores the nodes.  rows == 0 writes nothing. */
+ * -1, whatever an earlier step left there: a store of all `tokens` stores the nodes.  rows == 0 writes nothing.  What is written, the table too, may share no memory
+ * with another output or with an input. */
 int mv_tree_plan(const int32_t* ctx_lens, const int32_t* row_start, const int32_t* parents, int32_t* block_table, int64_t bt_stride,
                  int bt_cols, const int32_t* free_pages, int n_free, int rows, int tokens, int max_nodes, int page, int num_pages,
                  int32_t* slots, int32_t* positions, int32_t* row_of, uint64_t* mask, int words, int32_t* taken, mv_stream_t stream);

@@ -101,7 +101,7 @@ def tree_plan(ctx_lens: torch.Tensor, row_start: torch.Tensor, block_table: torc
     -1, and -1 in the columns that its nodes would open, which may hold pages that are another row's by now).  parents int32 [tokens], None: a chain.  `tokens` (default: those of parents or out) is the number of
     tokens that the outputs hold, which may be more than the rows have: the others' slots are negative afterwards (-1 in place of what an earlier
     step left), so that a store of all of them stores the nodes, and the rest of their values is left alone.  `mask` (default: with
-    parents or out, what they have) says whether a mask is wanted."""
+    parents or out, what they have) says whether a mask is wanted.  Outputs and table may share no memory with each other or the inputs."""
     rows, dev = ctx_lens.shape[0], _current(ctx_lens)
     if out is None:
         if tokens is None:

@@ -475,6 +475,16 @@ int mv_tree_plan(const int32_t* ctx_lens, const int32_t* row_start, const int32_
     const int threads = tree && max_nodes <= 64 && rows <= 1024 ? 64 : 256;
     const int chunks = tree || max_nodes == 0 ? 1 : (max_nodes + threads - 1) / threads;
     if (chunks > 65535) return MV_ERR_UNSUPPORTED;
+    // (a row's workgroup reads the lengths of those before it, whose workgroups write)
+    const int64_t r4 = (int64_t)rows * 4, n4 = (int64_t)tokens * 4;
+    const MemSpan outs[] = {{slots, n4}, {positions, n4}, {row_of, n4}, {mask, 2 * n4 * words}, {taken, r4}};
+    const MemSpan ins[] = {{ctx_lens, r4}, {row_start, r4 + 4}, {parents, n4}, {free_pages, (int64_t)n_free * 4}};
+    if (outputs_meet(outs, ins)) return MV_ERR_INVALID_ARG;
+    auto in_table = [&](const MemSpan& s) { return rows_meet_span(block_table, bt_stride * 4, (int64_t)bt_cols * 4, rows, s.p, s.n); };
+    for (const MemSpan& s : outs)
+        if (in_table(s)) return MV_ERR_INVALID_ARG;
+    for (const MemSpan& s : ins)
+        if (in_table(s)) return MV_ERR_INVALID_ARG;
     hipLaunchKernelGGL(tree_plan_kernel, dim3((unsigned)rows, (unsigned)chunks), dim3((unsigned)threads), 0, (hipStream_t)stream, a);
     return check_launch();
 }

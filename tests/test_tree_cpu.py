@@ -197,3 +197,26 @@ def test_acceptance_refuses_outputs_over_what_it_reads_or_writes(nv):
                     assert call(**{o: at}) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK), (o, other)
     assert call(counts=apart["bt"] + 4 * cols, lens=apart["bt"] + 4 * (stride + cols)) == nv.MV_ERR_INVALID_ARG       # 3 values between rows 2 apart
     assert call(lens=apart["bt"] + 4 * (stride * (rows - 1) + cols)) != nv.MV_ERR_INVALID_ARG
+
+
+def test_plan_refuses_outputs_over_what_it_reads_or_writes(nv):
+    rows, n, cols, stride, n_free, words, K = 3, 9, 5, 7, 6, 2, 1 << 12
+    sizes = {"ctx": 4 * rows, "starts": 4 * rows + 4, "parents": 4 * n, "free": 4 * n_free, "bt": 4 * ((rows - 1) * stride + cols), "slots": 4 * n,
+             "pos": 4 * n, "row": 4 * n, "mask": 8 * n * words, "taken": 4 * rows}
+    apart = {name: P + K * i for i, name in enumerate(sizes)}
+    ins = ("ctx", "starts", "parents", "free")
+    call = lambda **at: plan(nv, stride=stride, cols=cols, n_free=n_free, rows=rows, tokens=n, words=words, **{**apart, **at})      # noqa: E731
+    for o in sizes:
+        for other in sizes:
+            if other == o or (o in ins and other in ins):
+                continue
+            for at in (apart[other], apart[other] + sizes[other] - 4, apart[other] - sizes[o] + 4):
+                assert call(**{o: at}) == nv.MV_ERR_INVALID_ARG, (o, other)
+    if torch.cuda.is_available():
+        return
+    assert call() not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK)
+    for o in sizes:
+        for other in sizes:
+            if other != o:
+                for at in (apart[other] + sizes[other], apart[other] - sizes[o]):
+                    assert call(**{o: at}) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK), (o, other)
