@@ -984,7 +984,7 @@ int mv_qkv_norm_rotary_slots(const void* qkv, int64_t ld, const float* q_norm, c
  * whose keys and values are in the cache [num_pages, page, hkv, d].  q [tokens, ldq], out [tokens, ldo], caches bf16 or (f32) fp32, all 16-byte
  * aligned; d 64 or 128, hq / hkv <= 8, page a power of two >= 16, page * bt_cols <= 2^30.  A node that sees nothing: zeros.  Places whose
  * page is not in [0, num_pages) and keys behind column bt_cols do not count; q . k * scale below 2^30 in size (fp32 scores, and the
- * difference to the row's largest is formed from their rounded products).  scale > 0.  out may not share memory with q.  num_splits
+ * difference to the row's largest is formed from their rounded products).  scale > 0.  out and workspace may share no memory with each other or with an input.  num_splits
  * (1 .. 64) pieces of the keys side by side; rows < 2^16, rows * hkv * num_splits < 2^19.  workspace: of
  * mv_tree_attn_workspace_bytes, 16-byte aligned, needs no clearing, of one running call at a time. */
 size_t mv_tree_attn_workspace_bytes(int tokens, int hq, int d, int num_splits);

@@ -1315,6 +1315,16 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
         return MV_ERR_WORKSPACE;
     const int64_t bytes = f32 ? 4 : 2;
     if (rows_meet(q, ldq * bytes, hq * d * bytes, out, ldo * bytes, hq * d * bytes, tokens)) return MV_ERR_INVALID_ARG;
+    // neither the output nor the partial sums may lie over what other workgroups still read (the table as from its first to its last column)
+    const int64_t row = hq * d * bytes, pool = (int64_t)num_pages * page * hkv * d * bytes;
+    const MemSpan part[] = {{num_splits > 1 ? workspace : nullptr, (int64_t)mv_tree_attn_workspace_bytes(tokens, hq, d, num_splits)}};
+    const MemSpan ins[] = {{k_cache, pool}, {v_cache, pool}, {ctx_lens, (int64_t)rows * 4}, {row_start, (int64_t)rows * 4 + 4},
+                           {mask, (int64_t)tokens * words * 8}, {block_table, ((rows - 1) * bt_stride + bt_cols) * 4}};
+    if (outputs_meet(part, ins) || rows_meet_span(q, ldq * bytes, row, tokens, part[0].p, part[0].n) ||
+        rows_meet_span(out, ldo * bytes, row, tokens, part[0].p, part[0].n))
+        return MV_ERR_INVALID_ARG;
+    for (const MemSpan& s : ins)
+        if (rows_meet_span(out, ldo * bytes, row, tokens, s.p, s.n)) return MV_ERR_INVALID_ARG;
     TreeArgs a;
     a.q = q;
     a.k_cache = k_cache;

@@ -220,3 +220,37 @@ def test_plan_refuses_outputs_over_what_it_reads_or_writes(nv):
             if other != o:
                 for at in (apart[other] + sizes[other], apart[other] - sizes[o]):
                     assert call(**{o: at}) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK), (o, other)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+def test_attention_refuses_out_and_workspace_over_what_it_reads(nv, f32):
+    rows, n, hq, hkv, d, page, pages, cols, stride, words, splits, K = 3, 9, 8, 4, 64, 16, 5, 6, 9, 2, 3, 1 << 19
+    size = 4 if f32 else 2
+    need = nv.lib().mv_tree_attn_workspace_bytes(n, hq, d, splits)
+    pool = pages * page * hkv * d * size
+    ld = hq * d + 32                                         # rows of q and out with room behind each
+    span = ((n - 1) * ld + hq * d) * size
+    sizes = {"q": span, "k": pool, "v": pool, "ctx": 4 * rows, "starts": 4 * rows + 4, "bt": 4 * ((rows - 1) * stride + cols), "mask": 8 * n * words,
+             "out": span, "ws": need}
+    assert max(sizes.values()) < K // 2
+    apart = {name: FAR + K * i + K // 2 for i, name in enumerate(sizes)}
+    call = lambda **at: attn(nv, ldq=ld, ldo=ld, stride=stride, cols=cols, words=words, ws_bytes=need, rows=rows, tokens=n, hq=hq, hkv=hkv, d=d, page=page,      # noqa: E731
+                             pages=pages, splits=splits, f32=f32, **{**apart, **at})
+    even = lambda x: x // 16 * 16                            # noqa: E731  (out and workspace are 16-byte aligned)
+    for o in ("out", "ws"):
+        for other in sizes:
+            if other != o:
+                for at in (apart[other], even(apart[other] + sizes[other] - 1), even(apart[other] - sizes[o] + 16)):
+                    assert call(**{o: at}) == nv.MV_ERR_INVALID_ARG, (o, other, at - apart[other])
+    if torch.cuda.is_available():
+        return
+    assert call() not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK)
+    for o in ("out", "ws"):
+        for other in sizes:
+            if other != o:
+                for at in (even(apart[other] + sizes[other] + 15), even(apart[other] - sizes[o])):
+                    assert call(**{o: at}) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK), (o, other)
+    # one cache for keys and values is read alone, and rows of out in the room behind those of q are no overlap
+    assert call(v=apart["k"]) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK)
+    wide = dict(ldq=2 * hq * d, ldo=2 * hq * d)
+    assert attn(nv, q=FAR, out=FAR + hq * d * size, hq=hq, hkv=hkv, d=d, f32=f32, **wide) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK)
