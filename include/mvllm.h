@@ -974,7 +974,7 @@ int mv_tree_plan(const int32_t* ctx_lens, const int32_t* row_start, const int32_
  * itself (q_norm / k_norm fp32 [d]; NULL: none), then the rotation of its first `rot` dimensions by positions[t] * inv_freq[i] (fp64
  * [rot / 2]; adjacent pairs, or i with i + rot / 2); q to q_out [tokens, ldq], k and v to the caches' slot slots[t] (outside
  * [0, cache_slots): not stored), bf16 or (dst_f32, from fp32 rows only) fp32.  fp32 throughout, rounded once.  q_out may be
- * q's part of qkv where the types agree, and may share no other memory with it. */
+ * q's part of qkv where the types agree; beyond that what is written (q_out, each cache) may share no memory with the rest or with an input. */
 int mv_qkv_norm_rotary_slots(const void* qkv, int64_t ld, const float* q_norm, const float* k_norm, float eps, const double* inv_freq,
                              int rot, int adjacent, const int32_t* positions, const int32_t* slots, void* q_out, int64_t ldq,
                              void* k_cache, void* v_cache, int64_t cache_slots, int tokens, int heads, int kv_heads, int d, int src_f32,

@@ -151,7 +151,8 @@ def qkv_norm_rotary_slots(qkv: torch.Tensor, positions: torch.Tensor, slots: tor
     2 * inv_freq.numel() dimensions are turned by positions[t] * inv_freq (float64; None: no rotation; `adjacent` pairs (2i, 2i + 1), else i
     with i + half), all of it in fp32 and rounded once.  q goes to out [tokens, heads, d], k and v to k_cache / v_cache
     [pages, page, kv_heads, d] at slots[t] (negative or past the last page: not stored; no two tokens may name one slot).  qkv bf16 with bf16
-    caches, float32 with either; out has the caches' type and may be q's own part of qkv where the types agree, no other part of it."""
+    caches, float32 with either; out has the caches' type and may be q's own part of qkv where the types agree; apart from that out, k_cache and v_cache may share no
+    memory with each other or an input."""
     dev = _current(qkv)
     pages, page, kv_heads, d = _cache(k_cache, v_cache, dev)
     (tokens, width), src, dst = qkv.shape, qkv.dtype, k_cache.dtype

@@ -504,6 +504,17 @@ int mv_qkv_norm_rotary_slots(const void* qkv, int64_t ld, const float* q_norm, c
     if (!(q_out == qkv && ld * sb == ldq * db && sb == db) &&
         rows_meet(qkv, ld * sb, (int64_t)(heads + 2 * kv_heads) * d * sb, q_out, ldq * db, (int64_t)heads * d * db, tokens))
         return MV_ERR_INVALID_ARG;
+    // nor may the caches, which tokens in any order write, meet each other, q's place or what is read
+    const int64_t pool = cache_slots * kv_heads * d * db, t4 = (int64_t)tokens * 4;
+    const MemSpan outs[] = {{k_cache, pool}, {v_cache, pool}};
+    const MemSpan ins[] = {{positions, t4}, {slots, t4}, {q_norm, d * 4}, {k_norm, d * 4}, {rot > 0 ? inv_freq : nullptr, rot * 4}};
+    if (outputs_meet(outs, ins)) return MV_ERR_INVALID_ARG;
+    for (const MemSpan& s : outs)
+        if (rows_meet_span(qkv, ld * sb, (int64_t)(heads + 2 * kv_heads) * d * sb, tokens, s.p, s.n) ||
+            rows_meet_span(q_out, ldq * db, (int64_t)heads * d * db, tokens, s.p, s.n))
+            return MV_ERR_INVALID_ARG;
+    for (const MemSpan& s : ins)
+        if (rows_meet_span(q_out, ldq * db, (int64_t)heads * d * db, tokens, s.p, s.n)) return MV_ERR_INVALID_ARG;
     SlotStoreArgs a{qkv, ld, q_norm, k_norm, eps, inv_freq, rot, adjacent, positions, slots, q_out, ldq, k_cache, v_cache, tokens, heads,
                     kv_heads, d, cache_slots};
     hipStream_t s = (hipStream_t)stream;

@@ -254,3 +254,30 @@ def test_attention_refuses_out_and_workspace_over_what_it_reads(nv, f32):
     assert call(v=apart["k"]) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK)
     wide = dict(ldq=2 * hq * d, ldo=2 * hq * d)
     assert attn(nv, q=FAR, out=FAR + hq * d * size, hq=hq, hkv=hkv, d=d, f32=f32, **wide) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK)
+
+
+@pytest.mark.parametrize("src,dst", [(0, 0), (1, 0), (1, 1)])
+def test_store_refuses_caches_and_q_over_what_it_reads_or_writes(nv, src, dst):
+    n, hq, hkv, d, rot, slots, K = 9, 8, 4, 64, 32, 50, 1 << 19
+    sb, db, ld, ldq = (4 if src else 2), (4 if dst else 2), (hq + 2 * hkv) * d + 16, hq * d + 16
+    pool = slots * hkv * d * db
+    sizes = {"qkv": ((n - 1) * ld + (hq + 2 * hkv) * d) * sb, "qn": 4 * d, "kn": 4 * d, "freq": 4 * rot, "pos": 4 * n, "slots": 4 * n,
+             "out": ((n - 1) * ldq + hq * d) * db, "k": pool, "v": pool}
+    apart = {name: FAR + K * i + K // 2 for i, name in enumerate(sizes)}
+    outs = ("out", "k", "v")
+    call = lambda ldq=ldq, **at: store(nv, ld=ld, ldq=ldq, rot=rot, n=slots, tokens=n, hq=hq, hkv=hkv, d=d, src=src, dst=dst, **{**apart, **at})      # noqa: E731
+    for o in outs:
+        for other in sizes:
+            if other != o:
+                for at in (apart[other], apart[other] + sizes[other] - 2, apart[other] - sizes[o] + 2):
+                    assert call(**{o: at}) == nv.MV_ERR_INVALID_ARG, (o, other, at - apart[other])
+    if torch.cuda.is_available():
+        return
+    assert call() not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK)
+    for o in outs:
+        for other in sizes:
+            if other != o:
+                for at in (apart[other] + sizes[other], apart[other] - sizes[o]):
+                    assert call(**{o: at}) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK), (o, other)
+    if sb == db:                                              # q over its own part of the rows
+        assert call(out=apart["qkv"], ldq=ld) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK)
