@@ -998,7 +998,7 @@ int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_
 /* The walk from node 0 to the lowest later node whose parent is the current one and whose token is picks[current], and so on, up to max_path
  * nodes: path [rows, max_path] (-1 behind its end), ids [rows, max_path] = the picks along it (-1), counts [rows], lens [rows] = ctx_lens +
  * counts (NULL: not wanted).  No output may share memory with another or with anything that the call reads.  layers > 0: then keys and values (row_bytes a token, a multiple of 16, in each of the
- * layers' caches; the addresses are host arrays) at index ctx_lens + path[j] of the sequence go to index ctx_lens + j; places without a page:
+ * layers' caches; the addresses are host arrays, each cache named once) at index ctx_lens + path[j] of the sequence go to index ctx_lens + j; places without a page:
  * not.  One launch per 64 layers.  Every row must have got its pages. */
 int mv_tree_accept(const int64_t* tokens, const int64_t* picks, const int32_t* parents, const int32_t* row_start, const int32_t* ctx_lens,
                    const int32_t* block_table, int64_t bt_stride, int bt_cols, void* const* k_caches, void* const* v_caches, int layers,

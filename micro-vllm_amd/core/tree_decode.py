@@ -227,9 +227,16 @@ def tree_attn_workspace(tokens: int, rows: int, max_nodes: int, heads: int, kv_h
     return L.mv_tree_attn_workspace_bytes(tokens, heads, d, splits)
 
 
+def _apart(addresses, nbytes: int) -> bool:
+    """Whether pieces of nbytes at these addresses share nothing."""
+    at = sorted(addresses)
+    return all(b - a >= nbytes for a, b in zip(at, at[1:]))
+
+
 class TreeCaches:
     """The key and value caches of a model's layers for `tree_accept`: [layers, pages, page, kv_heads, d] each, or lists of
-    [pages, page, kv_heads, d] (KVCacheManager.k_caches / .v_caches).  Holds the tensors and their addresses."""
+    [pages, page, kv_heads, d] (KVCacheManager.k_caches / .v_caches), no two of which share memory (a cache that layers share is named once: named twice, its tokens would be
+    moved twice).  Holds the tensors and their addresses."""
 
     def __init__(self, k_caches, v_caches):
         k, v = list(k_caches), list(v_caches)
@@ -241,6 +248,7 @@ class TreeCaches:
             assert _cache(a, b, self.device) == k[0].shape and a.dtype is k[0].dtype, "the layers' caches are of one shape and type"
         self.row_bytes = kv_heads * d * k[0].element_size()
         assert self.row_bytes % 16 == 0 and all(t.data_ptr() % 16 == 0 for t in k + v), "a token's keys must be whole 16-byte pieces"
+        assert _apart([t.data_ptr() for t in k + v], k[0].numel() * k[0].element_size()), "every cache is named once, and none lies in another"
         self.layers = len(k)
         self._tensors = (k, v)
         self.k = (ctypes.c_void_p * len(k))(*[t.data_ptr() for t in k])

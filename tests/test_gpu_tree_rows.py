@@ -250,3 +250,14 @@ def test_a_recorded_step_whose_row_is_refused_and_comes_again(ops):
         assert got.counts.tolist() == ([6, 9] if turn else [6, 0]) and got.lens.tolist() == ([16, 25] if turn else [16, 48])
         if turn == 0:
             assert torch.equal(k[0, 1:7], begin[1][0, 1:7]) and torch.equal(k[0, 8:], begin[1][0, 8:])      # pages 0 and 7 are row 0's
+
+
+def test_caches_that_layers_share_are_named_once(ops):
+    """A path of 0, 2, 5 moved twice in one cache would leave node 5 where node 2 belongs: refused."""
+    k, v = (torch.zeros(3, 4, 16, 2, 64, dtype=BF16, device=DEV) for _ in range(2))
+    ops.TreeCaches(k, v)
+    ops.TreeCaches([k[2], k[0]], [v[2], v[0]])
+    flat = k.view(-1, 16, 2, 64)                                     # twelve pages: caches of four that overlap
+    for a, b in (([k[0], k[0]], [v[0], v[1]]), ([k[0]], [k[0]]), ([k[0], k[1]], [v[0], k[0]]), ([flat[0:4], flat[2:6]], [v[0], v[1]])):
+        with pytest.raises(AssertionError):
+            ops.TreeCaches(a, b)

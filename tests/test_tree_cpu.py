@@ -281,3 +281,9 @@ def test_store_refuses_caches_and_q_over_what_it_reads_or_writes(nv, src, dst):
                     assert call(**{o: at}) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK), (o, other)
     if sb == db:                                              # q over its own part of the rows
         assert call(out=apart["qkv"], ldq=ld) not in (nv.MV_ERR_INVALID_ARG, nv.MV_OK)
+
+
+def test_caches_are_named_once(nv):
+    from micro_vllm_amd.core.tree_decode import _apart
+    assert _apart([], 64) and _apart([128], 64) and _apart([256, 0, 64, 192, 128], 64)
+    assert not _apart([64, 128, 64], 64) and not _apart([0, 100, 48], 64)
