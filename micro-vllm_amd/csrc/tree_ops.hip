@@ -62,6 +62,7 @@ __global__ __launch_bounds__(256) void tree_plan_kernel(PlanArgs a) {
     const TreeRow row = tree_row(a.row_start, b, a.tokens, a.max_nodes);
     const int64_t ctx = max(a.ctx[b], 0);
     const PageNeed own = page_need(a, b);
+    const int first = max(a.row_start[0], 0), last = max(a.row_start[a.rows], 0);
 
     int64_t before = 0;
     for (int i = tid; i < b; i += nt) before += page_need(a, i).need();
@@ -82,16 +83,7 @@ __global__ __launch_bounds__(256) void tree_plan_kernel(PlanArgs a) {
         for (int64_t j = own.held + tid; j < end; j += nt) table[j] = refused ? -1 : a.free_pages[before + j - own.held];
     }
 
-    const auto none = [&](int64_t t, int64_t end, int64_t step) {
-        for (; t < end; t += step)
-            if (a.slots[t] >= 0) a.slots[t] = -1;
-    };
-    const int i = blockIdx.y * nt + tid, wide = gridDim.y * nt;
-    const int64_t nth = (int64_t)b * wide + i, all = (int64_t)gridDim.x * wide;
-    none(nth, min(max(a.row_start[0], 0), a.tokens), all);
-    none((int64_t)row.start + row.n + i, row.end, wide);
-    none((int64_t)max(a.row_start[a.rows], 0) + nth, a.tokens, all);
-
+    const int i = blockIdx.y * nt + tid;
     int depth = i;
     if (a.mask || a.parents) {       // one chunk holds the row
         int up = -1;
@@ -132,6 +124,17 @@ __global__ __launch_bounds__(256) void tree_plan_kernel(PlanArgs a) {
             for (int w = 0; w < kTreeWords; ++w)
                 if (w < a.words) a.mask[(int64_t)(row.start + i) * a.words + w] = bits[w];
         }
+    }
+    if (first > 0 || row.start + row.n < row.end || last < a.tokens) {
+        const auto none = [&](int64_t t, int64_t end, int64_t step) {
+            for (; t < end; t += step)
+                if (a.slots[t] >= 0) a.slots[t] = -1;
+        };
+        const int wide = gridDim.y * nt;
+        const int64_t nth = (int64_t)b * wide + i, all = (int64_t)gridDim.x * wide;
+        none(nth, min(first, a.tokens), all);
+        none((int64_t)row.start + row.n + i, row.end, wide);
+        none(last + nth, a.tokens, all);
     }
     if (i >= row.n) return;
     const int64_t at = ctx + i, col = at / a.page;
