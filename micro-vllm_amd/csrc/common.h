@@ -121,14 +121,19 @@ inline bool rows_meet(const void* a, int64_t lda, int64_t wa, const void* b, int
 // Whether `rows` rows of w bytes, ld apart from a on, share memory with the n bytes from p on (ld >= w; in between the rows they may lie).
 inline bool rows_meet_span(const void* a, int64_t ld, int64_t w, int64_t rows, const void* p, int64_t n) {
     if (!a || !p || rows <= 0 || w <= 0 || n <= 0) return false;
-    const int64_t at = (int64_t)(reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(a)), row = at < w ? 0 : (at - w) / ld + 1;
-    return row < rows && row * ld < at + n;      // the first row that ends behind p
+    const int64_t at = (int64_t)(reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(a));
+    if (at + n <= 0 || at >= (rows - 1) * ld + w) return false;
+    const int64_t row = at < w ? 0 : (at - w) / ld + 1;      // the first that ends behind p
+    return row * ld < at + n;
 }
 struct MemSpan {
     const void* p;      // NULL: none
     int64_t n;
 };
-inline bool spans_meet(const MemSpan& a, const MemSpan& b) { return rows_meet_span(a.p, a.n, a.n, 1, b.p, b.n); }
+inline bool spans_meet(const MemSpan& a, const MemSpan& b) {
+    const int64_t at = (int64_t)(reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p));
+    return a.p && b.p && a.n > 0 && b.n > 0 && at < a.n && at + b.n > 0;
+}
 // Whether any of `outs` shares memory with another of them or with any of `ins`
 template <int NO, int NI>
 inline bool outputs_meet(const MemSpan (&outs)[NO], const MemSpan (&ins)[NI]) {
