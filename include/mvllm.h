@@ -988,7 +988,8 @@ int mv_qkv_norm_rotary_slots(const void* qkv, int64_t ld, const float* q_norm, c
  * (1 .. 64) pieces of the keys side by side; rows < 2^16, rows * hkv * num_splits < 2^19.  workspace: of
  * mv_tree_attn_workspace_bytes, 16-byte aligned, needs no clearing, of one running call at a time. */
 size_t mv_tree_attn_workspace_bytes(int tokens, int hq, int d, int num_splits);
-/* How many pieces a step should be given (max_keys: the longest row there may be). */
+/* How many pieces a step should be given (max_keys: page * bt_cols of the call, by which its kernel is picked too: give no more columns than the rows
+ * may want). */
 int mv_tree_attn_pick_splits(int rows, int max_nodes, int hq, int hkv, int d, int max_keys, int f32);
 int mv_tree_attn(const void* q, int64_t ldq, const void* k_cache, const void* v_cache, const int32_t* ctx_lens, const int32_t* row_start,
                  const int32_t* block_table, int64_t bt_stride, int bt_cols, const uint64_t* mask, int words, void* out, int64_t ldo,

@@ -396,8 +396,9 @@ __global__ __launch_bounds__(256, 2) void tree_attn_f32_kernel(TreeArgs a) {
 //   S^T = K . Q^T   v_mfma_f32_16x16x32_bf16, operand A = key rows as they lie in memory (lane (r, q): row r, dimensions 32 k + 8 q ..);
 //   O^T = V^T . P^T operand B = P as S^T left it, rounded to bf16 (keys 4 q + j and 16 + 4 q + j), operand A through the wave's own piece of
 //                   LDS with the transposing read, which delivers those keys.
-// The normaliser sums the unrounded weights; rounding a weight to bf16 (2^-8 of it) is what the matrix instruction asks for, and half of what
-// the rounding of the output costs anyway.  The next block's keys and values are requested into the registers that this one leaves.
+// The normaliser sums the unrounded weights; rounding a weight to bf16 (2^-8 of it) is what the matrix instruction asks for: results are
+// 2.0 to 2.3e-3 of their size off 64 bits, where weights in 32 bits give 1.65e-3, the output's rounding alone.  The next block's keys and values are
+// requested into the registers that this one leaves.
 // Keys as the operand wants them are sixteen rows a quarter wave, which a compute unit's address path serves at a third of the rate of whole rows;
 // for 16 rows of heads of 128, where registers allow, they are read row by row and turned in LDS as well, and the next block's requests go out in front
 // of the first product: 8 heads of 128 on 1, 7 nodes, 45 keys 7.5 -> 6.4 us, 900 in one piece 15.6 -> 13.7.  (Heads of 64 are a piece's latency
@@ -1208,7 +1209,8 @@ __global__ __launch_bounds__(256) void tree_attn_merge_kernel(TreeArgs a) {
     }
 }
 
-// Which kernel a launch takes, with rows, workgroups and keys of its workgroups.
+// Which kernel a launch takes, with rows, workgroups and keys of its workgroups.  max_keys is what the table has room for: nothing is read back, and a table of
+// more columns than the rows want costs a short row up to twice its time (the shim's caller can pass fewer columns).
 // Where few workgroups have short rows, latency counts: a workgroup of 16 stacked rows is the quickest through its keys, and as many of them as the chip
 // has units ask for the same keys again out of L2.  Past `reach` (workgroups times keys) that traffic is what they take, and a workgroup takes more rows:
 // 32, then 64 (heads of 64), then the wide form.  In us, 16 rows a workgroup, 32, wide, each with the splits that it gets:
@@ -1250,8 +1252,11 @@ static TreeForm tree_form(int rows, int max_nodes, int hkv, int g, int d, int f3
     f.whole |= f.deep;
     f.round_keys = f.wide || f32 ? 64 : 32 * f.waves;
     // Work for one workgroup a unit, or for two where there are two without any cut (wide, us with one and two: 32 uneven rows of 256 to 8191, 64
-    // nodes of 8B heads 203, 199; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4;
-    // fp32 of much work, 4 rows of 6000, 64 nodes, 16 heads of 64 on 4 84, 76, of less one row of 3000, 16 nodes 12.9, 14.4, heads of 128 16.5, 19.5)
+    // nodes of 8B heads 203, 199; 16 nodes 151, 159; one row of 8191, 64 nodes 29.4, 33.5; 16 rows of 4000, 32 nodes 63.7, 70.4).  fp32 by workgroups times
+    // keys, us with one and two: under 100000 one is quicker (16 nodes of 16 heads of 64 on 4, one row of 3000 12.9, 14.6, two 15.4, 15.9; of 8 heads of 128 14.1, 16.0
+    // and 18.8, 20.8); from there to 200000 either (three rows 21.6, 18.4, four 19.5, 20; four of 8 heads of 128 25.2, 26.6); above it two by up to a quarter, one by 7 % in
+    // some (24 rows of 240 to 4000, 16 nodes, 8 heads of 64 52, 46, of 128 133, 100; 4 of 4000, 24 nodes, 16 heads of 128 on 8 77, 65; 8 of 3000, 16 nodes, 8 heads of 64
+    // 23.5, 23.9, of 128 39, 41; 16 of 480 to 8000, 4 nodes, 32 heads of 64 on 8 61, 69)
     const bool two = f.wide ? heads * f.row_blocks >= 2 * num_cus()
                             : f32 && (d == 64 || f.row_tiles == 1) && heads * f.row_blocks * max_keys >= 200000;
     f.per_unit = two ? 2 : 1;

@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256) void slot_store_any_kernel(SlotStoreArgs a) {
 // The forms of a head that are read as they lie: d / 8 = LPH lanes of eight values, whole pieces of the rotated part.  Workgroup = (token, some of its
 // heads): it forms the angles' sines and cosines once, for all of them, and leaves them with the weights in LDS; a lane asks for its own eight
 // values and (pairs half a head apart) for its partners', which a neighbour has too, out of L1: no exchange.  Bound by memory: 2048 tokens of 32 + 2 x 8
-// heads of 128 in bf16, 50 MB, 13 us (3.9 TB/s; a wave per head and value by value 39).
+// heads of 128 in bf16, 50 MB, 14 us (3.6 TB/s; a wave per head and value by value 39).
 template <bool F32>
 __device__ __forceinline__ void ld8(const void* base, int64_t at, float (&v)[8]) {
     if constexpr (F32) {
